@@ -79,6 +79,8 @@ class FcoseLevelStruct(ctypes.Structure):
     _fields_ = [("cls", c_void_p), ("ctr", c_void_p), ("reg", c_void_p), ("ext", c_void_p),
                 ("locations", c_void_p), ("hw", c_int), ("stride", c_float)]
 
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2          # DANCE_F32 / DANCE_F16 / DANCE_BF16
+ACT_NONE, ACT_RELU, ACT_SILU = 0, 1, 2              # DANCE_ACT_*
 
 P = c_void_p
 # name -> (restype, argtypes); every symbol include/dance_hip.h declares
@@ -97,6 +99,11 @@ SIGNATURES = {
     "dance_conv1x1_nhwc": (c_int, [P, P, P, P, c_int, c_int, c_int, c_int, c_int, P]),
     "dance_conv3x3_16_partial_floats": (c_int64, [c_int, c_int, c_int, c_int, c_int]),
     "dance_gn_relu": (c_int, [P, P, P, P, c_float, c_int, P, P, P, P, c_int, c_int, c_int, c_int, P]),
+    "dance_group_norm_workspace_bytes": (c_int64, [c_int, c_int, c_int64, c_int, c_int, c_int]),
+    "dance_group_norm_act": (c_int, [P, c_int64, c_int64, c_int, P, P, c_int, c_float, c_int, c_int, P, P, P, c_int64,
+                                     c_int, c_int, c_int64, P]),
+    "dance_group_norm_act_backward": (c_int, [P, c_int64, c_int64, P, c_int64, c_int64, c_int, P, P, c_int, c_int, c_int,
+                                              P, P, P, P, P, c_int64, c_int, c_int, c_int64, P]),
     "dance_nms_sorted": (c_int, [P, c_int, c_float, P, P, P, P]),
     "dance_nms_sorted_plain": (c_int, [P, c_int, c_float, P, P, P, P]),
     "dance_nms_sorted_plain_static": (c_int, [P, c_int, c_float, P, P, P]),

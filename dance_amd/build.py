@@ -46,6 +46,7 @@ SOURCES = [
     ("head16.hip", []),
     ("fuse16w.hip", []),
     ("featprep16.hip", []),
+    ("groupnorm.hip", []),
     ("raster.hip", ["-ffp-contract=off"]),
     ("attender.hip", []),
     ("fcose.hip", ["-ffp-contract=off"]),

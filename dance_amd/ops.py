@@ -9,8 +9,8 @@ import os
 
 import torch
 
-from ._lib import (ABSMAX_OF_FEATURES, ABSMAX_OF_GN_RELU, ABSMAX_OF_LAYOUT, ABSMAX_WORDS, check, current_stream,
-                   lib, ptr)
+from ._lib import (ACT_NONE, ACT_RELU, ACT_SILU, ABSMAX_OF_FEATURES, ABSMAX_OF_GN_RELU, ABSMAX_OF_LAYOUT, ABSMAX_WORDS, DTYPE_BF16,
+                   DTYPE_F16, DTYPE_F32, check, current_stream, lib, ptr)
 
 POLY_RAW, POLY_BOX, POLY_QUAD, POLY_OCTAGON = 0, 1, 2, 3
 PAD_ZEROS, PAD_REFLECTION = 0, 1
@@ -492,6 +492,129 @@ def conv1x1_nhwc(x, weight, bias=None):
         check(lib().dance_conv1x1_nhwc(ptr(x), ptr(wt), ptr(bs), ptr(out), b, h, w, c, k, current_stream()),
               "conv1x1_nhwc")
     return out
+
+
+# -------------------------------------------------------------- group norm + activation
+DTYPE_CODES = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
+ACTIVATIONS = {None: ACT_NONE, "none": ACT_NONE, "relu": ACT_RELU, "silu": ACT_SILU}
+
+
+def _channels_last_strides(t):
+    """(image stride, pixel stride) in elements of a (B, C, *spatial) tensor whose channels are adjacent in
+    memory and whose pixels are evenly spaced, or None."""
+    if t.size(1) > 1 and t.stride(1) != 1:
+        return None
+    pixel, expect = None, None                       # innermost spatial dimension first
+    for size, stride in zip(reversed(t.shape[2:]), reversed(t.stride()[2:])):
+        if size == 1:
+            continue
+        if pixel is None:
+            pixel = stride
+        elif stride != expect:
+            return None
+        expect = stride * size
+    return (t.stride(0) if t.size(0) > 1 else 0), (t.size(1) if pixel is None else pixel)
+
+
+def _nhwc_view(t):
+    """t itself when the kernels can walk its memory, else a dense channels-last copy."""
+    strides = _channels_last_strides(t)
+    if strides is None:
+        t = t.movedim(1, -1).contiguous().movedim(-1, 1)
+        strides = _channels_last_strides(t)
+    return (t,) + strides
+
+
+def _empty_nhwc(shape, dtype, device):
+    return torch.empty((shape[0],) + tuple(shape[2:]) + (shape[1],), dtype=dtype, device=device).movedim(-1, 1)
+
+
+def _group_norm_forward(x, groups, weight, bias, eps, act):
+    """-> (y, the map as it was read, stats (B, groups, 2) f64)"""
+    b, c = x.shape[:2]
+    hw = math.prod(x.shape[2:])
+    x, image, pixel = _nhwc_view(x)
+    y = _empty_nhwc(x.shape, x.dtype, x.device)
+    stats = torch.empty((b, groups, 2), dtype=torch.float64, device=x.device)
+    dt, affine = DTYPE_CODES[x.dtype], weight if weight is not None else bias
+    at = DTYPE_F32 if affine is None else DTYPE_CODES[affine.dtype]
+    nbytes = lib().dance_group_norm_workspace_bytes(b, c, hw, groups, dt, 0)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+        check(lib().dance_group_norm_act(ptr(x), image, pixel, dt, ptr(weight), ptr(bias), at, eps, act, groups, ptr(y),
+                                         ptr(stats), ptr(ws), nbytes, b, c, hw, current_stream()), "group_norm_act")
+    return y, x, stats
+
+
+class _GroupNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act):
+        y, x, stats = _group_norm_forward(x, groups, weight, bias, eps, act)
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.groups, ctx.act = groups, act
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, stats = ctx.saved_tensors
+        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        b, c = x.shape[:2]
+        hw = math.prod(x.shape[2:])
+        dx = _empty_nhwc(x.shape, x.dtype, x.device) if want_x else None
+        dw = torch.empty_like(weight) if want_w else None
+        db = torch.empty_like(bias) if want_b else None
+        if b == 0 or hw == 0:                        # empty sums
+            return dx, dw if dw is None else dw.zero_(), db if db is None else db.zero_(), None, None, None
+        dy, dy_image, dy_pixel = _nhwc_view(dy)
+        image, pixel = _channels_last_strides(x)
+        dt, affine = DTYPE_CODES[x.dtype], weight if weight is not None else bias
+        at = DTYPE_F32 if affine is None else DTYPE_CODES[affine.dtype]
+        nbytes = lib().dance_group_norm_workspace_bytes(b, c, hw, ctx.groups, dt, 1)
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=x.device)
+        with torch.cuda.device(x.device):
+            check(lib().dance_group_norm_act_backward(ptr(dy), dy_image, dy_pixel, ptr(x), image, pixel, dt, ptr(weight),
+                                                      ptr(bias), at, ctx.act, ctx.groups, ptr(stats), ptr(dx), ptr(dw),
+                                                      ptr(db), ptr(ws), nbytes, b, c, hw, current_stream()),
+                  "group_norm_act backward")
+        return dx, dw, db, None, None, None
+
+
+def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="relu"):
+    """act(F.group_norm(x, num_groups, weight, bias, eps)) on a channels-last map, differentiable once in x,
+    weight and bias.
+
+    x (B, C, *spatial) fp32 / fp16 / bf16 with adjacent channels (torch.channels_last memory, a channel slice
+    of it, or a (B, C) matrix); a map whose pixels are not evenly spaced (a crop) is copied first, a
+    channels-first map is refused.  weight, bias (C) of one type, or None; act None, "relu" or "silu".  The
+    statistics cover the whole map as F.group_norm's do, in fp64.  Returns y of x's type, channels last."""
+    _need_gpu(x, weight, bias)
+    if x.dim() < 2:
+        raise RuntimeError("group_norm_act: (B, C, *spatial) expected, got %d dimension(s)" % x.dim())
+    if x.dtype not in DTYPE_CODES:
+        raise RuntimeError("group_norm_act: fp32, fp16 or bf16 expected, got %s" % x.dtype)
+    if act not in ACTIVATIONS:
+        raise RuntimeError("group_norm_act: act is None, \"relu\" or \"silu\", got %r" % (act,))
+    c = x.size(1)
+    if c > 1 and x.numel() and x.stride(1) != 1:
+        raise RuntimeError("group_norm_act: a channels-last map expected (channels adjacent in memory), got strides %s"
+                           % (tuple(x.stride()),))
+    if num_groups < 1 or c < 1 or c % num_groups:
+        raise RuntimeError("group_norm_act: %d channels do not divide into %d groups" % (c, num_groups))
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if tuple(t.shape) != (c,) or t.dtype not in DTYPE_CODES or t.device != x.device:
+            raise RuntimeError("group_norm_act: %s must be (%d,) fp32, fp16 or bf16 on %s, got %s %s on %s"
+                               % (name, c, x.device, tuple(t.shape), t.dtype, t.device))
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise RuntimeError("group_norm_act: weight and bias differ in type (%s, %s)" % (weight.dtype, bias.dtype))
+    if not eps >= 0:
+        raise RuntimeError("group_norm_act: eps must not be negative, got %r" % (eps,))
+    weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _GroupNormAct.apply(x, weight, bias, int(num_groups), float(eps), ACTIVATIONS[act])
+    return _group_norm_forward(x, int(num_groups), weight, bias, float(eps), ACTIVATIONS[act])[0]
 
 
 # ---------------------------------------------------------------------------- attender
