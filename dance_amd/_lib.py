@@ -3,6 +3,7 @@
 There is NO fallback: if the shared object is missing or a symbol is absent, importing
 `lib()` raises.  The product path never routes through torch ops or the oracle.
 """
+import contextlib
 import ctypes
 import os
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
@@ -102,8 +103,9 @@ SIGNATURES = {
     "dance_group_norm_workspace_bytes": (c_int64, [c_int, c_int, c_int64, c_int, c_int, c_int]),
     "dance_group_norm_act": (c_int, [P, c_int64, c_int64, c_int, P, P, c_int, c_float, c_int, c_int, P, P, P, c_int64,
                                      c_int, c_int, c_int64, P]),
-    "dance_group_norm_act_backward": (c_int, [P, c_int64, c_int64, P, c_int64, c_int64, c_int, P, P, c_int, c_int, c_int,
-                                              P, P, P, P, P, c_int64, c_int, c_int, c_int64, P]),
+    "dance_group_norm_act_backward": (c_int, [P, c_int64, c_int64, P, c_int64, c_int64, c_int, c_int, c_int, c_int, P,
+                                              P, P, P, P, c_int64, c_int, c_int, c_int64, P]),
+    "dance_group_norm_saved_bytes": (c_int64, [c_int, c_int, c_int]),
     "dance_nms_sorted": (c_int, [P, c_int, c_float, P, P, P, P]),
     "dance_nms_sorted_plain": (c_int, [P, c_int, c_float, P, P, P, P]),
     "dance_nms_sorted_plain_static": (c_int, [P, c_int, c_float, P, P, P]),
@@ -206,3 +208,20 @@ def current_stream():
     import torch
 
     return torch.cuda.current_stream().cuda_stream
+
+
+_ON_CURRENT = contextlib.nullcontext()
+
+
+def on_device(device):
+    """`with torch.cuda.device(device)`, at no cost when it is the current one already."""
+    import torch
+
+    return _ON_CURRENT if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def stream_of(device):
+    """Handle of the device's current stream, without the Stream object current_stream() builds."""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(device.index)

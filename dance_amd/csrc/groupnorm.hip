@@ -45,286 +45,531 @@ __device__ __forceinline__ void store_affine(void *p, int dtype, int i, double v
         ((__bf16 *)p)[i] = (__bf16)(float)v;
 }
 
+constexpr int MAX_THREADS = 512;        // of a workgroup: 256 registers a thread, no pass spills
+
+// What a workgroup covers: a slab of whole groups' channels, a chunk of an image's pixels.
 struct GnDims {
     long long hw, chunk;        // pixels of an image; pixels of a workgroup
-    int c, cv, rows;            // channels; vectors of a pixel; pixels a workgroup covers at once
-    int groups, gc, nch;        // groups; channels of one; workgroups of an image
+    int c, groups, gc, nch;     // channels and groups of the map; channels of a group; workgroups along the pixels
+    int cs, cv, rows;           // channels of a slab; its vectors; pixels a workgroup covers at once
 };
 
-// the channel that element j of vector v holds.  WHOLE (c a multiple of the vector): 16 consecutive bytes;
+// the channel of the slab that element j of vector v holds.  WHOLE (whole vectors): 16 consecutive bytes;
 // otherwise element j of the whole row of vectors, so that a wave's scalar accesses are consecutive
 template <typename T, bool WHOLE> __device__ __forceinline__ int channel_of(const GnDims &d, int v, int j)
 {
     return WHOLE ? v * Vec<T>::N + j : v + j * d.cv;
 }
 
+// pixel: the slab's first channel
 template <typename T, bool WHOLE>
-__device__ __forceinline__ void load_vec(float (&r)[Vec<T>::N], const T *pixel, const GnDims &d, int v)
+__device__ __forceinline__ Word<T> load_word(const T *pixel, const GnDims &d, int v)
 {
-    if (WHOLE) {
-        const Word<T> w = *reinterpret_cast<const Word<T> *>(pixel + v * Vec<T>::N);
+    if (WHOLE)
+        return *reinterpret_cast<const Word<T> *>(pixel + v * Vec<T>::N);
+    Word<T> w;
 #pragma unroll
-        for (int j = 0; j < Vec<T>::N; ++j)
-            r[j] = (float)w.v[j];
-    } else {
-#pragma unroll
-        for (int j = 0; j < Vec<T>::N; ++j) {
-            const int ch = v + j * d.cv;
-            r[j] = ch < d.c ? (float)pixel[ch] : 0.0f;
-        }
+    for (int j = 0; j < Vec<T>::N; ++j) {
+        const int ch = v + j * d.cv;
+        w.v[j] = ch < d.cs ? pixel[ch] : (T)0.0f;
     }
+    return w;
 }
 
 template <typename T, bool WHOLE>
-__device__ __forceinline__ void store_vec(T *pixel, const float (&r)[Vec<T>::N], const GnDims &d, int v)
+__device__ __forceinline__ void store_word(T *pixel, const Word<T> &w, const GnDims &d, int v)
 {
     if (WHOLE) {
-        Word<T> w;
-#pragma unroll
-        for (int j = 0; j < Vec<T>::N; ++j)
-            w.v[j] = (T)r[j];
         *reinterpret_cast<Word<T> *>(pixel + v * Vec<T>::N) = w;
-    } else {
+        return;
+    }
 #pragma unroll
-        for (int j = 0; j < Vec<T>::N; ++j) {
-            const int ch = v + j * d.cv;
-            if (ch < d.c)
-                pixel[ch] = (T)r[j];
+    for (int j = 0; j < Vec<T>::N; ++j) {
+        const int ch = v + j * d.cv;
+        if (ch < d.cs)
+            pixel[ch] = w.v[j];
+    }
+}
+
+// ------------------------------------------------------------------- sums inside a workgroup
+// red [rows][units] pairs -> red [0][units], a fixed order: a unit is folded by `lanes` neighbouring threads
+// (a power of two up to a wave), rows lane, lane + lanes, ... each, then a butterfly over them
+template <typename A> __device__ __forceinline__ void fold_rows(A (*red)[2], int rows, int units)
+{
+    int lanes = 64;
+    while (lanes > 1 && (lanes * units > (int)blockDim.x || lanes >= 2 * rows))
+        lanes >>= 1;
+    __syncthreads();
+    if (rows == 1)
+        return;
+    const int lane = threadIdx.x & (lanes - 1), step = blockDim.x / lanes;
+    for (int u0 = 0; u0 < units; u0 += step) {
+        const int u = u0 + threadIdx.x / lanes;
+        A s = 0, q = 0;
+        if (u < units)
+            for (int r = lane; r < rows; r += lanes) {
+                s += red[r * units + u][0];
+                q += red[r * units + u][1];
+            }
+        for (int m = lanes >> 1; m >= 1; m >>= 1) {
+            s += __shfl_xor(s, m, 64);
+            q += __shfl_xor(q, m, 64);
         }
+        // row 0 of a unit is read by its own lanes alone, and they have read it
+        if (u < units && lane == 0) {
+            red[u][0] = s;
+            red[u][1] = q;
+        }
+    }
+    __syncthreads();
+}
+
+// f(group, sum of its `per` units' pairs) for every group of the slab, red [units]; f runs in one thread a group
+template <typename A, typename F>
+__device__ __forceinline__ void for_group_sums(const A (*red)[2], int groups, int per, F &&f)
+{
+    int lanes = 64;
+    while (lanes > 1 && (lanes * groups > (int)blockDim.x || lanes >= 2 * per))
+        lanes >>= 1;
+    const int lane = threadIdx.x & (lanes - 1), step = blockDim.x / lanes;
+    for (int g0 = 0; g0 < groups; g0 += step) {
+        const int g = g0 + threadIdx.x / lanes;
+        A s = 0, q = 0;
+        if (g < groups)
+            for (int k = lane; k < per; k += lanes) {
+                s += red[g * per + k][0];
+                q += red[g * per + k][1];
+            }
+        for (int m = lanes >> 1; m >= 1; m >>= 1) {
+            s += __shfl_xor(s, m, 64);
+            q += __shfl_xor(q, m, 64);
+        }
+        if (g < groups && lane == 0)
+            f(g, s, q);
     }
 }
 
 // ------------------------------------------------------------------------------------- statistics
-// Sum and sum of squares of a chunk of pixels, per group, both in fp64: the difference that makes the
-// variance then loses nothing at any mean / spread ratio fp32 inputs can hold.
-// partial (b, nch, groups, 2).  grid: b * nch workgroups.
-template <typename T, bool WHOLE>
-__global__ __launch_bounds__(1024) void k_gn_stats(const T *__restrict__ x, long long image_stride,
-                                                   long long pixel_stride, double *__restrict__ partial, GnDims d)
+// Sum and sum of squares in fp64: the difference that makes the variance then loses nothing at any mean /
+// spread ratio fp32 inputs can hold.  An fp64 fma is as fast as an fp32 one here; the pass stays bound by
+// its loads.
+template <typename T> __device__ __forceinline__ void add_word(double (&s)[Vec<T>::N], double (&q)[Vec<T>::N], const Word<T> &w)
 {
-    constexpr int N = Vec<T>::N;
-    extern __shared__ double red[];                       // [rows][cv * N][2]
-    const int b = blockIdx.x / d.nch, ch = blockIdx.x - b * d.nch;
-    const int row = threadIdx.x / d.cv, v = threadIdx.x - row * d.cv;
-    const long long p0 = ch * d.chunk, p1 = min(p0 + d.chunk, d.hw);
-    double s[N], q[N];
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-        s[j] = q[j] = 0.0;
-    if (row < d.rows) {
-        const T *xp = x + b * image_stride;
-#pragma unroll 4
-        for (long long p = p0 + row; p < p1; p += d.rows) {
-            float r[N];
-            load_vec<T, WHOLE>(r, xp + p * pixel_stride, d, v);
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                s[j] += (double)r[j];
-                q[j] = fma((double)r[j], (double)r[j], q[j]);
-            }
-        }
-    }
-    const int width = d.cv * N;
-    if (row < d.rows)
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            double *e = red + ((long long)row * width + channel_of<T, WHOLE>(d, v, j)) * 2;
-            e[0] = s[j];
-            e[1] = q[j];
-        }
-    __syncthreads();
-    for (int n = d.rows; n > 1;) {                        // fold the rows onto row 0
-        const int h = (n + 1) / 2;
-        for (int i = threadIdx.x; i < (n - h) * width * 2; i += blockDim.x)
-            red[i] += red[i + h * width * 2];
-        __syncthreads();
-        n = h;
-    }
-    for (int g = threadIdx.x; g < d.groups; g += blockDim.x) {
-        double sg = 0.0, qg = 0.0;
-        for (int k = 0; k < d.gc; ++k) {
-            sg += red[(g * d.gc + k) * 2];
-            qg += red[(g * d.gc + k) * 2 + 1];
-        }
-        double *o = partial + ((long long)blockIdx.x * d.groups + g) * 2;
-        o[0] = sg;
-        o[1] = qg;
+    for (int j = 0; j < Vec<T>::N; ++j) {
+        const double x = (double)(float)w.v[j];
+        s[j] += x;
+        q[j] = fma(x, x, q[j]);
     }
 }
 
-// partial (b, nch, groups, 2) -> stats (b, groups, 2) = mean, rstd.  grid: (groups, b), one wave each.
-__global__ __launch_bounds__(64) void k_gn_finish(const double *__restrict__ partial, double *__restrict__ stats,
-                                                  int groups, int nch, double count, double eps)
+// A thread's sums into red [rows][units].  A unit is a channel, or a whole vector where no vector holds two
+// groups (gc a multiple of it): an eighth or a quarter of the LDS and of the folding.
+template <typename T, bool WHOLE> __device__ __forceinline__ bool vector_units(const GnDims &d)
 {
+    return WHOLE && d.gc % Vec<T>::N == 0;
+}
+
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void put_units(double (*red)[2], const double (&s)[Vec<T>::N], const double (&q)[Vec<T>::N],
+                                          const GnDims &d, int row, int v)
+{
+    constexpr int N = Vec<T>::N;
+    if (vector_units<T, WHOLE>(d)) {
+        double ss = 0.0, qq = 0.0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            ss += s[j];
+            qq += q[j];
+        }
+        red[row * d.cv + v][0] = ss;
+        red[row * d.cv + v][1] = qq;
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int u = row * d.cv * N + channel_of<T, WHOLE>(d, v, j);
+            red[u][0] = s[j];
+            red[u][1] = q[j];
+        }
+    }
+}
+
+__device__ __forceinline__ void finish_group(double s, double q, double count, double eps, double &mean, double &rstd)
+{
+    mean = s / count;
+    double var = q / count - mean * mean;
+    var = var < 0.0 ? 0.0 : var;                          // (a NaN stays one: infinities in the map give NaN, as in torch)
+    rstd = 1.0 / sqrt(var + eps);
+}
+
+// Vectors of a thread that are loaded at once; a vector of scalar loads counts for several
+template <bool WHOLE> constexpr int IN_FLIGHT = WHOLE ? 8 : 2;
+
+// FL pixels of a thread from pixel p on, rows apart; those past the chunk are its last one again, so that
+// every load is issued
+template <typename T, bool WHOLE, int FL>
+__device__ __forceinline__ void load_batch(Word<T> (&w)[FL], const T *x, long long pixel_stride, long long p, long long p1,
+                                           const GnDims &d, int v)
+{
+    if (p + (FL - 1) * d.rows < p1) {
+        const T *xp = x + p * pixel_stride;
+        const long long step = d.rows * pixel_stride;
+#pragma unroll
+        for (int u = 0; u < FL; ++u)
+            w[u] = load_word<T, WHOLE>(xp + u * step, d, v);
+    } else {
+#pragma unroll
+        for (int u = 0; u < FL; ++u)
+            w[u] = load_word<T, WHOLE>(x + min(p + u * d.rows, p1 - 1) * pixel_stride, d, v);
+    }
+}
+
+// f(u) for the pixels p + u rows of a batch that lie in the chunk
+template <int FL, typename F> __device__ __forceinline__ void for_batch(long long p, long long p1, int rows, F &&f)
+{
+    if (p + (FL - 1) * rows < p1) {
+#pragma unroll
+        for (int u = 0; u < FL; ++u)
+            f(u);
+    } else {
+#pragma unroll
+        for (int u = 0; u < FL; ++u)
+            if (p + u * rows < p1)
+                f(u);
+    }
+}
+
+// partial (b, nch, groups, 2): sums of a chunk of pixels.  grid: b * nch workgroups, slab = the whole map.
+template <typename T, bool WHOLE>
+__global__ __launch_bounds__(MAX_THREADS) void k_gn_stats(const T *__restrict__ x, long long image_stride,
+                                                   long long pixel_stride, double *__restrict__ partial, GnDims d)
+{
+    constexpr int N = Vec<T>::N, FL = IN_FLIGHT<WHOLE>;
+    extern __shared__ __align__(16) double red[][2];
+    const int b = blockIdx.x / d.nch, ch = blockIdx.x - b * d.nch;
+    const int row = threadIdx.x / d.cv, v = threadIdx.x - row * d.cv;
+    const long long p0 = ch * d.chunk, p1 = min(p0 + d.chunk, d.hw);
+    if (row < d.rows) {
+        double s[N] = {}, q[N] = {};
+        const T *xp = x + b * image_stride;
+        Word<T> w[FL], next[FL];
+        long long p = p0 + row;
+        load_batch<T, WHOLE>(w, xp, pixel_stride, p, p1, d, v);
+        for (; p < p1; p += FL * d.rows) {
+            if (p + FL * d.rows < p1)
+                load_batch<T, WHOLE>(next, xp, pixel_stride, p + FL * d.rows, p1, d, v);
+            for_batch<FL>(p, p1, d.rows, [&](int u) { add_word<T>(s, q, w[u]); });
+#pragma unroll
+            for (int u = 0; u < FL; ++u)
+                w[u] = next[u];
+        }
+        put_units<T, WHOLE>(red, s, q, d, row, v);
+    }
+    const bool vu = vector_units<T, WHOLE>(d);
+    fold_rows(red, d.rows, vu ? d.cv : d.cv * N);
+    double *out = partial + (long long)blockIdx.x * d.groups * 2;
+    for_group_sums(red, d.groups, vu ? d.gc / N : d.gc, [&](int g, double s, double q) {
+        out[g * 2] = s;
+        out[g * 2 + 1] = q;
+    });
+}
+
+// ----------------------------------------------------------------------------- a channel's constants
+// The mean as a sum of two floats: x - mu keeps its low bits when the mean is large against the spread.  With
+// e = x - mu:  z = e (rstd w) + beta.  Written once an image and channel (by k_gn_finish or k_gn_one), read
+// as one 16-byte word: gathering mean, rstd, weight and bias of each of its channels cost a thread of the
+// apply pass two dozen dependent loads, 8 us of its 17 on a (1, 256, 200, 304) bf16 map.
+struct alignas(16) Channel {
+    float mhi, mlo, rw, beta;
+};
+
+// What the forward call leaves for the backward one, in this order: the groups' mean and rstd, the channels'
+// constants, the weight as fp32.
+struct Saved {
+    double *stats;              // (b, groups, 2)
+    Channel *channels;          // (b, c)
+    float *weight;              // (c)
+};
+
+__host__ __device__ inline Saved saved_at(void *p, int b, int c, int groups)
+{
+    Saved s;
+    s.stats = (double *)p;
+    s.channels = (Channel *)(s.stats + (size_t)b * groups * 2);
+    s.weight = (float *)(s.channels + (size_t)b * c);
+    return s;
+}
+
+__device__ __forceinline__ Channel channel_constants(double mean, double rstd, float weight, float beta)
+{
+    Channel k;
+    k.mhi = (float)mean;
+    k.mlo = (float)(mean - (double)k.mhi);
+    k.rw = (float)(rstd * (double)weight);
+    k.beta = beta;
+    return k;
+}
+
+__device__ __forceinline__ float centred(float x, const Channel &k) { return (x - k.mhi) - k.mlo; }
+
+// partial (b, nch, groups, 2) -> the saved words of a group and its channels.  grid: (groups, b).
+__global__ __launch_bounds__(256) void k_gn_finish(const double *__restrict__ partial, Saved out, const void *weight,
+                                                   const void *bias, int affine_dtype, double count, double eps, GnDims d)
+{
+    __shared__ double red[4][2];
     const int g = blockIdx.x, b = blockIdx.y;
     double s = 0.0, q = 0.0;
-    for (int i = threadIdx.x; i < nch; i += 64) {
-        const double *p = partial + (((long long)b * nch + i) * groups + g) * 2;
-        s += p[0];
-        q += p[1];
+#pragma unroll 4
+    for (int i = threadIdx.x; i < d.nch; i += 256) {
+        const double2 p = *reinterpret_cast<const double2 *>(partial + (((long long)b * d.nch + i) * d.groups + g) * 2);
+        s += p.x;
+        q += p.y;
+    }
+    // (the affine parameters arrive meanwhile)
+    int cl = threadIdx.x;
+    float w = 1.0f, beta = 0.0f;
+    if (cl < d.gc) {
+        w = load_affine(weight, affine_dtype, g * d.gc + cl, 1.0f);
+        beta = load_affine(bias, affine_dtype, g * d.gc + cl, 0.0f);
     }
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) {
         s += __shfl_xor(s, m, 64);
         q += __shfl_xor(q, m, 64);
     }
+    if ((threadIdx.x & 63) == 0) {
+        red[threadIdx.x >> 6][0] = s;
+        red[threadIdx.x >> 6][1] = q;
+    }
+    __syncthreads();
+    double mean, rstd;
+    finish_group(red[0][0] + red[1][0] + red[2][0] + red[3][0], red[0][1] + red[1][1] + red[2][1] + red[3][1], count, eps,
+                 mean, rstd);
     if (threadIdx.x == 0) {
-        const double mean = s / count;
-        double var = q / count - mean * mean;
-        var = var < 0.0 ? 0.0 : var;                      // (a NaN stays one: infinities in the map give NaN, as in torch)
-        stats[((long long)b * groups + g) * 2] = mean;
-        stats[((long long)b * groups + g) * 2 + 1] = 1.0 / sqrt(var + eps);
+        double *o = out.stats + ((long long)b * d.groups + g) * 2;
+        o[0] = mean;
+        o[1] = rstd;
+    }
+    while (cl < d.gc) {
+        const int c = g * d.gc + cl;
+        out.channels[(long long)b * d.c + c] = channel_constants(mean, rstd, w, beta);
+        if (b == 0)
+            out.weight[c] = w;
+        cl += 256;
+        if (cl < d.gc) {
+            w = load_affine(weight, affine_dtype, g * d.gc + cl, 1.0f);
+            beta = load_affine(bias, affine_dtype, g * d.gc + cl, 0.0f);
+        }
     }
 }
 
 // ------------------------------------------------------------------------------------------ apply
-// A channel's constants.  The mean as a sum of two floats: x - mu keeps its low bits when the mean is large
-// against the spread.
-struct Channel {
-    float mhi, mlo, rstd, w, beta;
-};
-
-__device__ __forceinline__ Channel channel_constants(const double *stats, const void *weight, const void *bias,
-                                                     int affine_dtype, const GnDims &d, int b, int ch)
-{
-    Channel k = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (ch < d.c) {
-        const double *st = stats + ((long long)b * d.groups + ch / d.gc) * 2;
-        k.mhi = (float)st[0];
-        k.mlo = (float)(st[0] - (double)k.mhi);
-        k.rstd = (float)st[1];
-        k.w = load_affine(weight, affine_dtype, ch, 1.0f);
-        k.beta = load_affine(bias, affine_dtype, ch, 0.0f);
-    }
-    return k;
-}
-
-__device__ __forceinline__ float normalised(float x, const Channel &k) { return ((x - k.mhi) - k.mlo) * k.rstd; }
-
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
 
-template <int ACT> __device__ __forceinline__ float activate(float z)
+__device__ __forceinline__ float activate(float z, int act)
 {
-    if (ACT == DANCE_ACT_RELU)
+    if (act == DANCE_ACT_RELU)
         return z > 0.0f ? z : (z != z ? z : 0.0f);
-    if (ACT == DANCE_ACT_SILU)
+    if (act == DANCE_ACT_SILU)
         return z * sigmoid(z);
     return z;
 }
 
-// grid: b * nch workgroups
-template <typename T, bool WHOLE, int ACT>
-__global__ __launch_bounds__(1024) void k_gn_apply(const T *__restrict__ x, long long image_stride,
-                                                   long long pixel_stride, const double *__restrict__ stats,
-                                                   const void *weight, const void *bias, int affine_dtype,
-                                                   T *__restrict__ y, GnDims d)
+template <typename T> __device__ __forceinline__ Word<T> apply_word(const Word<T> &w, const Channel (&k)[Vec<T>::N], int act)
 {
-    constexpr int N = Vec<T>::N;
+    Word<T> r;
+#pragma unroll
+    for (int j = 0; j < Vec<T>::N; ++j)
+        r.v[j] = (T)activate(fmaf(centred((float)w.v[j], k[j]), k[j].rw, k[j].beta), act);
+    return r;
+}
+
+// grid: b * nch workgroups, slab = the whole map
+template <typename T, bool WHOLE, int ACT>
+__global__ __launch_bounds__(MAX_THREADS) void k_gn_apply(const T *__restrict__ x, long long image_stride,
+                                                          long long pixel_stride, const Channel *__restrict__ channels,
+                                                          T *__restrict__ y, GnDims d)
+{
+    constexpr int N = Vec<T>::N, FL = IN_FLIGHT<WHOLE>;
     const int b = blockIdx.x / d.nch, ch = blockIdx.x - b * d.nch;
     const int row = threadIdx.x / d.cv, v = threadIdx.x - row * d.cv;
     if (row >= d.rows)
         return;
-    Channel k[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-        k[j] = channel_constants(stats, weight, bias, affine_dtype, d, b, channel_of<T, WHOLE>(d, v, j));
     const long long p0 = ch * d.chunk, p1 = min(p0 + d.chunk, d.hw);
     const T *xp = x + b * image_stride;
     T *yp = y + b * d.hw * d.c;
-#pragma unroll 4
-    for (long long p = p0 + row; p < p1; p += d.rows) {
-        float r[N];
-        load_vec<T, WHOLE>(r, xp + p * pixel_stride, d, v);
+    Word<T> w[FL], next[FL];
+    long long p = p0 + row;
+    load_batch<T, WHOLE>(w, xp, pixel_stride, p, p1, d, v);        // in flight while the constants arrive
+    Channel k[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-            r[j] = activate<ACT>(fmaf(normalised(r[j], k[j]), k[j].w, k[j].beta));
-        store_vec<T, WHOLE>(yp + p * d.c, r, d, v);
+    for (int j = 0; j < N; ++j)
+        k[j] = channels[(long long)b * d.c + min(channel_of<T, WHOLE>(d, v, j), d.c - 1)];
+    const long long step = (long long)d.rows * d.c;
+    for (; p < p1; p += FL * d.rows) {
+        if (p + FL * d.rows < p1)
+            load_batch<T, WHOLE>(next, xp, pixel_stride, p + FL * d.rows, p1, d, v);
+        T *yq = yp + p * d.c;
+        for_batch<FL>(p, p1, d.rows, [&](int u) { store_word<T, WHOLE>(yq + u * step, apply_word<T>(w[u], k, ACT), d, v); });
+#pragma unroll
+        for (int u = 0; u < FL; ++u)
+            w[u] = next[u];
     }
 }
 
-// --------------------------------------------------------------------------------------- backward
-// dz = dy act'(z) and xh of one element.  ReLU: which side of zero z lies on decides whole gradients, so a
-// z within fp32 rounding of zero is evaluated again in fp64 (the rounding of z is a few 2^-24 of its two
-// terms; 2^-20 of them covers it, one element in a million takes the branch).
-template <int ACT>
-__device__ __forceinline__ float grad_z(float dy, float x, const Channel &k, const double *st, float &xh)
+// Small maps: a workgroup owns a slab of whole groups of an image over all its pixels, at most U vectors a
+// thread, and keeps them in registers: one read, one launch.  grid: b * slabs.
+template <typename T, bool WHOLE, int U>
+__global__ __launch_bounds__(MAX_THREADS) void k_gn_one(const T *__restrict__ x, long long image_stride, long long pixel_stride,
+                                                 const void *weight, const void *bias, int affine_dtype, double eps,
+                                                 int act, T *__restrict__ y, Saved out, GnDims d)
 {
-    xh = normalised(x, k);
-    if (ACT == DANCE_ACT_NONE)
+    constexpr int N = Vec<T>::N;
+    extern __shared__ __align__(16) double red[][2];
+    const int slabs = d.c / d.cs, b = blockIdx.x / slabs, c0 = (blockIdx.x - b * slabs) * d.cs;
+    const int row = threadIdx.x / d.cv, v = threadIdx.x - row * d.cv;
+    const bool live = row < d.rows;
+    const T *xp = x + b * image_stride + c0;
+    Word<T> w[U];
+    double s[N] = {}, q[N] = {};
+    if (live) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            w[u] = load_word<T, WHOLE>(xp + min((long long)(row + u * d.rows), d.hw - 1) * pixel_stride, d, v);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (row + u * d.rows < d.hw)
+                add_word<T>(s, q, w[u]);
+        put_units<T, WHOLE>(red, s, q, d, row, v);
+    }
+    const bool vu = vector_units<T, WHOLE>(d);
+    const int units = vu ? d.cv : d.cv * N, sg = d.cs / d.gc;
+    fold_rows(red, d.rows, units);
+    const double (*sums)[2] = red;
+    double (*done)[2] = red + units;                      // behind row 0, whose sums are still read
+    Channel *constants = reinterpret_cast<Channel *>(done + sg);
+    double *st = out.stats + ((long long)b * d.groups + c0 / d.gc) * 2;
+    for_group_sums(sums, sg, vu ? d.gc / N : d.gc, [&](int g, double gs, double gq) {
+        finish_group(gs, gq, (double)d.gc * (double)d.hw, eps, done[g][0], done[g][1]);
+        st[g * 2] = done[g][0];
+        st[g * 2 + 1] = done[g][1];
+    });
+    __syncthreads();
+    for (int cl = threadIdx.x; cl < d.cs; cl += blockDim.x) {
+        const float wt = load_affine(weight, affine_dtype, c0 + cl, 1.0f);
+        const Channel k = channel_constants(done[cl / d.gc][0], done[cl / d.gc][1], wt,
+                                            load_affine(bias, affine_dtype, c0 + cl, 0.0f));
+        constants[cl] = k;
+        out.channels[(long long)b * d.c + c0 + cl] = k;
+        if (b == 0)
+            out.weight[c0 + cl] = wt;
+    }
+    __syncthreads();
+    if (!live)
+        return;
+    Channel k[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+        k[j] = constants[min(channel_of<T, WHOLE>(d, v, j), d.cs - 1)];
+    T *yp = y + b * d.hw * d.c + c0;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (row + u * d.rows < d.hw)
+            store_word<T, WHOLE>(yp + (long long)(row + u * d.rows) * d.c, apply_word<T>(w[u], k, act), d, v);
+}
+
+// --------------------------------------------------------------------------------------- backward
+// dz = dy act'(z) and e = x - mu of one element.  ReLU: which side of zero z lies on decides whole gradients,
+// so a z within fp32 rounding of zero is evaluated again in fp64 (the rounding of z is a few 2^-24 of its two
+// terms; 2^-20 of them covers it, one element in a million takes the branch).  st: the group's mean and rstd,
+// weight: the channel's, read there only.
+__device__ __forceinline__ float grad_z(float dy, float x, const Channel &k, const double *st, const float *weight, int act,
+                                        float &e)
+{
+    e = centred(x, k);
+    if (act == DANCE_ACT_NONE)
         return dy;
-    const float t = xh * k.w, z = t + k.beta;
-    if (ACT == DANCE_ACT_RELU) {
+    const float t = e * k.rw, z = t + k.beta;
+    if (act == DANCE_ACT_RELU) {
         bool on = z > 0.0f;
         if (fabsf(z) <= 9.5367431640625e-7f * (fabsf(t) + fabsf(k.beta)))
-            on = ((double)x - st[0]) * st[1] * (double)k.w + (double)k.beta > 0.0;
+            on = ((double)x - st[0]) * st[1] * (double)*weight + (double)k.beta > 0.0;
         return on ? dy : (z != z ? z : 0.0f);
     }
     const float s = sigmoid(z);
     return dy * (s * (1.0f + z * (1.0f - s)));
 }
 
-// Per-channel sums of dz and dz xh over a chunk of pixels: partial (b, nch, c, 2) fp32.  grid: b * nch.
-template <typename T, bool WHOLE, int ACT>
-__global__ __launch_bounds__(1024) void k_gn_grad_sums(const T *__restrict__ dy, long long dy_image, long long dy_pixel,
-                                                       const T *__restrict__ x, long long image_stride,
-                                                       long long pixel_stride, const double *__restrict__ stats,
-                                                       const void *weight, const void *bias, int affine_dtype,
-                                                       float *__restrict__ partial, GnDims d)
+// dx = rstd (w dz - m1 - xh m2) = dz (rstd w) - a1 - e a2,  a1 = rstd m1,  a2 = rstd^2 m2
+__device__ __forceinline__ float grad_x(float dz, float e, const Channel &k, float2 a)
 {
-    constexpr int N = Vec<T>::N;
-    extern __shared__ float redf[];                       // [rows][cv * N][2]
+    return fmaf(dz, k.rw, -fmaf(e, a.y, a.x));
+}
+
+template <bool WHOLE> constexpr int GRAD_IN_FLIGHT = WHOLE ? 4 : 1;       // of each of the two maps
+
+// Per-channel sums of dz and dz xh over a chunk of pixels: partial (b, nch, c, 2) fp32, a thread's own sums
+// of at most chunk / rows terms.  grid: b * nch, slab = the whole map.
+template <typename T, bool WHOLE, int ACT>
+__global__ __launch_bounds__(MAX_THREADS) void k_gn_grad_sums(const T *__restrict__ dy, long long dy_image,
+                                                              long long dy_pixel, const T *__restrict__ x,
+                                                              long long image_stride, long long pixel_stride, Saved saved,
+                                                              float *__restrict__ partial, GnDims d)
+{
+    constexpr int N = Vec<T>::N, FL = GRAD_IN_FLIGHT<WHOLE>;
+    extern __shared__ __align__(16) float redf[][2];
     const int b = blockIdx.x / d.nch, ch = blockIdx.x - b * d.nch;
     const int row = threadIdx.x / d.cv, v = threadIdx.x - row * d.cv;
-    const int width = d.cv * N;
+    const int units = d.cv * N;
+    const double *st = saved.stats + (long long)b * d.groups * 2;
     if (row < d.rows) {
+        const long long p0 = ch * d.chunk, p1 = min(p0 + d.chunk, d.hw);
+        const T *xp = x + b * image_stride, *dp = dy + b * dy_image;
+        Word<T> w[FL], g[FL];
+        long long p = p0 + row;
+        load_batch<T, WHOLE>(w, xp, pixel_stride, p, p1, d, v);
+        load_batch<T, WHOLE>(g, dp, dy_pixel, p, p1, d, v);
         Channel k[N];
-        const double *st[N];
         float s[N], q[N];
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const int c = channel_of<T, WHOLE>(d, v, j);
-            k[j] = channel_constants(stats, weight, bias, affine_dtype, d, b, c);
-            st[j] = stats + ((long long)b * d.groups + min(c, d.c - 1) / d.gc) * 2;
+            k[j] = saved.channels[(long long)b * d.c + min(channel_of<T, WHOLE>(d, v, j), d.c - 1)];
             s[j] = q[j] = 0.0f;
         }
-        const long long p0 = ch * d.chunk, p1 = min(p0 + d.chunk, d.hw);
-        const T *xp = x + b * image_stride, *dp = dy + b * dy_image;
-#pragma unroll 2
-        for (long long p = p0 + row; p < p1; p += d.rows) {
-            float r[N], g[N];
-            load_vec<T, WHOLE>(r, xp + p * pixel_stride, d, v);
-            load_vec<T, WHOLE>(g, dp + p * dy_pixel, d, v);
+        while (p < p1) {
+            for_batch<FL>(p, p1, d.rows, [&](int u) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                float xh;
-                const float dz = grad_z<ACT>(g[j], r[j], k[j], st[j], xh);
-                s[j] += dz;
-                q[j] = fmaf(dz, xh, q[j]);
+                for (int j = 0; j < N; ++j) {
+                    const int c = min(channel_of<T, WHOLE>(d, v, j), d.c - 1);
+                    float e;
+                    const float dz = grad_z((float)g[u].v[j], (float)w[u].v[j], k[j], st + c / d.gc * 2, saved.weight + c,
+                                            ACT, e);
+                    s[j] += dz;
+                    q[j] = fmaf(dz, e, q[j]);
+                }
+            });
+            p += FL * d.rows;
+            if (p < p1) {
+                load_batch<T, WHOLE>(w, xp, pixel_stride, p, p1, d, v);
+                load_batch<T, WHOLE>(g, dp, dy_pixel, p, p1, d, v);
             }
         }
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            float *e = redf + ((long long)row * width + channel_of<T, WHOLE>(d, v, j)) * 2;
-            e[0] = s[j];
-            e[1] = q[j];
+            float *o = redf[row * units + channel_of<T, WHOLE>(d, v, j)];
+            o[0] = s[j];
+            o[1] = q[j];
         }
     }
-    __syncthreads();
-    for (int n = d.rows; n > 1;) {
-        const int h = (n + 1) / 2;
-        for (int i = threadIdx.x; i < (n - h) * width * 2; i += blockDim.x)
-            redf[i] += redf[i + h * width * 2];
-        __syncthreads();
-        n = h;
-    }
-    for (int i = threadIdx.x; i < d.c * 2; i += blockDim.x)
-        partial[(long long)blockIdx.x * d.c * 2 + i] = redf[i];
+    fold_rows(redf, d.rows, units);
+    float *out = partial + (long long)blockIdx.x * d.c * 2;
+    for (int c = threadIdx.x; c < d.c; c += blockDim.x)
+        *reinterpret_cast<float2 *>(out + c * 2) = float2{redf[c][0], redf[c][1] * (float)st[c / d.gc * 2 + 1]};
 }
 
-// partial (b, nch, c, 2) -> sums (b, c, 2) and means (b, groups, 2) = m1, m2, in fp64.  grid: (groups, b).
-__global__ __launch_bounds__(256) void k_gn_grad_finish(const float *__restrict__ partial, const void *weight,
-                                                        int affine_dtype, double *__restrict__ sums,
-                                                        double *__restrict__ means, GnDims d)
+// partial (b, nch, c, 2) -> sums (b, c, 2) in fp64 and a group's a1, a2 of grad_x.  grid: (groups, b).
+__global__ __launch_bounds__(256) void k_gn_grad_finish(const float *__restrict__ partial, Saved saved,
+                                                        double *__restrict__ sums, float2 *__restrict__ means, GnDims d)
 {
     __shared__ double red[256 * 2];
     const int g = blockIdx.x, b = blockIdx.y;
@@ -338,10 +583,11 @@ __global__ __launch_bounds__(256) void k_gn_grad_finish(const float *__restrict_
         const int cl = c0 + sub, c = g * d.gc + cl;
         double s = 0.0, q = 0.0;
         if (cl < d.gc)
+#pragma unroll 8
             for (int i = lane; i < d.nch; i += lanes) {
-                const float *p = partial + (((long long)b * d.nch + i) * d.c + c) * 2;
-                s += (double)p[0];
-                q += (double)p[1];
+                const float2 p = *reinterpret_cast<const float2 *>(partial + (((long long)b * d.nch + i) * d.c + c) * 2);
+                s += (double)p.x;
+                q += (double)p.y;
             }
         for (int m = lanes >> 1; m >= 1; m >>= 1) {
             s += __shfl_xor(s, m, 64);
@@ -350,7 +596,7 @@ __global__ __launch_bounds__(256) void k_gn_grad_finish(const float *__restrict_
         if (cl < d.gc && lane == 0) {
             sums[((long long)b * d.c + c) * 2] = s;
             sums[((long long)b * d.c + c) * 2 + 1] = q;
-            const double w = (double)load_affine(weight, affine_dtype, c, 1.0f);
+            const double w = (double)saved.weight[c];
             m1 += w * s;
             m2 += w * q;
         }
@@ -365,17 +611,16 @@ __global__ __launch_bounds__(256) void k_gn_grad_finish(const float *__restrict_
         }
         __syncthreads();
     }
-    if (threadIdx.x < 2)
-        means[((long long)b * d.groups + g) * 2 + threadIdx.x] = red[threadIdx.x] / ((double)d.gc * (double)d.hw);
+    if (threadIdx.x == 0) {
+        const double count = (double)d.gc * (double)d.hw, rstd = saved.stats[((long long)b * d.groups + g) * 2 + 1];
+        means[(long long)b * d.groups + g] = float2{(float)(rstd * red[0] / count), (float)(rstd * rstd * red[1] / count)};
+    }
 }
 
-// dw, dbeta: the images' sums added in order.  grid: ceil(c / 64)
-__global__ __launch_bounds__(64) void k_gn_grad_affine(const double *__restrict__ sums, void *dweight, void *dbias,
-                                                       int affine_dtype, int b, int c)
+// dw, dbeta: the images' sums added in order.  One thread a channel.
+__device__ __forceinline__ void affine_gradient(const double *sums, void *dweight, void *dbias, int affine_dtype, int b,
+                                                int c, int ch)
 {
-    const int ch = blockIdx.x * 64 + threadIdx.x;
-    if (ch >= c)
-        return;
     double s = 0.0, q = 0.0;
     for (int i = 0; i < b; ++i) {
         s += sums[((long long)i * c + ch) * 2];
@@ -387,63 +632,184 @@ __global__ __launch_bounds__(64) void k_gn_grad_affine(const double *__restrict_
         store_affine(dbias, affine_dtype, ch, s);
 }
 
-// grid: b * nch workgroups
-template <typename T, bool WHOLE, int ACT>
-__global__ __launch_bounds__(1024) void k_gn_grad_apply(const T *__restrict__ dy, long long dy_image, long long dy_pixel,
-                                                        const T *__restrict__ x, long long image_stride,
-                                                        long long pixel_stride, const double *__restrict__ stats,
-                                                        const double *__restrict__ means, const void *weight,
-                                                        const void *bias, int affine_dtype, T *__restrict__ dx, GnDims d)
+__global__ __launch_bounds__(64) void k_gn_grad_affine(const double *__restrict__ sums, void *dweight, void *dbias,
+                                                       int affine_dtype, int b, int c)
 {
-    constexpr int N = Vec<T>::N;
+    const int ch = blockIdx.x * 64 + threadIdx.x;
+    if (ch < c)
+        affine_gradient(sums, dweight, dbias, affine_dtype, b, c, ch);
+}
+
+// grid: b * nch workgroups, slab = the whole map; dx may be NULL (only dw, dbeta wanted: one workgroup then).
+// The last workgroups write dw and dbeta, too: no launch of their own.
+template <typename T, bool WHOLE, int ACT>
+__global__ __launch_bounds__(MAX_THREADS) void k_gn_grad_apply(const T *__restrict__ dy, long long dy_image,
+                                                               long long dy_pixel, const T *__restrict__ x,
+                                                               long long image_stride, long long pixel_stride, Saved saved,
+                                                               const float2 *__restrict__ means,
+                                                               const double *__restrict__ sums, T *__restrict__ dx,
+                                                               void *dweight, void *dbias, int affine_dtype, int images,
+                                                               GnDims d)
+{
+    constexpr int N = Vec<T>::N, FL = GRAD_IN_FLIGHT<WHOLE>;
+    if (dweight != nullptr || dbias != nullptr)
+        for (int c = (gridDim.x - 1 - blockIdx.x) * blockDim.x + threadIdx.x; c < d.c; c += gridDim.x * blockDim.x)
+            affine_gradient(sums, dweight, dbias, affine_dtype, images, d.c, c);
     const int b = blockIdx.x / d.nch, ch = blockIdx.x - b * d.nch;
     const int row = threadIdx.x / d.cv, v = threadIdx.x - row * d.cv;
-    if (row >= d.rows)
+    if (row >= d.rows || dx == nullptr)
         return;
-    Channel k[N];
-    const double *st[N];
-    float m1[N], m2[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const int c = channel_of<T, WHOLE>(d, v, j);
-        const long long g = (long long)b * d.groups + min(c, d.c - 1) / d.gc;
-        k[j] = channel_constants(stats, weight, bias, affine_dtype, d, b, c);
-        st[j] = stats + g * 2;
-        m1[j] = (float)means[g * 2];
-        m2[j] = (float)means[g * 2 + 1];
-    }
     const long long p0 = ch * d.chunk, p1 = min(p0 + d.chunk, d.hw);
     const T *xp = x + b * image_stride, *dp = dy + b * dy_image;
     T *op = dx + b * d.hw * d.c;
-#pragma unroll 2
-    for (long long p = p0 + row; p < p1; p += d.rows) {
-        float r[N], g[N];
-        load_vec<T, WHOLE>(r, xp + p * pixel_stride, d, v);
-        load_vec<T, WHOLE>(g, dp + p * dy_pixel, d, v);
+    Word<T> w[FL], g[FL];
+    long long p = p0 + row;
+    load_batch<T, WHOLE>(w, xp, pixel_stride, p, p1, d, v);
+    load_batch<T, WHOLE>(g, dp, dy_pixel, p, p1, d, v);
+    const double *st = saved.stats + (long long)b * d.groups * 2;
+    Channel k[N];
+    float2 a[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            float xh;
-            const float dz = grad_z<ACT>(g[j], r[j], k[j], st[j], xh);
-            r[j] = k[j].rstd * (dz * k[j].w - m1[j] - xh * m2[j]);
+    for (int j = 0; j < N; ++j) {
+        const int c = min(channel_of<T, WHOLE>(d, v, j), d.c - 1);
+        k[j] = saved.channels[(long long)b * d.c + c];
+        a[j] = means[(long long)b * d.groups + c / d.gc];
+    }
+    const long long step = (long long)d.rows * d.c;
+    while (p < p1) {
+        T *oq = op + p * d.c;
+        for_batch<FL>(p, p1, d.rows, [&](int u) {
+            Word<T> r;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int c = min(channel_of<T, WHOLE>(d, v, j), d.c - 1);
+                float e;
+                const float dz = grad_z((float)g[u].v[j], (float)w[u].v[j], k[j], st + c / d.gc * 2, saved.weight + c, ACT, e);
+                r.v[j] = (T)grad_x(dz, e, k[j], a[j]);
+            }
+            store_word<T, WHOLE>(oq + u * step, r, d, v);
+        });
+        p += FL * d.rows;
+        if (p < p1) {
+            load_batch<T, WHOLE>(w, xp, pixel_stride, p, p1, d, v);
+            load_batch<T, WHOLE>(g, dp, dy_pixel, p, p1, d, v);
         }
-        store_vec<T, WHOLE>(op + p * d.c, r, d, v);
     }
 }
 
+// The backward pass of small maps as k_gn_one is the forward's: x and dy of a slab in registers.  sums
+// (b, c, 2) for k_gn_grad_affine, or, of a single image, dw and dbeta themselves.  grid: b * slabs.
+template <typename T, bool WHOLE, int U>
+__global__ __launch_bounds__(MAX_THREADS) void k_gn_grad_one(const T *__restrict__ dy, long long dy_image,
+                                                             long long dy_pixel, const T *__restrict__ x,
+                                                             long long image_stride, long long pixel_stride, Saved saved,
+                                                             int act, T *__restrict__ dx, void *dweight, void *dbias,
+                                                             int affine_dtype, double *__restrict__ sums, int images,
+                                                             GnDims d)
+{
+    constexpr int N = Vec<T>::N;
+    extern __shared__ __align__(16) float redf[][2];
+    const int slabs = d.c / d.cs, b = blockIdx.x / slabs, c0 = (blockIdx.x - b * slabs) * d.cs;
+    const int row = threadIdx.x / d.cv, v = threadIdx.x - row * d.cv;
+    const bool live = row < d.rows;
+    const int units = d.cv * N, sg = d.cs / d.gc;
+    const T *xp = x + b * image_stride + c0, *dp = dy + b * dy_image + c0;
+    const double *st = saved.stats + ((long long)b * d.groups + c0 / d.gc) * 2;
+    const float *weight = saved.weight + c0;
+    Word<T> w[U], g[U];
+    Channel k[N];
+    if (live) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long long pp = min((long long)(row + u * d.rows), d.hw - 1);
+            w[u] = load_word<T, WHOLE>(xp + pp * pixel_stride, d, v);
+            g[u] = load_word<T, WHOLE>(dp + pp * dy_pixel, d, v);
+        }
+        float s[N], q[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            k[j] = saved.channels[(long long)b * d.c + c0 + min(channel_of<T, WHOLE>(d, v, j), d.cs - 1)];
+            s[j] = q[j] = 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (row + u * d.rows < d.hw)
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const int cl = min(channel_of<T, WHOLE>(d, v, j), d.cs - 1);
+                    float e;
+                    const float dz = grad_z((float)g[u].v[j], (float)w[u].v[j], k[j], st + cl / d.gc * 2, weight + cl, act, e);
+                    s[j] += dz;
+                    q[j] = fmaf(dz, e, q[j]);
+                }
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            float *o = redf[row * units + channel_of<T, WHOLE>(d, v, j)];
+            o[0] = s[j];
+            o[1] = q[j];
+        }
+    }
+    fold_rows(redf, d.rows, units);
+    // a channel's sums go out, and times its weight back for its group's a1 and a2
+    float (*weighted)[2] = redf + units;
+    float2 *means = reinterpret_cast<float2 *>(weighted + units);
+    for (int cl = threadIdx.x; cl < d.cs; cl += blockDim.x) {
+        const float s = redf[cl][0], q = redf[cl][1] * (float)st[cl / d.gc * 2 + 1], wt = weight[cl];
+        weighted[cl][0] = wt * s;
+        weighted[cl][1] = wt * q;
+        if (images > 1) {
+            sums[((long long)b * d.c + c0 + cl) * 2] = s;
+            sums[((long long)b * d.c + c0 + cl) * 2 + 1] = q;
+        } else {
+            if (dweight)
+                store_affine(dweight, affine_dtype, c0 + cl, q);
+            if (dbias)
+                store_affine(dbias, affine_dtype, c0 + cl, s);
+        }
+    }
+    if (dx == nullptr)
+        return;
+    __syncthreads();
+    const float (*wsums)[2] = weighted;
+    for_group_sums(wsums, sg, d.gc, [&](int i, float s, float q) {
+        const double count = (double)d.gc * (double)d.hw, rstd = st[i * 2 + 1];
+        means[i] = float2{(float)(rstd * (double)s / count), (float)(rstd * rstd * (double)q / count)};
+    });
+    __syncthreads();
+    if (!live)
+        return;
+    T *op = dx + b * d.hw * d.c + c0;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (row + u * d.rows < d.hw) {
+            Word<T> r;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int cl = min(channel_of<T, WHOLE>(d, v, j), d.cs - 1);
+                float e;
+                const float dz = grad_z((float)g[u].v[j], (float)w[u].v[j], k[j], st + cl / d.gc * 2, weight + cl, act, e);
+                r.v[j] = (T)grad_x(dz, e, k[j], means[cl / d.gc]);
+            }
+            store_word<T, WHOLE>(op + (long long)(row + u * d.rows) * d.c, r, d, v);
+        }
+}
+
 // ------------------------------------------------------------------------------------------- host
-constexpr int MAX_VECTORS = 1024;       // vectors of a pixel a workgroup can own
+constexpr int MAX_VECTORS = MAX_THREADS;        // vectors of a pixel: a thread each
 
-int vectors_of(int c, int dtype) { return ceil_div(c, dtype == DANCE_F32 ? 4 : 8); }
+int vector_of(int dtype) { return dtype == DANCE_F32 ? 4 : 8; }
 
-int threads_of(int cv) { return cv <= 256 ? 256 : cv <= 512 ? 512 : 1024; }
+int vectors_of(int c, int dtype) { return ceil_div(c, vector_of(dtype)); }
 
-// Workgroups of an image: about 2048 over the whole batch (eight a compute unit), each with 8 pixels a
-// thread at least, so that a workgroup's reduction is paid by enough reading.
+int threads_of(int cv) { return cv <= 256 ? 256 : MAX_THREADS; }
+
+// The two-pass form.  Workgroups of an image: about 2048 over the whole batch (eight a compute unit), each
+// with 8 pixels a thread at least, so that a workgroup's reduction is paid by enough reading.
 GnDims dims_of(int b, int c, long long hw, int groups, int dtype)
 {
     GnDims d;
     d.hw = hw;
-    d.c = c;
+    d.c = d.cs = c;
     d.cv = vectors_of(c, dtype);
     d.rows = threads_of(d.cv) / d.cv;
     d.groups = groups;
@@ -455,6 +821,41 @@ GnDims dims_of(int b, int c, long long hw, int groups, int dtype)
     d.nch = (int)((hw + d.chunk - 1) / d.chunk);
     return d;
 }
+
+// The one-launch form: MAX_THREADS a workgroup, at most `most` vectors a thread.  A slab is the fewest whole
+// groups that make whole vectors and a wanted width.  Wide slabs share fewer cache lines with other
+// workgroups, narrow ones are more workgroups with fewer vectors a thread: 64 bytes a pixel where that still
+// gives the chip a workgroup per unit, else 32, else 16.  false: the map is too large for any.
+constexpr int ONE_MOST = 16, GRAD_ONE_MOST = 8;
+
+bool one_launch(GnDims &d, int b, int dtype, int most)
+{
+    const int n = vector_of(dtype);
+    const bool whole = d.c % n == 0;
+    if (!whole)
+        most = 4;                                         // a vector of scalar loads is n registers
+    bool fits = false;
+    for (int least = 4 * n; least >= n; least /= 2) {
+        int k = 1;                                        // groups of a slab
+        while (k < d.groups && (d.groups % k != 0 || k * d.gc < least || (whole && k * d.gc % n != 0)))
+            ++k;
+        const int cs = k * d.gc, cv = ceil_div(cs, n);
+        if (cv > MAX_THREADS)
+            continue;
+        const int rows = MAX_THREADS / cv;
+        if (d.hw > (long long)rows * most)
+            continue;
+        fits = true;
+        d.cs = cs;
+        d.cv = cv;
+        d.rows = rows < d.hw ? rows : (int)d.hw;
+        if ((long long)b * (d.c / cs) >= 256)
+            break;
+    }
+    return fits;
+}
+
+int words_of(const GnDims &d) { return (int)((d.hw + d.rows - 1) / d.rows); }
 
 template <typename F> int with_type(int dtype, bool whole, F &&f)
 {
@@ -484,16 +885,25 @@ extern "C" int64_t dance_group_norm_workspace_bytes(int b, int c, int64_t hw, in
 {
     if (b <= 0 || c <= 0 || hw <= 0 || groups <= 0 || c % groups || !known_dtype(dtype) || vectors_of(c, dtype) > MAX_VECTORS)
         return 0;
-    const GnDims d = dims_of(b, c, hw, groups, dtype);
+    GnDims d = dims_of(b, c, hw, groups, dtype), one = d;
     if (!backward)
-        return (int64_t)b * d.nch * groups * 2 * sizeof(double);
+        return one_launch(one, b, dtype, ONE_MOST) ? 0 : (int64_t)b * d.nch * groups * 2 * sizeof(double);
+    if (one_launch(one, b, dtype, GRAD_ONE_MOST))
+        return b == 1 ? 0 : (int64_t)b * c * 2 * sizeof(double);
     return (int64_t)(whole_16((size_t)b * d.nch * c * 2 * sizeof(float)) + (size_t)b * c * 2 * sizeof(double) +
-                     (size_t)b * groups * 2 * sizeof(double));
+                     (size_t)b * groups * sizeof(float2));
+}
+
+extern "C" int64_t dance_group_norm_saved_bytes(int b, int c, int groups)
+{
+    if (b <= 0 || c <= 0 || groups <= 0 || c % groups)
+        return 0;
+    return (int64_t)((size_t)b * groups * 2 * sizeof(double) + (size_t)b * c * sizeof(Channel) + (size_t)c * sizeof(float));
 }
 
 extern "C" int dance_group_norm_act(const void *x, int64_t image_stride, int64_t pixel_stride, int dtype,
                                     const void *weight, const void *bias, int affine_dtype, float eps, int act,
-                                    int groups, void *y, double *stats, void *ws, int64_t ws_bytes, int b, int c,
+                                    int groups, void *y, void *saved, void *ws, int64_t ws_bytes, int b, int c,
                                     int64_t hw, void *stream)
 {
     DANCE_REQUIRE(b >= 0 && c >= 1 && hw >= 0 && groups >= 1 && c % groups == 0);
@@ -503,62 +913,114 @@ extern "C" int dance_group_norm_act(const void *x, int64_t image_stride, int64_t
     DANCE_REQUIRE(image_stride >= 0 && pixel_stride >= 0);
     if (b == 0 || hw == 0)
         return 0;
-    DANCE_REQUIRE(x && y && stats && ws && b <= 65535 && groups <= 65535);
-    DANCE_REQUIRE(ws_bytes >= dance_group_norm_workspace_bytes(b, c, hw, groups, dtype, 0));
-    const GnDims d = dims_of(b, c, hw, groups, dtype);
+    DANCE_REQUIRE(x && y && saved && ((uintptr_t)saved & 15) == 0 && b <= 65535 && groups <= 65535);
+    DANCE_REQUIRE(ws_bytes >= dance_group_norm_workspace_bytes(b, c, hw, groups, dtype, 0) && (ws || ws_bytes <= 0));
+    DANCE_REQUIRE(((uintptr_t)ws & 15) == 0);
+    GnDims d = dims_of(b, c, hw, groups, dtype);
     DANCE_REQUIRE((long long)b * d.nch < (1ll << 31));
     const int threads = threads_of(d.cv);
     const dim3 grid((unsigned)(b * d.nch));
     hipStream_t st = (hipStream_t)stream;
-    double *partial = (double *)ws;
-    return with_type(dtype, c % (dtype == DANCE_F32 ? 4 : 8) == 0, [&](auto t, auto whole) {
+    const Saved out = saved_at(saved, b, c, groups);
+    const char *fn = "dance_group_norm_act";
+    return with_type(dtype, c % vector_of(dtype) == 0, [&](auto t, auto whole) {
         using T = decltype(t);
         constexpr bool W = decltype(whole)::value;
-        const size_t lds = (size_t)d.rows * d.cv * Vec<T>::N * 2 * sizeof(double);
-        if (int rc = dance::allow_lds((const void *)k_gn_stats<T, W>, lds, "dance_group_norm_act"))
+        const bool vu = W && d.gc % Vec<T>::N == 0;
+        if (one_launch(d, b, dtype, ONE_MOST)) {
+            auto one = [&](auto u) {
+                constexpr int U = decltype(u)::value;
+                const int units = vu ? d.cv : d.cv * Vec<T>::N;
+                // the sums of the rows; or row 0 and, behind it, the groups' statistics and the channels' constants
+                const size_t sums = (size_t)d.rows * units * 2 * sizeof(double);
+                const size_t after = ((size_t)units + d.cs / d.gc) * 2 * sizeof(double) + d.cs * sizeof(Channel);
+                const size_t lds = sums > after ? sums : after;
+                if (int rc = dance::allow_lds((const void *)k_gn_one<T, W, U>, lds, fn))
+                    return rc;
+                hipLaunchKernelGGL((k_gn_one<T, W, U>), dim3((unsigned)(b * (c / d.cs))), dim3(MAX_THREADS), lds, st,
+                                   (const T *)x, (long long)image_stride, (long long)pixel_stride, weight, bias,
+                                   affine_dtype, (double)eps, act, (T *)y, out, d);
+                return launch_check(fn);
+            };
+            if constexpr (W)
+                if (words_of(d) > 4)
+                    return one(std::integral_constant<int, ONE_MOST>{});
+            return one(std::integral_constant<int, 4>{});
+        }
+        double *partial = (double *)ws;
+        const size_t lds = (size_t)d.rows * d.cv * (vu ? 1 : Vec<T>::N) * 2 * sizeof(double);
+        if (int rc = dance::allow_lds((const void *)k_gn_stats<T, W>, lds, fn))
             return rc;
         hipLaunchKernelGGL((k_gn_stats<T, W>), grid, dim3(threads), lds, st, (const T *)x, (long long)image_stride,
                            (long long)pixel_stride, partial, d);
-        if (int rc = launch_check("dance_group_norm_act"))
+        if (int rc = launch_check(fn))
             return rc;
-        hipLaunchKernelGGL(k_gn_finish, dim3(groups, b), dim3(64), 0, st, (const double *)partial, stats, groups, d.nch,
-                           (double)d.gc * (double)d.hw, (double)eps);
-        if (int rc = launch_check("dance_group_norm_act"))
+        hipLaunchKernelGGL(k_gn_finish, dim3(groups, b), dim3(256), 0, st, (const double *)partial, out, weight, bias,
+                           affine_dtype, (double)d.gc * (double)d.hw, (double)eps, d);
+        if (int rc = launch_check(fn))
             return rc;
         return with_act(act, [&](auto a) {
             hipLaunchKernelGGL((k_gn_apply<T, W, decltype(a)::value>), grid, dim3(threads), 0, st, (const T *)x,
-                               (long long)image_stride, (long long)pixel_stride, (const double *)stats, weight, bias,
-                               affine_dtype, (T *)y, d);
-            return launch_check("dance_group_norm_act");
+                               (long long)image_stride, (long long)pixel_stride, (const Channel *)out.channels, (T *)y, d);
+            return launch_check(fn);
         });
     });
 }
 
 extern "C" int dance_group_norm_act_backward(const void *dy, int64_t dy_image_stride, int64_t dy_pixel_stride,
                                              const void *x, int64_t image_stride, int64_t pixel_stride, int dtype,
-                                             const void *weight, const void *bias, int affine_dtype, int act, int groups,
-                                             const double *stats, void *dx, void *dweight, void *dbias, void *ws,
-                                             int64_t ws_bytes, int b, int c, int64_t hw, void *stream)
+                                             int affine_dtype, int act, int groups, const void *saved, void *dx,
+                                             void *dweight, void *dbias, void *ws, int64_t ws_bytes, int b, int c,
+                                             int64_t hw, void *stream)
 {
     DANCE_REQUIRE(b >= 1 && c >= 1 && hw >= 1 && groups >= 1 && c % groups == 0);
     DANCE_REQUIRE(known_dtype(dtype) && known_dtype(affine_dtype));
     DANCE_REQUIRE(act == DANCE_ACT_NONE || act == DANCE_ACT_RELU || act == DANCE_ACT_SILU);
     DANCE_REQUIRE(vectors_of(c, dtype) <= MAX_VECTORS);
     DANCE_REQUIRE(dy_image_stride >= 0 && dy_pixel_stride >= 0 && image_stride >= 0 && pixel_stride >= 0);
-    DANCE_REQUIRE(dy && x && stats && ws && b <= 65535 && groups <= 65535);
-    DANCE_REQUIRE(ws_bytes >= dance_group_norm_workspace_bytes(b, c, hw, groups, dtype, 1));
-    const GnDims d = dims_of(b, c, hw, groups, dtype);
+    DANCE_REQUIRE(dy && x && saved && ((uintptr_t)saved & 15) == 0 && b <= 65535 && groups <= 65535);
+    DANCE_REQUIRE(ws_bytes >= dance_group_norm_workspace_bytes(b, c, hw, groups, dtype, 1) && (ws || ws_bytes <= 0));
+    DANCE_REQUIRE(((uintptr_t)ws & 15) == 0);
+    if (!dx && !dweight && !dbias)
+        return 0;
+    GnDims d = dims_of(b, c, hw, groups, dtype);
     DANCE_REQUIRE((long long)b * d.nch < (1ll << 31));
     const int threads = threads_of(d.cv);
     const dim3 grid((unsigned)(b * d.nch));
     hipStream_t st = (hipStream_t)stream;
-    float *partial = (float *)ws;
-    double *sums = (double *)((char *)ws + whole_16((size_t)b * d.nch * c * 2 * sizeof(float)));
-    double *means = sums + (size_t)b * c * 2;
+    const Saved sv = saved_at(const_cast<void *>(saved), b, c, groups);        // read only
     const char *fn = "dance_group_norm_act_backward";
-    return with_type(dtype, c % (dtype == DANCE_F32 ? 4 : 8) == 0, [&](auto t, auto whole) {
+    return with_type(dtype, c % vector_of(dtype) == 0, [&](auto t, auto whole) {
         using T = decltype(t);
         constexpr bool W = decltype(whole)::value;
+        if (one_launch(d, b, dtype, GRAD_ONE_MOST)) {
+            auto one = [&](auto u) {
+                constexpr int U = decltype(u)::value;
+                const int units = d.cv * Vec<T>::N;
+                // the sums of the rows; or row 0, the weighted sums and the groups' means
+                const size_t sums = (size_t)d.rows * units, after = 2 * (size_t)units + d.cs / d.gc;
+                const size_t lds = (sums > after ? sums : after) * 2 * sizeof(float);
+                if (int rc = dance::allow_lds((const void *)k_gn_grad_one<T, W, U>, lds, fn))
+                    return rc;
+                hipLaunchKernelGGL((k_gn_grad_one<T, W, U>), dim3((unsigned)(b * (c / d.cs))), dim3(MAX_THREADS), lds, st,
+                                   (const T *)dy, (long long)dy_image_stride, (long long)dy_pixel_stride, (const T *)x,
+                                   (long long)image_stride, (long long)pixel_stride, sv, act, (T *)dx, dweight, dbias,
+                                   affine_dtype, (double *)ws, b, d);
+                return launch_check(fn);
+            };
+            // (four vectors of scalar loads are the most of the other kind)
+            constexpr int MOST = W ? GRAD_ONE_MOST : 4;
+            if (int rc = words_of(d) <= 2 ? one(std::integral_constant<int, 2>{}) : one(std::integral_constant<int, MOST>{}))
+                return rc;
+            if (b == 1 || (!dweight && !dbias))
+                return 0;
+            hipLaunchKernelGGL(k_gn_grad_affine, dim3(ceil_div(c, 64)), dim3(64), 0, st, (const double *)ws, dweight, dbias,
+                               affine_dtype, b, c);
+            return launch_check(fn);
+        }
+        float *partial = (float *)ws;
+        double *sums = (double *)((char *)ws + whole_16((size_t)b * d.nch * c * 2 * sizeof(float)));
+        float2 *means = (float2 *)(sums + (size_t)b * c * 2);
         return with_act(act, [&](auto a) {
             constexpr int ACT = decltype(a)::value;
             const size_t lds = (size_t)d.rows * d.cv * Vec<T>::N * 2 * sizeof(float);
@@ -566,28 +1028,17 @@ extern "C" int dance_group_norm_act_backward(const void *dy, int64_t dy_image_st
                 return rc;
             hipLaunchKernelGGL((k_gn_grad_sums<T, W, ACT>), grid, dim3(threads), lds, st, (const T *)dy,
                                (long long)dy_image_stride, (long long)dy_pixel_stride, (const T *)x,
-                               (long long)image_stride, (long long)pixel_stride, stats, weight, bias, affine_dtype,
-                               partial, d);
+                               (long long)image_stride, (long long)pixel_stride, sv, partial, d);
             if (int rc = launch_check(fn))
                 return rc;
-            hipLaunchKernelGGL(k_gn_grad_finish, dim3(groups, b), dim3(256), 0, st, (const float *)partial, weight,
-                               affine_dtype, sums, means, d);
+            hipLaunchKernelGGL(k_gn_grad_finish, dim3(groups, b), dim3(256), 0, st, (const float *)partial, sv, sums, means, d);
             if (int rc = launch_check(fn))
                 return rc;
-            if (dweight || dbias) {
-                hipLaunchKernelGGL(k_gn_grad_affine, dim3(ceil_div(c, 64)), dim3(64), 0, st, (const double *)sums,
-                                   dweight, dbias, affine_dtype, b, c);
-                if (int rc = launch_check(fn))
-                    return rc;
-            }
-            if (dx) {
-                hipLaunchKernelGGL((k_gn_grad_apply<T, W, ACT>), grid, dim3(threads), 0, st, (const T *)dy,
-                                   (long long)dy_image_stride, (long long)dy_pixel_stride, (const T *)x,
-                                   (long long)image_stride, (long long)pixel_stride, stats, (const double *)means,
-                                   weight, bias, affine_dtype, (T *)dx, d);
-                return launch_check(fn);
-            }
-            return 0;
+            hipLaunchKernelGGL((k_gn_grad_apply<T, W, ACT>), dx ? grid : dim3(1), dim3(threads), 0, st, (const T *)dy,
+                               (long long)dy_image_stride, (long long)dy_pixel_stride, (const T *)x,
+                               (long long)image_stride, (long long)pixel_stride, sv, (const float2 *)means,
+                               (const double *)sums, (T *)dx, dweight, dbias, affine_dtype, b, d);
+            return launch_check(fn);
         });
     });
 }

@@ -10,7 +10,7 @@ import os
 import torch
 
 from ._lib import (ACT_NONE, ACT_RELU, ACT_SILU, ABSMAX_OF_FEATURES, ABSMAX_OF_GN_RELU, ABSMAX_OF_LAYOUT, ABSMAX_WORDS, DTYPE_BF16,
-                   DTYPE_F16, DTYPE_F32, check, current_stream, lib, ptr)
+                   DTYPE_F16, DTYPE_F32, check, current_stream, lib, on_device, ptr, stream_of)
 
 POLY_RAW, POLY_BOX, POLY_QUAD, POLY_OCTAGON = 0, 1, 2, 3
 PAD_ZEROS, PAD_REFLECTION = 0, 1
@@ -529,39 +529,45 @@ def _empty_nhwc(shape, dtype, device):
     return torch.empty((shape[0],) + tuple(shape[2:]) + (shape[1],), dtype=dtype, device=device).movedim(-1, 1)
 
 
+def _scratch(nbytes, device):
+    return torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes else None
+
+
 def _group_norm_forward(x, groups, weight, bias, eps, act):
-    """-> (y, the map as it was read, stats (B, groups, 2) f64)"""
-    b, c = x.shape[:2]
-    hw = math.prod(x.shape[2:])
+    """-> (y, the map as it was read, what the backward call takes)"""
+    shape, dev = x.shape, x.device
+    b, c, hw = shape[0], shape[1], math.prod(shape[2:])
     x, image, pixel = _nhwc_view(x)
-    y = _empty_nhwc(x.shape, x.dtype, x.device)
-    stats = torch.empty((b, groups, 2), dtype=torch.float64, device=x.device)
+    y = _empty_nhwc(shape, x.dtype, dev)
+    h = lib()
+    saved = torch.empty((h.dance_group_norm_saved_bytes(b, c, groups),), dtype=torch.uint8, device=dev)
     dt, affine = DTYPE_CODES[x.dtype], weight if weight is not None else bias
     at = DTYPE_F32 if affine is None else DTYPE_CODES[affine.dtype]
-    nbytes = lib().dance_group_norm_workspace_bytes(b, c, hw, groups, dt, 0)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
-        check(lib().dance_group_norm_act(ptr(x), image, pixel, dt, ptr(weight), ptr(bias), at, eps, act, groups, ptr(y),
-                                         ptr(stats), ptr(ws), nbytes, b, c, hw, current_stream()), "group_norm_act")
-    return y, x, stats
+    nbytes = h.dance_group_norm_workspace_bytes(b, c, hw, groups, dt, 0)
+    ws = _scratch(nbytes, dev)
+    with on_device(dev):
+        check(h.dance_group_norm_act(x.data_ptr(), image, pixel, dt, ptr(weight), ptr(bias), at, eps, act, groups,
+                                     y.data_ptr(), saved.data_ptr(), ptr(ws), nbytes, b, c, hw, stream_of(dev)),
+              "group_norm_act")
+    return y, x, saved
 
 
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
-        y, x, stats = _group_norm_forward(x, groups, weight, bias, eps, act)
-        ctx.save_for_backward(x, weight, bias, stats)
+        y, x, saved = _group_norm_forward(x, groups, weight, bias, eps, act)
+        ctx.save_for_backward(x, weight, bias, saved)
         ctx.groups, ctx.act = groups, act
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, stats = ctx.saved_tensors
+        x, weight, bias, saved = ctx.saved_tensors
         want_x, want_w, want_b = ctx.needs_input_grad[:3]
-        b, c = x.shape[:2]
-        hw = math.prod(x.shape[2:])
-        dx = _empty_nhwc(x.shape, x.dtype, x.device) if want_x else None
+        shape, dev = x.shape, x.device
+        b, c, hw = shape[0], shape[1], math.prod(shape[2:])
+        dx = _empty_nhwc(shape, x.dtype, dev) if want_x else None
         dw = torch.empty_like(weight) if want_w else None
         db = torch.empty_like(bias) if want_b else None
         if b == 0 or hw == 0:                        # empty sums
@@ -570,12 +576,13 @@ class _GroupNormAct(torch.autograd.Function):
         image, pixel = _channels_last_strides(x)
         dt, affine = DTYPE_CODES[x.dtype], weight if weight is not None else bias
         at = DTYPE_F32 if affine is None else DTYPE_CODES[affine.dtype]
-        nbytes = lib().dance_group_norm_workspace_bytes(b, c, hw, ctx.groups, dt, 1)
-        ws = torch.empty((nbytes,), dtype=torch.uint8, device=x.device)
-        with torch.cuda.device(x.device):
-            check(lib().dance_group_norm_act_backward(ptr(dy), dy_image, dy_pixel, ptr(x), image, pixel, dt, ptr(weight),
-                                                      ptr(bias), at, ctx.act, ctx.groups, ptr(stats), ptr(dx), ptr(dw),
-                                                      ptr(db), ptr(ws), nbytes, b, c, hw, current_stream()),
+        h = lib()
+        nbytes = h.dance_group_norm_workspace_bytes(b, c, hw, ctx.groups, dt, 1)
+        ws = _scratch(nbytes, dev)
+        with on_device(dev):
+            check(h.dance_group_norm_act_backward(dy.data_ptr(), dy_image, dy_pixel, x.data_ptr(), image, pixel, dt,
+                                                  at, ctx.act, ctx.groups, saved.data_ptr(), ptr(dx), ptr(dw), ptr(db),
+                                                  ptr(ws), nbytes, b, c, hw, stream_of(dev)),
                   "group_norm_act backward")
         return dx, dw, db, None, None, None
 

@@ -653,11 +653,13 @@ int dance_snake_init16(const dance_snake_net16 *net_host, const dance_init_fuse1
  *
  * x: c channels innermost; image i, pixel p at x + i * image_stride + p * pixel_stride (elements, >= 0; any
  * alignment an element has).  dtype / affine_dtype: DANCE_F32 / DANCE_F16 / DANCE_BF16; weight, bias (c) or
- * NULL (1 and 0).  At most 1024 vectors of 16 bytes a pixel: c <= 4096 (fp32), 8192 (16-bit types).
+ * NULL (1 and 0).  At most 512 vectors of 16 bytes a pixel: c <= 2048 (fp32), 4096 (16-bit types).
  *   mu, var over a group's c / groups channels and hw pixels;  y = act((x - mu) / sqrt(var + eps) * weight + bias)
- * y: dense (b, hw, c).  stats (b, groups, 2) f64: mean and 1 / sqrt(var + eps), what the backward pass
- * takes.  ws: dance_group_norm_workspace_bytes of scratch, nothing to clear.  b == 0 or hw == 0: nothing is
- * done.  Results do not depend on the run (no atomics); a NaN or an infinity makes its group NaN. */
+ * y: dense (b, hw, c).  saved: dance_group_norm_saved_bytes, 16-byte aligned: what the backward call takes
+ * (fp64 mean and 1 / sqrt(var + eps) of every group first, (b, groups, 2)).  ws:
+ * dance_group_norm_workspace_bytes of 16-byte aligned scratch (0 for small maps: NULL), nothing to clear.
+ * b == 0 or hw == 0: nothing is done.  Results do not depend on the run (no atomics); a NaN or an infinity
+ * makes its group NaN. */
 #define DANCE_F32 0
 #define DANCE_F16 1
 #define DANCE_BF16 2
@@ -665,19 +667,20 @@ int dance_snake_init16(const dance_snake_net16 *net_host, const dance_init_fuse1
 #define DANCE_ACT_RELU 1
 #define DANCE_ACT_SILU 2
 int64_t dance_group_norm_workspace_bytes(int b, int c, int64_t hw, int groups, int dtype, int backward);
+int64_t dance_group_norm_saved_bytes(int b, int c, int groups);
 int dance_group_norm_act(const void *x, int64_t image_stride, int64_t pixel_stride, int dtype,
                          const void *weight, const void *bias, int affine_dtype, float eps, int act,
-                         int groups, void *y, double *stats, void *ws, int64_t ws_bytes, int b, int c,
+                         int groups, void *y, void *saved, void *ws, int64_t ws_bytes, int b, int c,
                          int64_t hw, void *stream);
 
 /* The gradients of dance_group_norm_act: dy (strides as x's) -> dx dense (b, hw, c) of x's type, dweight and
- * dbias (c) of the affine type; any of the three may be NULL (not wanted).  stats as the forward call left
- * them.  ReLU's gradient is dy where z > 0, z evaluated in fp64 near zero. */
+ * dbias (c) of the affine type; any of the three may be NULL (not wanted).  x and saved as the forward call had
+ * and left them.  ReLU's gradient is dy where z > 0, z evaluated in fp64 near zero. */
 int dance_group_norm_act_backward(const void *dy, int64_t dy_image_stride, int64_t dy_pixel_stride,
                                   const void *x, int64_t image_stride, int64_t pixel_stride, int dtype,
-                                  const void *weight, const void *bias, int affine_dtype, int act,
-                                  int groups, const double *stats, void *dx, void *dweight, void *dbias,
-                                  void *ws, int64_t ws_bytes, int b, int c, int64_t hw, void *stream);
+                                  int affine_dtype, int act, int groups, const void *saved, void *dx,
+                                  void *dweight, void *dbias, void *ws, int64_t ws_bytes, int b, int c,
+                                  int64_t hw, void *stream);
 
 #ifdef __cplusplus
 }

@@ -10,21 +10,21 @@ BAD = 1                                                    # hipErrorInvalidValu
 
 
 def _norm(**over):
-    a = dict(x=None, image=0, pixel=8, dtype=0, w=None, b=None, affine=0, eps=1e-5, act=1, groups=2, y=None, stats=None,
+    a = dict(x=None, image=0, pixel=8, dtype=0, w=None, b=None, affine=0, eps=1e-5, act=1, groups=2, y=None, saved=None,
              ws=None, ws_bytes=0, n=1, c=8, hw=4, stream=None)
     a.update(over)
     return _lib.lib().dance_group_norm_act(*a.values())
 
 
 def _norm_backward(**over):
-    a = dict(dy=None, dy_image=0, dy_pixel=8, x=None, image=0, pixel=8, dtype=0, w=None, b=None, affine=0, act=1, groups=2,
-             stats=None, dx=None, dw=None, db=None, ws=None, ws_bytes=0, n=1, c=8, hw=4, stream=None)
+    a = dict(dy=None, dy_image=0, dy_pixel=8, x=None, image=0, pixel=8, dtype=0, affine=0, act=1, groups=2,
+             saved=None, dx=None, dw=None, db=None, ws=None, ws_bytes=0, n=1, c=8, hw=4, stream=None)
     a.update(over)
     return _lib.lib().dance_group_norm_act_backward(*a.values())
 
 
 @pytest.mark.parametrize("over", [dict(dtype=3), dict(affine=-1), dict(act=9), dict(groups=3), dict(groups=0), dict(c=0),
-                                  dict(c=4100, groups=1), dict(c=8200, groups=1, dtype=2), dict(eps=-1.0), dict(eps=float("nan")),
+                                  dict(c=2052, groups=1), dict(c=4104, groups=1, dtype=2), dict(eps=-1.0), dict(eps=float("nan")),
                                   dict(image=-1), dict(pixel=-8), dict(n=-1), dict(hw=-1), dict(), dict(n=70000)])
 def test_group_norm_refuses(over):
     assert _norm(**over) == BAD and b"requirement failed" in _lib.lib().dance_last_error()
@@ -37,15 +37,17 @@ def test_group_norm_empty_calls_do_nothing():
 
 
 def test_group_norm_workspace():
-    """positive where the call is allowed, large enough to be refused when it is one byte short"""
+    """none for maps of one launch; otherwise large enough for every group's sums, and refused one byte short"""
     size = _lib.lib().dance_group_norm_workspace_bytes
-    assert size(1, 4100, 4, 1, 0, 0) == 0 and size(1, 8, 4, 3, 0, 0) == 0 and size(0, 8, 4, 2, 0, 0) == 0
+    assert size(1, 2052, 4, 1, 0, 0) == 0 and size(1, 8, 4, 3, 0, 0) == 0 and size(0, 8, 4, 2, 0, 0) == 0
+    fake = ctypes.c_void_p(64)                             # never reached: the size is looked at first
     for dtype in (0, 1, 2):
-        for n, c, hw, groups in ((1, 8, 1, 2), (2, 256, 60800, 32), (3, 2050, 9, 2)):
-            need = size(n, c, hw, groups, dtype, 0)
-            assert need >= 16 * n * groups and size(n, c, hw, groups, dtype, 1) >= 16 * n * c
-            fake = ctypes.c_void_p(64)                     # never reached: the size is looked at first
-            assert _norm(x=fake, y=fake, stats=fake, ws=fake, ws_bytes=need - 1, n=n, c=c, hw=hw, groups=groups, dtype=dtype) == BAD
+        assert size(1, 8, 1, 2, dtype, 0) == 0 and size(1, 8, 1, 2, dtype, 1) == 0
+        assert size(3, 8, 1, 2, dtype, 1) == 3 * 8 * 16     # a channel's two sums of every image
+        need = size(2, 256, 60800, 32, dtype, 0)
+        assert need >= 2 * 32 * 16 and size(2, 256, 60800, 32, dtype, 1) >= 2 * 256 * 16
+        big = dict(x=fake, y=fake, saved=fake, n=2, c=256, hw=60800, groups=32, dtype=dtype)
+        assert _norm(ws=fake, ws_bytes=need - 1, **big) == BAD and _norm(ws=None, ws_bytes=need, **big) == BAD
 
 
 def test_group_norm_needs_a_gpu_tensor():
