@@ -6,7 +6,7 @@ There is NO fallback: if the shared object is missing or a symbol is absent, imp
 import contextlib
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # DANCE_HIP_LIB: load another build of the same library (A/B kernel experiments)
@@ -80,6 +80,12 @@ class FcoseLevelStruct(ctypes.Structure):
     _fields_ = [("cls", c_void_p), ("ctr", c_void_p), ("reg", c_void_p), ("ext", c_void_p),
                 ("locations", c_void_p), ("hw", c_int), ("stride", c_float)]
 
+class MuonItemStruct(ctypes.Structure):
+    """Mirror of `dance_muon_item` (include/dance_hip.h)."""
+
+    _fields_ = [("param", c_void_p), ("grad", c_void_p), ("momentum", c_void_p), ("rows", c_int), ("cols", c_int)]
+
+
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2          # DANCE_F32 / DANCE_F16 / DANCE_BF16
 ACT_NONE, ACT_RELU, ACT_SILU = 0, 1, 2              # DANCE_ACT_*
 
@@ -106,6 +112,12 @@ SIGNATURES = {
     "dance_group_norm_act_backward": (c_int, [P, c_int64, c_int64, P, c_int64, c_int64, c_int, c_int, c_int, c_int, P,
                                               P, P, P, P, c_int64, c_int, c_int, c_int64, P]),
     "dance_group_norm_saved_bytes": (c_int64, [c_int, c_int, c_int]),
+    "dance_orthogonalize_workspace_bytes": (c_int64, [c_int, c_int, c_int]),
+    "dance_orthogonalize": (c_int, [P, c_int64, c_int64, c_int64, c_int, P, c_int, c_int, c_int, c_int, c_float, c_float,
+                                    c_float, c_float, P, c_int64, P]),
+    "dance_muon_workspace_bytes": (c_int64, [POINTER(MuonItemStruct), c_int]),
+    "dance_muon_step": (c_int, [POINTER(MuonItemStruct), c_int, c_int, c_double, c_double, c_int, c_double, c_int, c_float,
+                                c_float, c_float, c_float, P, c_int64, P]),
     "dance_nms_sorted": (c_int, [P, c_int, c_float, P, P, P, P]),
     "dance_nms_sorted_plain": (c_int, [P, c_int, c_float, P, P, P, P]),
     "dance_nms_sorted_plain_static": (c_int, [P, c_int, c_float, P, P, P]),

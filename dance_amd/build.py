@@ -47,6 +47,7 @@ SOURCES = [
     ("fuse16w.hip", []),
     ("featprep16.hip", []),
     ("groupnorm.hip", []),
+    ("newton_schulz.hip", []),
     ("raster.hip", ["-ffp-contract=off"]),
     ("attender.hip", []),
     ("fcose.hip", ["-ffp-contract=off"]),

@@ -624,6 +624,49 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="relu"):
     return _group_norm_forward(x, int(num_groups), weight, bias, float(eps), ACTIVATIONS[act])[0]
 
 
+# -------------------------------------------------------------------- orthogonalised updates
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)     # singular values from 0.01 up end within 0.7 .. 1.2 in 5 steps
+
+
+def check_newton_schulz(what, steps, eps, coefficients):
+    """The chain's settings, refused as ops.orthogonalize and optim.Muon do -> (steps, eps, (a, b, c))"""
+    if int(steps) != steps or not 1 <= steps <= 100:
+        raise RuntimeError("%s: 1 to 100 steps, got %r" % (what, steps))
+    if not 1e-30 <= eps < float("inf"):
+        raise RuntimeError("%s: eps must be positive and finite, got %r" % (what, eps))
+    if len(coefficients) != 3 or not all(math.isfinite(v) for v in coefficients):
+        raise RuntimeError("%s: three finite coefficients expected, got %r" % (what, coefficients))
+    return int(steps), float(eps), tuple(float(v) for v in coefficients)
+
+
+def orthogonalize(x, steps=5, eps=1e-7, coefficients=NS_COEFFICIENTS):
+    """The orthogonal factor of a matrix, or of every matrix of a batch, by Newton-Schulz products (what the
+    Muon optimizer does to an update): X = x / max(|x|_F, eps), then `steps` times A = X X',
+    X <- a X + (b A + c A A) X, on the smaller side.
+
+    x (..., m, n) fp32 / fp16 / bf16, any strides; the products are fp32-accurate for every type.  The
+    coefficients have to keep singular values below 2.  Returns a dense tensor of x's shape and type; not
+    differentiable (call it on a detached tensor or under no_grad)."""
+    _need_gpu(x)
+    steps, eps, (a, b, c) = check_newton_schulz("orthogonalize", steps, eps, coefficients)
+    if x.dim() < 2 or x.dtype not in DTYPE_CODES:
+        raise RuntimeError("orthogonalize: (..., m, n) fp32, fp16 or bf16 expected, got %s %s" % (tuple(x.shape), x.dtype))
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("orthogonalize is not differentiable: call it on a detached tensor or under torch.no_grad()")
+    m, n = x.shape[-2:]
+    dev = x.device
+    out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    x = x.reshape((-1, m, n)) if x.numel() else x.new_empty((0, m, n))
+    batch = x.size(0)
+    h = lib()
+    nbytes = h.dance_orthogonalize_workspace_bytes(batch, m, n)
+    ws = _scratch(nbytes, dev)
+    with on_device(dev):
+        check(h.dance_orthogonalize(x.data_ptr(), *x.stride(), DTYPE_CODES[x.dtype], out.data_ptr(), batch, m, n, steps,
+                                    a, b, c, eps, ptr(ws), nbytes, stream_of(dev)), "orthogonalize")
+    return out
+
+
 # ---------------------------------------------------------------------------- attender
 def attender(x, w1, gn1_w, gn1_b, w2_packed, gn2_w, gn2_b, w3, b3, eps=1e-5):
     """EdgeSnakeFPNHead.attender (edge_det.py:66-100) on x = 1 - pred_edge, (B,1,H,W) or (B,H,W)

@@ -682,6 +682,38 @@ int dance_group_norm_act_backward(const void *dy, int64_t dy_image_stride, int64
                                   void *dweight, void *dbias, void *ws, int64_t ws_bytes, int b, int c,
                                   int64_t hw, void *stream);
 
+/* ---- orthogonalised updates (Newton-Schulz) and the Muon step built on them ----
+ * No counterpart in the reference, which trains with SGD; for the weight matrices of the heads (a convolution's
+ * weight as (out, in * taps)).
+ *
+ * dance_orthogonalize: of every matrix M (m, n) of a batch, out (batch, m, n) dense of x's type:
+ *   X = M / max(|M|_F, eps), then `steps` times  A = X X',  X <- a X + (b A + c A A) X.
+ * x: element strides >= 0 of the batch, the rows and the columns.  The products are fp32-accurate (split
+ * halves, three f16 MFMAs each) for every type; out is rounded once.  Coefficients have to keep the
+ * singular values below 2 (the usual 3.4445, -4.7750, 2.0315 stay below 1.21), or the result is not finite.
+ * A matrix with a NaN or an infinity comes out NaN, a zero matrix zero.  m n < 2^31.  ws:
+ * dance_orthogonalize_workspace_bytes of 16-byte aligned scratch, nothing to clear. */
+int64_t dance_orthogonalize_workspace_bytes(int batch, int m, int n);
+int dance_orthogonalize(const void *x, int64_t batch_stride, int64_t row_stride, int64_t col_stride,
+                        int dtype, void *out, int batch, int m, int n, int steps, float a, float b,
+                        float c, float eps, void *ws, int64_t ws_bytes, void *stream);
+
+/* dance_muon_step: one optimizer step over `count` matrices of any shapes and one type, dense (rows, cols)
+ * parameter, gradient and momentum each:
+ *   m <- momentum m + (1 - momentum) g;   u = nesterov ? momentum m + (1 - momentum) g : m
+ *   p <- p (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) O,   O = orthogonalize(u)
+ * in fp32, m and p rounded to the type once each.  items_host is read during the call only. */
+typedef struct dance_muon_item {
+    void *param;
+    const void *grad;
+    void *momentum;
+    int rows, cols;
+} dance_muon_item;
+int64_t dance_muon_workspace_bytes(const dance_muon_item *items_host, int count);
+int dance_muon_step(const dance_muon_item *items_host, int count, int dtype, double lr, double momentum,
+                    int nesterov, double weight_decay, int steps, float a, float b, float c, float eps,
+                    void *ws, int64_t ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -67,3 +67,81 @@ def test_channels_last_strides():
     assert s(torch.zeros((3, 6))) == (6, 6)
     assert s(torch.zeros((3, 1, 4, 4))) == (16, 1)         # one channel: any layout
     assert s(torch.zeros((3, 6, 1, 1))) == (6, 6)
+
+
+def _orth(**over):
+    a = dict(x=None, bs=0, rs=8, cs=1, dtype=0, out=None, batch=1, m=4, n=8, steps=5, a=3.4445, b=-4.775, c=2.0315, eps=1e-7,
+             ws=None, ws_bytes=0, stream=None)
+    a.update(over)
+    return _lib.lib().dance_orthogonalize(*a.values())
+
+
+@pytest.mark.parametrize("over", [dict(dtype=7), dict(steps=0), dict(steps=101), dict(a=float("nan")), dict(c=float("inf")),
+                                  dict(eps=0.0), dict(eps=float("nan")), dict(rs=-1), dict(bs=-1), dict(cs=-1), dict(m=-1),
+                                  dict(batch=-1), dict(m=1 << 16, n=1 << 15), dict()])
+def test_orthogonalize_refuses(over):
+    assert _orth(**over) == BAD and b"requirement failed" in _lib.lib().dance_last_error()
+
+
+def test_orthogonalize_empty_and_workspace():
+    assert _orth(batch=0) == 0 and _orth(m=0) == 0 and _orth(n=0) == 0
+    size = _lib.lib().dance_orthogonalize_workspace_bytes
+    assert size(0, 4, 8) == 0 and size(1, 0, 8) == 0 and size(1, 1 << 16, 1 << 15) == 0
+    need = size(3, 100, 200)
+    assert need % 3 == 0 and need >= 3 * 16 * 100 * 200     # two layouts, two steps, 4 bytes each
+    fake = ctypes.c_void_p(64)
+    assert _orth(x=fake, out=fake, ws=fake, ws_bytes=need - 1, batch=3, m=100, n=200) == BAD
+    assert size(1000, 100, 200) < 1000 * need / 3           # of the items of one launch
+
+
+def _muon(items, **over):
+    a = dict(items=items, count=1, dtype=0, lr=0.1, momentum=0.9, nesterov=1, wd=0.0, steps=5, a=3.4445, b=-4.775, c=2.0315,
+             eps=1e-7, ws=None, ws_bytes=0, stream=None)
+    a.update(over)
+    return _lib.lib().dance_muon_step(*a.values())
+
+
+def test_muon_refuses():
+    items = (_lib.MuonItemStruct * 2)()
+    for it in items:
+        it.param, it.grad, it.momentum, it.rows, it.cols = 64, 64, 64, 4, 8
+    size = _lib.lib().dance_muon_workspace_bytes
+    need = size(items, 2)
+    assert need == 2 * size(items, 1) > 0 and size(items, 0) == 0
+    fake = ctypes.c_void_p(64)
+    assert _muon(items, count=0) == 0 and _muon(None, count=0) == 0
+    good = dict(count=2, ws=fake, ws_bytes=need)
+    for over in (dict(count=-1), dict(dtype=5), dict(lr=float("nan")), dict(momentum=float("inf")), dict(wd=float("nan")),
+                 dict(steps=0), dict(eps=-1.0), dict(b=float("nan")), dict(ws_bytes=need - 1), dict(ws=None)):
+        assert _muon(items, **{**good, **over}) == BAD, over
+    for field, bad in (("param", 0), ("grad", 0), ("momentum", 0), ("rows", 0), ("cols", -1), ("rows", 1 << 30)):
+        keep = getattr(items[1], field)
+        setattr(items[1], field, bad)
+        assert _muon(items, **good) == BAD, field
+        setattr(items[1], field, keep)
+
+
+def test_muon_item_layout_matches_header():
+    assert ctypes.sizeof(_lib.MuonItemStruct) == 3 * 8 + 2 * 4
+
+
+def test_newton_schulz_needs_gpu_tensors_and_matrices():
+    from dance_amd import optim
+
+    with pytest.raises(RuntimeError, match="GPU tensors"):
+        ops.orthogonalize(torch.zeros((4, 4)))
+    with pytest.raises(RuntimeError, match="GPU tensors"):
+        optim.muon_step([torch.zeros((4, 4))], [torch.zeros((4, 4))], [torch.zeros((4, 4))], lr=0.1)
+    with pytest.raises(ValueError, match="not a matrix"):
+        optim.Muon([torch.zeros(4, requires_grad=True)])
+    with pytest.raises(RuntimeError, match="steps"):
+        optim.Muon([torch.zeros((4, 4), requires_grad=True)], steps=0)
+
+
+def test_rows_outermost():
+    from dance_amd.optim import _rows_outermost as f
+
+    t = torch.zeros((6, 4, 3, 3))
+    assert f(t) and f(t.to(memory_format=torch.channels_last)) and f(t[2:4]) and f(t[:1, 1:2])
+    assert not f(t.transpose(0, 1)) and not f(t[:, ::2]) and not f(t[::2]) and not f(t[:, :, :2])
+    assert f(torch.zeros((1, 9)).t()) and not f(torch.zeros((3, 9)).t())
