@@ -17,11 +17,13 @@
 // X is kept twice, with k along its columns (for X X') and along its rows (for Q X); A and Q are symmetric.
 // Rows and columns are padded with zeros to whole tiles of 64.
 //
-// One launch covers matrices of any number of shapes (up to NS_ITEMS): their descriptions travel in the kernel
-// arguments, a workgroup finds its matrix from the tile counts.
+// One launch covers matrices of any number of shapes (up to NS_ITEMS): a workgroup finds its matrix from the tile
+// counts in a table.  The first kernel gets the table as its arguments and leaves it in the workspace for the
+// others: kernel arguments lie in host memory.
 #include "common.h"
 #include "p16.h"
 
+#include <limits.h>
 #include <math.h>
 
 namespace {
@@ -29,10 +31,12 @@ namespace {
 using dance::launch_check;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
-constexpr int TILE = 64, LDT = TILE + 1;            // LDS row stride: odd, conflict-free both ways
+constexpr int PAD = 128;                            // rows and columns are padded to whole tiles of the GEMM
+constexpr int PACK = 64;                            // side of the tiles M is packed by
 constexpr int NS_ITEMS = 48;                        // 48 descriptions fit the 4 KB of kernel arguments
-constexpr int NS_SLICES = 64;                       // workgroups that share a matrix's norm
+constexpr int NS_SLICES = 256;                      // most workgroups that share a matrix's norm
 constexpr int X_EXP = 14;                           // X and A are stored times 2^14: |X|_2 < 2 (1.21 with the usual
                                                     // coefficients) keeps |A| below 65504 / 2^14
 
@@ -43,17 +47,18 @@ struct NsItem {
     char *ws;
     int m, n;
     float scale;                // Muon: lr sqrt(max(1, m / n))
-    int pad;
+    int split;                  // workgroups that share a tile of A along k
 };
+static_assert(sizeof(NsItem) == 48, "three words of 16 bytes: find_item");
 
 struct NsTable {
     NsItem it[NS_ITEMS];
-    int square[NS_ITEMS];       // workgroups up to and including item i: lower tiles of the r x r matrices
-    int rect[NS_ITEMS];         // tiles of the r x k matrices
-    int slices[NS_ITEMS];       // slices of the norm
+    // workgroups up to and including item i, INT_MAX past the last: slices of the norm; pack tiles; shares of a narrow
+    // matrix; of the others the lower tiles of A, times split; units (64 x 64) of the sum; lower tiles of Q; tiles of X
+    int slices[NS_ITEMS], pack[NS_ITEMS], narrow[NS_ITEMS], gram[NS_ITEMS], sum[NS_ITEMS], poly[NS_ITEMS], rect[NS_ITEMS];
     int count, dtype;
     long long row_stride, col_stride;                // of src, orthogonalize only
-    int muon, nesterov;
+    int muon, nesterov, steps, gram_side;            // gram_side: of the tiles of A
     float momentum, fresh, keep;        // mu, 1 - mu, 1 - lr weight_decay
     float a, b, c, q_mul;       // Q is stored times q_mul, a power of two
     double eps;
@@ -71,28 +76,37 @@ __host__ __device__ inline NsDims ns_dims(int m, int n)
     d.tall = m > n;
     d.r = d.tall ? n : m;
     d.k = d.tall ? m : n;
-    d.rp = (d.r + TILE - 1) / TILE * TILE;
-    d.kp = (d.k + TILE - 1) / TILE * TILE;
+    d.rp = (d.r + PAD - 1) / PAD * PAD;
+    d.kp = (d.k + PAD - 1) / PAD * PAD;
     return d;
 }
 
+// one tile of rows: k_ns_narrow's
+__host__ __device__ inline bool narrow(const NsDims &d) { return d.rp == PAD; }
+
+// tiles of side `side` on and below the diagonal
+__host__ __device__ inline int lower_tiles(const NsDims &d, int side) { return d.rp / side * (d.rp / side + 1) / 2; }
+
 struct NsSpace {
     double *sums;               // NS_SLICES partial sums of squares
+    float *part;                // [split][lower tile][side * side]: a tile of A summed over a share of k
     _Float16 *a, *q;            // [2][rp / 8][rp][8]
     _Float16 *xk[2], *xr[2];    // [2][kp / 8][rp][8], [2][rp / 8][kp][8]: this step's and the next one's
 };
 
-__host__ __device__ inline size_t ns_space(char *ws, const NsDims &d, NsSpace &s)
+__host__ __device__ inline size_t ns_space(char *ws, const NsDims &d, int split, NsSpace &s)
 {
     size_t at = 0;
     s.sums = (double *)(ws + at);
     at += NS_SLICES * sizeof(double);
+    s.part = (float *)(ws + at);
+    at += (size_t)split * lower_tiles(d, PAD) * PAD * PAD * sizeof(float);         // (smaller tiles are less)
     const size_t square = (size_t)d.rp * d.rp * 4, rect = (size_t)d.rp * d.kp * 4;
     s.a = (_Float16 *)(ws + at);
     at += square;
     s.q = (_Float16 *)(ws + at);
-    at += square;
-    for (int i = 0; i < 2; ++i) {
+    at += narrow(d) ? 0 : square;
+    for (int i = 0; i < (narrow(d) ? 1 : 2); ++i) {
         s.xk[i] = (_Float16 *)(ws + at);
         at += rect;
         s.xr[i] = (_Float16 *)(ws + at);
@@ -102,14 +116,35 @@ __host__ __device__ inline size_t ns_space(char *ws, const NsDims &d, NsSpace &s
 }
 
 // ---------------------------------------------------------------------------------- which matrix
-// The item that workgroup `bid` belongs to and its number there
-__device__ __forceinline__ int find_item(const int *ends, int count, int bid, int &local)
+// Workgroups are dealt to the chip's 8 dies in turn: number them so that a die's are neighbours, which share
+// operands in its L2
+__device__ __forceinline__ int die_order()
 {
-    const int lane = threadIdx.x & 63;
-    const unsigned long long behind = __ballot(lane < count && ends[lane < count ? lane : 0] <= bid);
-    const int i = __builtin_amdgcn_readfirstlane(__popcll(behind));
-    local = bid - (i ? ends[i - 1] : 0);
-    return i;
+    const int n = gridDim.x, die = blockIdx.x & 7, q = n >> 3, rest = n & 7;
+    return die * q + min(die, rest) + ((int)blockIdx.x >> 3);
+}
+
+// The item that workgroup `bid` belongs to, its index and the workgroup's number there.  ends: past the last item they
+// hold INT_MAX.  A lane reads each item's end and description, the right one is broadcast: one round trip to memory.
+__device__ __forceinline__ NsItem find_item(const NsTable &t, const int *ends, int bid, int &index, int &local)
+{
+    const int lane = min((int)(threadIdx.x & 63), NS_ITEMS - 1), end = ends[lane];
+    const int4 *from = reinterpret_cast<const int4 *>(&t.it[lane]);
+    const int4 w[3] = {from[0], from[1], from[2]};
+    index = __builtin_amdgcn_readfirstlane(min(__popcll(__ballot(end <= bid)), NS_ITEMS - 1));
+    local = bid - (index ? __builtin_amdgcn_readlane(end, index - 1) : 0);
+    union {
+        NsItem it;
+        int v[12];
+    } u;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        u.v[4 * i] = __builtin_amdgcn_readlane(w[i].x, index);
+        u.v[4 * i + 1] = __builtin_amdgcn_readlane(w[i].y, index);
+        u.v[4 * i + 2] = __builtin_amdgcn_readlane(w[i].z, index);
+        u.v[4 * i + 3] = __builtin_amdgcn_readlane(w[i].w, index);
+    }
+    return u.it;
 }
 
 // tile t of the lower triangle of a square of tiles, row by row -> (i, j), j <= i
@@ -124,55 +159,89 @@ __device__ __forceinline__ void lower_tile(int t, int &i, int &j)
 }
 
 // ------------------------------------------------------------------------------------- elements
-__device__ __forceinline__ float load_as_float(const void *p, int dtype, long long i)
-{
-    if (dtype == DANCE_F32)
-        return ((const float *)p)[i];
-    return dtype == DANCE_F16 ? (float)((const _Float16 *)p)[i] : (float)((const __bf16 *)p)[i];
-}
-
-__device__ __forceinline__ void store_as(void *p, int dtype, long long i, float v)
-{
-    if (dtype == DANCE_F32)
-        ((float *)p)[i] = v;
-    else if (dtype == DANCE_F16)
-        ((_Float16 *)p)[i] = (_Float16)v;
-    else
-        ((__bf16 *)p)[i] = (__bf16)v;
-}
-
 // Element (row, col) of what is orthogonalised.  Muon: m = mu m + (1 - mu) g (returned in `mom`), and the update
 // u = mu m + (1 - mu) g with Nesterov, m without; both in fp32, the unrounded m in u.
+template <typename T>
 __device__ __forceinline__ float element(const NsTable &t, const NsItem &it, int row, int col, float &mom)
 {
+    const long long e = t.muon ? (long long)row * it.n + col : row * t.row_stride + col * t.col_stride;
+    float g = (float)((const T *)it.src)[e];
     if (!t.muon)
-        return load_as_float(it.src, t.dtype, row * t.row_stride + col * t.col_stride);
-    const long long e = (long long)row * it.n + col;
-    const float g = load_as_float(it.src, t.dtype, e) * t.fresh;
-    mom = fmaf(load_as_float(it.momentum, t.dtype, e), t.momentum, g);
+        return g;
+    g *= t.fresh;
+    mom = fmaf((float)((const T *)it.momentum)[e], t.momentum, g);
     return t.nesterov ? fmaf(mom, t.momentum, g) : mom;
 }
 
-// sums[slice] = sum of squares of a slice of the matrix, in fp64: no square over- or underflows
-__global__ __launch_bounds__(256) void k_ns_norm(NsTable t)
+__device__ __forceinline__ double wave_sum(double x)
 {
-    __shared__ double red[4];
-    int slice;
-    const int i = find_item(t.slices, t.count, blockIdx.x, slice);
-    const NsItem it = t.it[i];
-    NsSpace s;
-    ns_space(it.ws, ns_dims(it.m, it.n), s);
-    const unsigned total = (unsigned)it.m * (unsigned)it.n, slices = t.slices[i] - (i ? t.slices[i - 1] : 0);
-    double acc = 0.0;
-#pragma unroll 4
-    for (unsigned e = slice * 256u + threadIdx.x; e < total; e += slices * 256u) {
-        float mom;
-        const float u = element(t, it, (int)(e / (unsigned)it.n), (int)(e % (unsigned)it.n), mom);
-        acc = fma((double)u, (double)u, acc);
-    }
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1)
-        acc += __shfl_xor(acc, m, 64);
+        x += __shfl_xor(x, m, 64);
+    return x;
+}
+
+// N consecutive elements of a dense matrix, at any alignment
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Word { T v[16 / sizeof(T)]; };
+
+// What `element` is, for a vector of a dense matrix: g, and in Muon m, which becomes the new momentum -> x
+template <typename T>
+__device__ __forceinline__ void elements(const NsTable &t, const Word<T> &g, Word<T> &m, float (&x)[16 / sizeof(T)])
+{
+#pragma unroll
+    for (int q = 0; q < (int)(16 / sizeof(T)); ++q) {
+        x[q] = (float)g.v[q];
+        if (t.muon) {
+            x[q] *= t.fresh;
+            const float mm = fmaf((float)m.v[q], t.momentum, x[q]);
+            m.v[q] = (T)mm;
+            x[q] = t.nesterov ? fmaf(mm, t.momentum, x[q]) : mm;
+        }
+    }
+}
+
+// the vector of the gradient and of the momentum from element e on
+template <typename T>
+__device__ __forceinline__ void load_words(const NsTable &t, const NsItem &it, long long e, Word<T> &g, Word<T> &m)
+{
+    g = *reinterpret_cast<const Word<T> *>((const T *)it.src + e);
+    if (t.muon)
+        m = *reinterpret_cast<const Word<T> *>((const T *)it.momentum + e);
+}
+
+// sums[slice] = sum of squares of a slice of the matrix, in fp64: no square over- or underflows.  DENSE: whole
+// vectors first, the rest one by one; otherwise any strides.
+template <typename T, bool DENSE> __global__ __launch_bounds__(256) void k_ns_norm(NsTable t, NsTable *kept)
+{
+    constexpr int N = 16 / sizeof(T);
+    __shared__ double red[4];
+    int i, slice;
+    const NsItem it = find_item(t, t.slices, blockIdx.x, i, slice);
+    NsSpace s;
+    ns_space(it.ws, ns_dims(it.m, it.n), it.split, s);
+    if (blockIdx.x == 0)
+        for (int w = threadIdx.x; w < (int)(sizeof(NsTable) / 4); w += 256)
+            ((int *)kept)[w] = ((const int *)&t)[w];
+    const unsigned total = (unsigned)it.m * (unsigned)it.n, slices = t.slices[i] - (i ? t.slices[i - 1] : 0);
+    const unsigned first = slice * 256u + threadIdx.x, step = slices * 256u, vectors = DENSE ? total / N : 0u;
+    double acc = 0.0;
+    if (DENSE)
+#pragma unroll 4
+        for (unsigned v = first; v < vectors; v += step) {
+            float x[N];
+            Word<T> g, m;
+            load_words<T>(t, it, (long long)v * N, g, m);
+            elements<T>(t, g, m, x);
+#pragma unroll
+            for (int q = 0; q < N; ++q)
+                acc = fma((double)x[q], (double)x[q], acc);
+        }
+    for (unsigned e = vectors * N + first; e < total; e += step) {
+        float mom;
+        const float u = element<T>(t, it, (int)(e / (unsigned)it.n), (int)(e % (unsigned)it.n), mom);
+        acc = fma((double)u, (double)u, acc);
+    }
+    acc = wave_sum(acc);
     if ((threadIdx.x & 63) == 0)
         red[threadIdx.x >> 6] = acc;
     __syncthreads();
@@ -181,285 +250,939 @@ __global__ __launch_bounds__(256) void k_ns_norm(NsTable t)
 }
 
 // ------------------------------------------------------------------------------ tiles in LDS, split
-// word: 8 consecutive k of one row, in both planes
-__device__ __forceinline__ void put_word(_Float16 *p, size_t plane, const float (&x)[8])
+// hi in the low half, lo in the high one: dance::split_half as one word
+__device__ __forceinline__ unsigned split_word(float x)
 {
-    h8 hi, lo;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        _Float16 h, l;
-        dance::split_half(x[i], h, l);
-        hi[i] = h;
-        lo[i] = l;
-    }
-    *reinterpret_cast<h8 *>(p) = hi;
-    *reinterpret_cast<h8 *>(p + plane) = lo;
+    asm("" : "+v"(x));
+    h2 p;
+    p[0] = (_Float16)x;
+    p[1] = (_Float16)(x - (float)p[0]);
+    return __builtin_bit_cast(unsigned, p);
 }
 
-// tile [i][j] -> operand with rows i (from i0 of `rows`) and k along j (from j0)
-__device__ __forceinline__ void put_rows(_Float16 *out, size_t plane, int rows, int i0, int j0, const float (*tile)[LDT])
+__device__ __forceinline__ unsigned hi_pair(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+__device__ __forceinline__ unsigned lo_pair(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+// 8 (4) consecutive k of one row into both planes
+__device__ __forceinline__ void put8(_Float16 *p, size_t plane, const unsigned (&x)[8])
 {
-    for (int w = threadIdx.x; w < TILE * TILE / 8; w += blockDim.x) {
-        const int i = w & (TILE - 1), jb = w / TILE;
-        float x[8];
+    *reinterpret_cast<uint4 *>(p) = uint4{hi_pair(x[0], x[1]), hi_pair(x[2], x[3]), hi_pair(x[4], x[5]), hi_pair(x[6], x[7])};
+    *reinterpret_cast<uint4 *>(p + plane) = uint4{lo_pair(x[0], x[1]), lo_pair(x[2], x[3]), lo_pair(x[4], x[5]), lo_pair(x[6], x[7])};
+}
+
+__device__ __forceinline__ void put4(_Float16 *p, size_t plane, unsigned a, unsigned b, unsigned c, unsigned d)
+{
+    *reinterpret_cast<uint2 *>(p) = uint2{hi_pair(a, b), hi_pair(c, d)};
+    *reinterpret_cast<uint2 *>(p + plane) = uint2{lo_pair(a, b), lo_pair(c, d)};
+}
+
+// 4 x 4 words over 4 neighbouring lanes transposed: lane l's word q becomes lane q's word l
+__device__ __forceinline__ void transpose4(unsigned (&x)[4])
+{
+    const bool odd = threadIdx.x & 1, upper = threadIdx.x & 2;
+    auto swap = [](unsigned &a, unsigned &b, bool second, auto pattern) {       // b of the first lane against a of the second
+        const unsigned sent = second ? a : b;
+        const unsigned got = (unsigned)__builtin_amdgcn_mov_dpp((int)sent, decltype(pattern)::value, 0xf, 0xf, true);
+        a = second ? got : a;
+        b = second ? b : got;
+    };
+    constexpr std::integral_constant<int, 0xB1> by1{};                   // quad_perm 1 0 3 2
+    constexpr std::integral_constant<int, 0x4E> by2{};                   // quad_perm 2 3 0 1
+    swap(x[0], x[1], odd, by1);
+    swap(x[2], x[3], odd, by1);
+    swap(x[0], x[2], upper, by2);
+    swap(x[1], x[3], upper, by2);
+}
+
+// tile [I][J] of split words in LDS, row stride J + 1 (odd: conflict-free both ways) -> operand with rows i (from i0
+// of `rows`) and k along j (from j0).  T threads.
+template <int I, int J, int T>
+__device__ __forceinline__ void put_rows(_Float16 *out, size_t plane, int rows, int i0, int j0, const unsigned *tile)
+{
+    const int i = threadIdx.x % I, jb0 = threadIdx.x / I;
+    const unsigned *from = tile + i * (J + 1) + jb0 * 8;
+    _Float16 *to = out + ((size_t)(j0 / 8 + jb0) * rows + i0 + i) * 8;
+    const size_t step = (size_t)(T / I) * rows * 8;
+#pragma unroll 4
+    for (int n = 0; n < I * J / 8 / T; ++n) {
+        unsigned x[8];
 #pragma unroll
         for (int q = 0; q < 8; ++q)
-            x[q] = tile[i][jb * 8 + q];
-        put_word(out + ((size_t)(j0 / 8 + jb) * rows + i0 + i) * 8, plane, x);
+            x[q] = from[n * (T / I) * 8 + q];
+        put8(to, plane, x);
+        to += step;
     }
 }
 
-// tile [i][j] -> operand with rows j (from j0 of `rows`) and k along i (from i0)
-__device__ __forceinline__ void put_cols(_Float16 *out, size_t plane, int rows, int i0, int j0, const float (*tile)[LDT])
+// the same tile -> operand with rows j (from j0 of `rows`) and k along i (from i0)
+template <int I, int J, int T>
+__device__ __forceinline__ void put_cols(_Float16 *out, size_t plane, int rows, int i0, int j0, const unsigned *tile)
 {
-    for (int w = threadIdx.x; w < TILE * TILE / 8; w += blockDim.x) {
-        const int j = w & (TILE - 1), ib = w / TILE;
-        float x[8];
+    const int j = threadIdx.x % J, ib0 = threadIdx.x / J;
+    const unsigned *from = tile + ib0 * 8 * (J + 1) + j;
+    _Float16 *to = out + ((size_t)(i0 / 8 + ib0) * rows + j0 + j) * 8;
+    const size_t step = (size_t)(T / J) * rows * 8;
+#pragma unroll 4
+    for (int n = 0; n < I * J / 8 / T; ++n) {
+        unsigned x[8];
 #pragma unroll
         for (int q = 0; q < 8; ++q)
-            x[q] = tile[ib * 8 + q][j];
-        put_word(out + ((size_t)(i0 / 8 + ib) * rows + j0 + j) * 8, plane, x);
+            x[q] = from[(n * (T / J) * 8 + q) * (J + 1)];
+        put8(to, plane, x);
+        to += step;
     }
 }
 
-__device__ __forceinline__ double norm_of(const double *sums, int slices, double eps)
+// 1 / max(norm, eps) as a power of two and a factor within (1, 2]: the exponents of M need not fit those of fp32's
+// reciprocals
+struct Scale {
+    int exp;
+    float by;
+    __device__ float operator()(float x) const { return ldexpf(x, exp) * by; }
+};
+
+// sum: of the squares
+__device__ __forceinline__ Scale scale_of(double sum, double eps)
 {
-    const int lane = threadIdx.x & 63;
-    double s = lane < slices ? sums[lane] : 0.0;
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1)
-        s += __shfl_xor(s, m, 64);
-    s = sqrt(s);
-    return s < eps ? eps : s;                       // (a NaN stays one)
+    double norm = sqrt(sum);
+    norm = norm < eps ? eps : norm;                 // (a NaN stays one)
+    int e;
+    const double m = frexp(norm, &e);
+    return Scale{X_EXP - e, 1.0f / (float)m};
 }
 
 // M / norm -> the first X, a tile of 64 x 64 a workgroup; Muon: the momentum is stored on the way
-__global__ __launch_bounds__(256) void k_ns_pack(NsTable t)
+template <typename T, bool DENSE> __global__ __launch_bounds__(256) void k_ns_pack(const NsTable *__restrict__ tp)
 {
-    __shared__ float tile[TILE][LDT];
-    int local;
-    const int n_item = find_item(t.rect, t.count, blockIdx.x, local);
-    const NsItem it = t.it[n_item];
+    const NsTable &t = *tp;
+    constexpr int N = 16 / sizeof(T), LD = PACK + 1;
+    __shared__ unsigned tile[PACK * LD];
+    int n_item, local;
+    const NsItem it = find_item(t, t.pack, blockIdx.x, n_item, local);
     const NsDims d = ns_dims(it.m, it.n);
     NsSpace s;
-    ns_space(it.ws, d, s);
-    const int across = d.kp / TILE, i0 = local / across * TILE, j0 = local % across * TILE;
-    const double inv = ldexp(1.0, X_EXP) / norm_of(s.sums, t.slices[n_item] - (n_item ? t.slices[n_item - 1] : 0), t.eps);
-#pragma unroll 4
-    for (int e = threadIdx.x; e < TILE * TILE; e += 256) {
-        // neighbouring threads take neighbours of a row of M
-        const int hi = e / TILE, lo = e & (TILE - 1), i = d.tall ? lo : hi, j = d.tall ? hi : lo;
-        float x = 0.0f;
-        if (i0 + i < d.r && j0 + j < d.k) {
-            const int row = d.tall ? j0 + j : i0 + i, col = d.tall ? i0 + i : j0 + j;
-            float mom;
-            x = (float)((double)element(t, it, row, col, mom) * inv);
+    ns_space(it.ws, d, it.split, s);
+    const int across = d.kp / PACK, i0 = local / across * PACK, j0 = local % across * PACK;
+    const int slices = t.slices[n_item] - (n_item ? t.slices[n_item - 1] : 0);
+    double sum = 0.0;
+    for (int i = threadIdx.x & 63; i < slices; i += 64)
+        sum += s.sums[i];
+    const Scale scaled = scale_of(wave_sum(sum), t.eps);
+    // N neighbours of a row of M at once: along j, or along i where M is tall
+    const int row0 = d.tall ? j0 : i0, col0 = d.tall ? i0 : j0;
+    const int step_j = d.tall ? LD : 1, step_i = d.tall ? 1 : LD;           // of a row and a column of M in the tile
+    if (DENSE && row0 + PACK <= it.m && col0 + PACK <= it.n) {
+        constexpr int WORDS = PACK * PACK / N / 256;
+        Word<T> g[WORDS], m[WORDS];
+        const int rr = threadIdx.x / (PACK / N), cc = threadIdx.x % (PACK / N) * N;
+        const long long e = (long long)(row0 + rr) * it.n + col0 + cc, down = 256 / (PACK / N) * (long long)it.n;
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w)
+            load_words<T>(t, it, e + w * down, g[w], m[w]);
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) {
+            float x[N];
+            elements<T>(t, g[w], m[w], x);
             if (t.muon)
-                store_as(it.momentum, t.dtype, (long long)row * it.n + col, mom);
+                *reinterpret_cast<Word<T> *>((T *)it.momentum + e + w * down) = m[w];
+#pragma unroll
+            for (int q = 0; q < N; ++q)
+                tile[(rr + w * (256 / (PACK / N))) * step_i + (cc + q) * step_j] = split_word(scaled(x[q]));
         }
-        tile[i][j] = x;
+    } else {
+#pragma unroll 8
+        for (int w = threadIdx.x; w < PACK * PACK; w += 256) {
+            const int rr = w / PACK, cc = w % PACK, row = row0 + rr, col = col0 + cc;
+            float x = 0.0f;
+            if (row < it.m && col < it.n) {
+                float mom;
+                x = element<T>(t, it, row, col, mom);
+                if (t.muon)
+                    ((T *)it.momentum)[(long long)row * it.n + col] = (T)mom;
+            }
+            tile[rr * step_i + cc * step_j] = split_word(scaled(x));
+        }
     }
     __syncthreads();
     const size_t plane = (size_t)d.rp * d.kp;
-    put_rows(s.xk[0], plane, d.rp, i0, j0, tile);
-    put_cols(s.xr[0], plane, d.kp, i0, j0, tile);
+    put_rows<PACK, PACK, 256>(s.xk[0], plane, d.rp, i0, j0, tile);
+    put_cols<PACK, PACK, 256>(s.xr[0], plane, d.kp, i0, j0, tile);
 }
 
 // ------------------------------------------------------------------------------------------- GEMM
-// acc += U[i..][k0 .. k0 + 32 steps) V[j..]': the wave's IT x JT fragments of 16 x 16.
-// u, v: this lane's words of the first fragments at k0 ((lane >> 4) is the k block, (lane & 15) the row)
-template <int IT, int JT>
-__device__ __forceinline__ void wave_gemm(f32x4 (&acc)[IT][JT], const _Float16 *u, size_t u_plane, int u_rows,
-                                          const _Float16 *v, size_t v_plane, int v_rows, int steps)
+// A square tile of side S = 32 F by 4 waves of F x F fragments of 16 x 16, three products each, k in steps of 32.  A
+// step's operands, S rows of each side, are copied from L2 to LDS without passing registers (global_load_lds_dwordx4),
+// the next step's while this one's are multiplied.
+//   F = 4 (128): per step and wave 48 MFMAs (768 clocks) stand against 16 KB read from LDS (512 clocks for all four
+//     waves); two workgroups share a compute unit, one multiplies while the other waits: 820 clocks a step.
+//   F = 2 (64): 192 against 256 clocks, so less of the chip's rate, but four times the workgroups: where 128-tiles do
+//     not give every compute unit one, a step of theirs lasts 1550 clocks, four of these 600 each.
+constexpr int STEP = 32;
+template <int F> struct Tile {
+    static constexpr int SIDE = 32 * F, LD = SIDE + 1;
+    static constexpr int SIDE_BYTES = 2 * (STEP / 8) * SIDE * 16;        // [plane][k block][row] words of 16 bytes
+    static constexpr int BUFFER = 2 * SIDE_BYTES;
+    static constexpr int LDS = 2 * BUFFER > SIDE * LD * 4 ? 2 * BUFFER : SIDE * LD * 4;      // two buffers, then the tile in 32 bits
+};
+constexpr int GEMM_THREADS = 256;
+
+struct Side {
+    const _Float16 *p;          // the operand's first row of the tile at the first k
+    size_t plane;
+    int rows;
+};
+
+__device__ __forceinline__ Side side_of(const _Float16 *op, size_t plane, int rows, int row0, int k0)
 {
-    h8 ah[IT], al[IT], bh[JT], bl[JT];
-    auto load = [&](int s) {
-        const _Float16 *us = u + (size_t)s * 4 * u_rows * 8, *vs = v + (size_t)s * 4 * v_rows * 8;
-#pragma unroll
-        for (int i = 0; i < IT; ++i) {
-            ah[i] = *reinterpret_cast<const h8 *>(us + i * 128);
-            al[i] = *reinterpret_cast<const h8 *>(us + u_plane + i * 128);
-        }
-#pragma unroll
-        for (int j = 0; j < JT; ++j) {
-            bh[j] = *reinterpret_cast<const h8 *>(vs + j * 128);
-            bl[j] = *reinterpret_cast<const h8 *>(vs + v_plane + j * 128);
-        }
-    };
-    if (steps <= 0)
-        return;
-    load(0);
-    for (int s = 0; s < steps; ++s) {
-        h8 ch[IT], cl[IT], dh[JT], dl[JT];
-#pragma unroll
-        for (int i = 0; i < IT; ++i) {
-            ch[i] = ah[i];
-            cl[i] = al[i];
-        }
-#pragma unroll
-        for (int j = 0; j < JT; ++j) {
-            dh[j] = bh[j];
-            dl[j] = bl[j];
-        }
-        if (s + 1 < steps)
-            load(s + 1);
-#pragma unroll
-        for (int i = 0; i < IT; ++i)
-#pragma unroll
-            for (int j = 0; j < JT; ++j) {
-                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(cl[i], dh[j], acc[i][j], 0, 0, 0);
-                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ch[i], dl[j], acc[i][j], 0, 0, 0);
-                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ch[i], dh[j], acc[i][j], 0, 0, 0);
-            }
-    }
+    return Side{op + ((size_t)(k0 / 8) * rows + row0) * 8, plane, rows};
 }
 
-// A 64 x 64 tile of U V' by WM x WN waves on its parts times WK waves on shares of k, summed into `tile`
-// (one buffer of TILE x LDT floats a share of k; the sum ends up in the first)
-template <int WM, int WN, int WK>
-__device__ __forceinline__ void tile_gemm(float (*tile)[LDT], const _Float16 *u, size_t u_plane, int u_rows, int i0,
-                                          const _Float16 *v, size_t v_plane, int v_rows, int j0, int k)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+// 64 words of 16 bytes, a lane each, from memory to LDS at byte `lds` on.  Inline assembly so that the compiler does
+// not wait for the copy at every LDS read; gemm_wait does before the barrier.
+__device__ __forceinline__ void copy_words(const _Float16 *from, unsigned lds)
 {
-    constexpr int IT = TILE / 16 / WM, JT = TILE / 16 / WN;
+    const unsigned l = __builtin_amdgcn_readfirstlane(lds);
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(l) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// one plane of one side of one step into LDS at byte `lds`
+template <int F> __device__ __forceinline__ void stage_plane(const Side &s, int plane, int step, unsigned lds)
+{
+    const int lane = threadIdx.x & 63;
+    const _Float16 *src = s.p + (plane ? s.plane : 0) + ((size_t)step * (STEP / 8) * s.rows + lane) * 8;
+    lds += plane * (Tile<F>::SIDE_BYTES / 2);
+#pragma unroll
+    for (int kb = 0; kb < STEP / 8; ++kb)
+#pragma unroll
+        for (int part = 0; part < F / 2; ++part)
+            copy_words(src + ((size_t)kb * s.rows + part * 64) * 8, lds + (kb * Tile<F>::SIDE + part * 64) * 16);
+}
+
+__device__ __forceinline__ void gemm_wait()
+{
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
+__device__ __forceinline__ unsigned lds_address(const void *p)
+{
+    return (unsigned)(size_t)(__attribute__((address_space(3))) const char *)p;
+}
+
+// acc = U V' over `steps` steps; same: both sides are the same rows, copied once.  lds: the kernel's dynamic LDS,
+// Tile<F>::LDS bytes; free again at return.  acc[i][j]: rows 16 i + 4 (lane / 16) .., column 16 j + lane % 16 of the
+// wave's quarter (wave / 2, wave % 2).
+template <int F>
+__device__ __forceinline__ void tile_gemm(f32x4 (&acc)[F][F], char *lds, const Side &u, const Side &v, bool same, int steps)
+{
+    constexpr int SIDE_BYTES = Tile<F>::SIDE_BYTES, SIDE = Tile<F>::SIDE;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int wk = wave / (WM * WN), wm = wave / WN % WM, wn = wave % WN;
-    const int steps = k / 32, s0 = steps * wk / WK, s1 = steps * (wk + 1) / WK;
-    f32x4 acc[IT][JT];
+    const unsigned base = lds_address(lds);
+    auto stage = [&](int step, int buffer) {
+        const unsigned to = base + buffer * Tile<F>::BUFFER;
+        if (wave < 2)
+            stage_plane<F>(u, wave, step, to);
+        else if (!same)
+            stage_plane<F>(v, wave - 2, step, to + SIDE_BYTES);
+    };
 #pragma unroll
-    for (int i = 0; i < IT; ++i)
+    for (int i = 0; i < F; ++i)
 #pragma unroll
-        for (int j = 0; j < JT; ++j)
+        for (int j = 0; j < F; ++j)
             acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const size_t kb = (size_t)s0 * 4 + (lane >> 4);
-    wave_gemm<IT, JT>(acc, u + (kb * u_rows + i0 + wm * IT * 16 + (lane & 15)) * 8, u_plane, u_rows,
-                      v + (kb * v_rows + j0 + wn * JT * 16 + (lane & 15)) * 8, v_plane, v_rows, s1 - s0);
-    // a lane holds 4 consecutive rows of one column of every fragment
-    float (*mine)[LDT] = tile + wk * TILE;
+    const int word = (lane >> 4) * SIDE + (lane & 15);
+    const char *us = lds + ((wave >> 1) * 16 * F + word) * 16;
+    const char *vs = lds + (same ? 0 : SIDE_BYTES) + ((wave & 1) * 16 * F + word) * 16;
+    stage(0, 0);
+    gemm_wait();
+    for (int s = 0; s < steps; ++s) {
+        const int now = (s & 1) * Tile<F>::BUFFER;
+        if (s + 1 < steps)
+            stage(s + 1, (s + 1) & 1);
+        h8 uh[F], ul[F], vh[F], vl[F];
+        auto load_u = [&](int i) {
+            uh[i] = *reinterpret_cast<const h8 *>(us + now + i * 256);
+            ul[i] = *reinterpret_cast<const h8 *>(us + now + SIDE_BYTES / 2 + i * 256);
+        };
+        load_u(0);
 #pragma unroll
-    for (int i = 0; i < IT; ++i)
-#pragma unroll
-        for (int j = 0; j < JT; ++j)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                mine[(wm * IT + i) * 16 + (lane >> 4) * 4 + q][(wn * JT + j) * 16 + (lane & 15)] = acc[i][j][q];
-    __syncthreads();
-    if (WK > 1) {
-        for (int e = threadIdx.x; e < TILE * TILE; e += blockDim.x) {
-            const int i = e / TILE, j = e & (TILE - 1);
-            float s = tile[i][j];
-#pragma unroll
-            for (int w = 1; w < WK; ++w)
-                s += tile[w * TILE + i][j];
-            tile[i][j] = s;
+        for (int j = 0; j < F; ++j) {
+            vh[j] = *reinterpret_cast<const h8 *>(vs + now + j * 256);
+            vl[j] = *reinterpret_cast<const h8 *>(vs + now + SIDE_BYTES / 2 + j * 256);
         }
-        __syncthreads();
+#pragma unroll
+        for (int i = 1; i < F; ++i)
+            load_u(i);
+#pragma unroll
+        for (int i = 0; i < F; ++i)
+#pragma unroll
+            for (int j = 0; j < F; ++j) {
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ul[i], vh[j], acc[i][j], 0, 0, 0);
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[i], vl[j], acc[i][j], 0, 0, 0);
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[i], vh[j], acc[i][j], 0, 0, 0);
+            }
+        gemm_wait();
     }
 }
 
-template <typename F> __device__ __forceinline__ void each(float (*tile)[LDT], F &&f)
+// this lane's first value of the tile: acc[i][j][q] lies 16 i + q rows and 16 j columns from it
+template <int F> __device__ __forceinline__ int lane_row() { return (threadIdx.x >> 7) * 16 * F + 4 * ((threadIdx.x & 63) >> 4); }
+
+template <int F> __device__ __forceinline__ int lane_col() { return (threadIdx.x >> 6 & 1) * 16 * F + (threadIdx.x & 15); }
+
+// the workgroup's tile as W = f(i, j, 4 accumulated values) of every fragment, 4 words of 32 bits, in LDS
+template <typename W, int F, typename V>
+__device__ __forceinline__ const W *tile_to_lds(const f32x4 (&acc)[F][F], char *lds, V &&f)
 {
-    for (int e = threadIdx.x; e < TILE * TILE; e += blockDim.x) {
-        const int i = e / TILE, j = e & (TILE - 1);
-        tile[i][j] = f(i, j, tile[i][j]);
-    }
+    W *mine = reinterpret_cast<W *>(lds) + lane_row<F>() * Tile<F>::LD + lane_col<F>();
+#pragma unroll
+    for (int i = 0; i < F; ++i)
+#pragma unroll
+        for (int j = 0; j < F; ++j) {
+            const f32x4 v = f(i, j, acc[i][j]);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if constexpr (std::is_same<W, unsigned>::value)
+                    mine[(16 * i + q) * Tile<F>::LD + 16 * j] = split_word(v[q]);
+                else
+                    mine[(16 * i + q) * Tile<F>::LD + 16 * j] = v[q];
+            }
+        }
     __syncthreads();
+    return reinterpret_cast<const W *>(lds);
 }
 
-// a symmetric matrix's tile at (i0, j0) and its mirror image
-__device__ __forceinline__ void put_symmetric(_Float16 *out, int rp, int i0, int j0, const float (*tile)[LDT])
+// A = X X', lower tiles, each over a share of k: the accumulators as they lie, 16 bytes a lane
+template <int F> __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_gram(const NsTable *__restrict__ tp, int step)
 {
-    const size_t plane = (size_t)rp * rp;
-    put_rows(out, plane, rp, i0, j0, tile);
-    if (i0 != j0)
-        put_cols(out, plane, rp, i0, j0, tile);
-}
-
-constexpr int GRAM_WK = 8;
-
-// A = X X', lower tiles
-__global__ __launch_bounds__(64 * GRAM_WK) void k_ns_gram(NsTable t, int step)
-{
-    extern __shared__ __align__(16) float lds[];
-    float (*tile)[LDT] = reinterpret_cast<float (*)[LDT]>(lds);
-    int local, ti, tj;
-    const NsItem it = t.it[find_item(t.square, t.count, blockIdx.x, local)];
+    const NsTable &t = *tp;
+    constexpr int SIDE = Tile<F>::SIDE;
+    extern __shared__ __align__(16) char lds[];
+    int index, local, ti, tj;
+    const NsItem it = find_item(t, t.gram, die_order(), index, local);
     const NsDims d = ns_dims(it.m, it.n);
     NsSpace s;
-    ns_space(it.ws, d, s);
-    lower_tile(local, ti, tj);
+    ns_space(it.ws, d, it.split, s);
+    const int tiles = lower_tiles(d, SIDE), share = local / tiles, all = d.kp / STEP;
+    lower_tile(local - share * tiles, ti, tj);
+    const int s0 = (int)((long long)all * share / it.split), s1 = (int)((long long)all * (share + 1) / it.split);
     const _Float16 *x = step & 1 ? s.xk[1] : s.xk[0];
     const size_t plane = (size_t)d.rp * d.kp;
-    tile_gemm<1, 1, GRAM_WK>(tile, x, plane, d.rp, ti * TILE, x, plane, d.rp, tj * TILE, d.kp);
-    const float mul = dance::pow2f(-X_EXP);
-    each(tile, [&](int, int, float v) { return v * mul; });
-    put_symmetric(s.a, d.rp, ti * TILE, tj * TILE, tile);
+    f32x4 acc[F][F];
+    tile_gemm<F>(acc, lds, side_of(x, plane, d.rp, ti * SIDE, s0 * STEP), side_of(x, plane, d.rp, tj * SIDE, s0 * STEP),
+                 ti == tj, s1 - s0);
+    f32x4 *out = reinterpret_cast<f32x4 *>(s.part + (size_t)local * SIDE * SIDE) + (threadIdx.x >> 6) * F * F * 64 + (threadIdx.x & 63);
+#pragma unroll
+    for (int i = 0; i < F; ++i)
+#pragma unroll
+        for (int j = 0; j < F; ++j)
+            out[(i * F + j) * 64] = acc[i][j];
 }
 
-// Q = a I + b A + c A A, lower tiles
-__global__ __launch_bounds__(512) void k_ns_poly(NsTable t)
+// the shares added in order, split, mirrored: 64 x 64 of A a workgroup, a quarter of a tile of 128 or a tile of 64
+__global__ __launch_bounds__(256) void k_ns_sum(const NsTable *__restrict__ tp)
 {
-    extern __shared__ __align__(16) float lds[];
-    float (*tile)[LDT] = reinterpret_cast<float (*)[LDT]>(lds);
-    int local, ti, tj;
-    const NsItem it = t.it[find_item(t.square, t.count, blockIdx.x, local)];
+    const NsTable &t = *tp;
+    constexpr int UNIT = 64, LD = UNIT + 1;
+    __shared__ unsigned tile[UNIT * LD];
+    int index, local, ti, tj;
+    const NsItem it = find_item(t, t.sum, die_order(), index, local);
     const NsDims d = ns_dims(it.m, it.n);
     NsSpace s;
-    ns_space(it.ws, d, s);
+    ns_space(it.ws, d, it.split, s);
+    const int side = narrow(d) ? PAD : t.gram_side, parts = side == PAD ? 4 : 1;
+    const int part = local & (parts - 1);
+    lower_tile(local / parts, ti, tj);
+    const size_t share = (size_t)lower_tiles(d, side) * side * side / 4;
+    const f32x4 *in = reinterpret_cast<const f32x4 *>(s.part + (size_t)(local / parts) * side * side) + part * 16 * 64 + threadIdx.x;
+    f32x4 v[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+        v[w] = in[256 * w];
+#pragma unroll 2
+    for (int k = 1; k < it.split; ++k)
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+            v[w] += in[k * share + 256 * w];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        // fragment f of the unit: 4 x 4 of a wave, or 2 x 2 of each of 4 waves
+        const int f = 4 * w + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+        const int i = parts == 4 ? f >> 2 : (f >> 3) * 2 + (f >> 1 & 1), j = parts == 4 ? f & 3 : (f >> 2 & 1) * 2 + (f & 1);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            tile[(16 * i + 4 * (lane >> 4) + q) * LD + 16 * j + (lane & 15)] = split_word(v[w][q] * dance::pow2f(-X_EXP));
+    }
+    __syncthreads();
+    const size_t plane = (size_t)d.rp * d.rp;
+    const int i0 = ti * side + (part >> 1) * UNIT, j0 = tj * side + (part & 1) * UNIT;
+    put_rows<UNIT, UNIT, 256>(s.a, plane, d.rp, i0, j0, tile);
+    if (ti != tj)
+        put_cols<UNIT, UNIT, 256>(s.a, plane, d.rp, i0, j0, tile);
+}
+
+// Q = a I + b A + c A A, lower tiles and their mirror images
+template <int F> __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_poly(const NsTable *__restrict__ tp)
+{
+    const NsTable &t = *tp;
+    constexpr int SIDE = Tile<F>::SIDE;
+    extern __shared__ __align__(16) char lds[];
+    int index, local, ti, tj;
+    const NsItem it = find_item(t, t.poly, die_order(), index, local);
+    const NsDims d = ns_dims(it.m, it.n);
+    NsSpace s;
+    ns_space(it.ws, d, it.split, s);
     lower_tile(local, ti, tj);
     const size_t plane = (size_t)d.rp * d.rp;
-    const int i0 = ti * TILE, j0 = tj * TILE;
-    tile_gemm<2, 2, 2>(tile, s.a, plane, d.rp, i0, s.a, plane, d.rp, j0, d.rp);
-    const float ca = t.c * dance::pow2f(-2 * X_EXP), ba = t.b * dance::pow2f(-X_EXP);
-    each(tile, [&](int i, int j, float v) {
-        const _Float16 *p = s.a + ((size_t)((j0 + j) / 8) * d.rp + i0 + i) * 8 + (j & 7);
-        const float aij = (float)p[0] + (float)p[plane];
-        v = fmaf(ca, v, ba * aij);
-        if (i0 + i == j0 + j && i0 + i < d.r)
-            v += t.a;
-        return v * t.q_mul;
+    const int i0 = ti * SIDE, j0 = tj * SIDE;
+    // A's own values, for the end: a lane's 4 rows of a column are, A being symmetric, 4 neighbours of that column's row
+    const int row = i0 + lane_row<F>(), col = j0 + lane_col<F>();
+    const _Float16 *p = s.a + ((size_t)(row / 8) * d.rp + col) * 8 + (row & 7);
+    h4 hi[F][F], lo[F][F];
+#pragma unroll
+    for (int i = 0; i < F; ++i)
+#pragma unroll
+        for (int j = 0; j < F; ++j) {
+            const _Float16 *pij = p + ((size_t)(2 * i) * d.rp + 16 * j) * 8;
+            hi[i][j] = *reinterpret_cast<const h4 *>(pij);
+            lo[i][j] = *reinterpret_cast<const h4 *>(pij + plane);
+        }
+    f32x4 acc[F][F];
+    tile_gemm<F>(acc, lds, side_of(s.a, plane, d.rp, i0, 0), side_of(s.a, plane, d.rp, j0, 0), ti == tj, d.rp / STEP);
+    const float ca = t.c * dance::pow2f(-2 * X_EXP) * t.q_mul, ba = t.b * dance::pow2f(-X_EXP) * t.q_mul, a = t.a * t.q_mul;
+    const unsigned *tile = tile_to_lds<unsigned>(acc, lds, [&](int i, int j, f32x4 v) {
+        const int diagonal = col + 16 * j < d.r ? col + 16 * j - row - 16 * i : -1;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            v[q] = fmaf(ca, v[q], ba * ((float)hi[i][j][q] + (float)lo[i][j][q])) + (q == diagonal ? a : 0.0f);
+        return v;
     });
-    put_symmetric(s.q, d.rp, i0, j0, tile);
+    put_rows<SIDE, SIDE, GEMM_THREADS>(s.q, plane, d.rp, i0, j0, tile);
+    if (ti != tj)
+        put_cols<SIDE, SIDE, GEMM_THREADS>(s.q, plane, d.rp, i0, j0, tile);
 }
 
-// X <- Q X, a tile of 64 x 64 a workgroup; the last step writes the result
-__global__ __launch_bounds__(256) void k_ns_apply(NsTable t, int step, int last)
+// a tile of the result, rows i and columns j of X from (i0, j0) on; Muon: the parameter's update
+template <typename T, int SIDE>
+__device__ __forceinline__ void put_result(const NsTable &t, const NsItem &it, const NsDims &d, int i0, int j0, const float *tile)
 {
-    __shared__ __align__(16) float tile[TILE][LDT];
-    int local;
-    const NsItem it = t.it[find_item(t.rect, t.count, blockIdx.x, local)];
+    const int row0 = d.tall ? j0 : i0, col = (d.tall ? i0 : j0) + (int)threadIdx.x % SIDE;
+    const int step_row = d.tall ? 1 : (SIDE + 1);
+    const float *from = tile + threadIdx.x % SIDE * (d.tall ? (SIDE + 1) : 1);
+    if (col >= it.n)
+        return;
+#pragma unroll 1
+    for (int r = threadIdx.x / SIDE; r < SIDE && row0 + r < it.m; r += 8 * (GEMM_THREADS / SIDE)) {
+        T *to = (T *)it.dst + (long long)(row0 + r) * it.n + col;
+        T old[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int rr = r + u * (GEMM_THREADS / SIDE);
+            if (t.muon && row0 + rr < it.m)
+                old[u] = to[(long long)u * (GEMM_THREADS / SIDE) * it.n];
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int rr = r + u * (GEMM_THREADS / SIDE);
+            const float v = from[rr * step_row];
+            if (row0 + rr < it.m)
+                to[(long long)u * (GEMM_THREADS / SIDE) * it.n] = (T)(t.muon ? fmaf(-it.scale, v, (float)old[u] * t.keep) : v);
+        }
+    }
+}
+
+// X <- Q X; the last step writes the result
+template <int F> __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_apply(const NsTable *__restrict__ tp, int step, int last)
+{
+    const NsTable &t = *tp;
+    constexpr int SIDE = Tile<F>::SIDE;
+    extern __shared__ __align__(16) char lds[];
+    int index, local;
+    const NsItem it = find_item(t, t.rect, die_order(), index, local);
     const NsDims d = ns_dims(it.m, it.n);
     NsSpace s;
-    ns_space(it.ws, d, s);
-    const int down = d.rp / TILE, i0 = local % down * TILE, j0 = local / down * TILE;
+    ns_space(it.ws, d, it.split, s);
+    const int down = d.rp / SIDE, i0 = local % down * SIDE, j0 = local / down * SIDE;
     const size_t square = (size_t)d.rp * d.rp, rect = (size_t)d.rp * d.kp;
-    tile_gemm<2, 2, 1>(tile, s.q, square, d.rp, i0, step & 1 ? s.xr[1] : s.xr[0], rect, d.kp, j0, d.rp);
+    f32x4 acc[F][F];
+    tile_gemm<F>(acc, lds, side_of(s.q, square, d.rp, i0, 0), side_of(step & 1 ? s.xr[1] : s.xr[0], rect, d.kp, j0, 0), false,
+              d.rp / STEP);
     const float mul = 1.0f / t.q_mul;
     if (!last) {
-        each(tile, [&](int, int, float v) { return v * mul; });
-        put_rows(step & 1 ? s.xk[0] : s.xk[1], rect, d.rp, i0, j0, tile);
-        put_cols(step & 1 ? s.xr[0] : s.xr[1], rect, d.kp, i0, j0, tile);
+        const unsigned *tile = tile_to_lds<unsigned>(acc, lds, [&](int, int, f32x4 v) { return v * mul; });
+        put_rows<SIDE, SIDE, GEMM_THREADS>(step & 1 ? s.xk[0] : s.xk[1], rect, d.rp, i0, j0, tile);
+        put_cols<SIDE, SIDE, GEMM_THREADS>(step & 1 ? s.xr[0] : s.xr[1], rect, d.kp, i0, j0, tile);
         return;
     }
     const float out = mul * dance::pow2f(-X_EXP);
-    for (int e = threadIdx.x; e < TILE * TILE; e += 256) {
-        const int hi = e / TILE, lo = e & (TILE - 1), i = d.tall ? lo : hi, j = d.tall ? hi : lo;
-        if (i0 + i >= d.r || j0 + j >= d.k)
-            continue;
-        const long long at = d.tall ? (long long)(j0 + j) * it.n + i0 + i : (long long)(i0 + i) * it.n + j0 + j;
-        float v = tile[i][j] * out;
+    const float *tile = tile_to_lds<float>(acc, lds, [&](int, int, f32x4 v) { return v * out; });
+    // neighbouring threads write neighbours of a row of M
+    if (t.dtype == DANCE_F32)
+        put_result<float, SIDE>(t, it, d, i0, j0, tile);
+    else if (t.dtype == DANCE_F16)
+        put_result<_Float16, SIDE>(t, it, d, i0, j0, tile);
+    else
+        put_result<__bf16, SIDE>(t, it, d, i0, j0, tile);
+}
+
+// ------------------------------------------------------------------------------ narrow matrices
+// Up to 128 rows: a whole step in a launch of its own and one that adds the shares of A (k_ns_sum).  A workgroup owns
+// columns of X, a tile of 128 at a time.  It takes A, computes Q (128^3, in every workgroup: cheaper than a launch),
+// replaces its columns by Q X and sums their own share of the next A.  A, then Q, and the columns lie in LDS, 64 KB
+// each; 8 waves of 64 x 32.
+constexpr int NARROW_THREADS = 512;
+constexpr int REGION = 2 * (PAD / 8) * PAD * 16;             // [plane][k block][row] words of 16 bytes
+constexpr int NARROW_LDS = 2 * REGION;
+
+__device__ __forceinline__ void narrow_gemm(f32x4 (&acc)[4][2], const char *u, const char *v)
+{
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const char *us = u + ((lane >> 4) * PAD + (wave >> 2) * 64 + (lane & 15)) * 16;
+    const char *vs = v + ((lane >> 4) * PAD + (wave & 3) * 32 + (lane & 15)) * 16;
+#pragma unroll 1
+    for (int s = 0; s < PAD / 32; ++s) {
+        h8 uh[4], ul[4], vh[2], vl[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            vh[j] = *reinterpret_cast<const h8 *>(vs + j * 256);
+            vl[j] = *reinterpret_cast<const h8 *>(vs + REGION / 2 + j * 256);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uh[i] = *reinterpret_cast<const h8 *>(us + i * 256);
+            ul[i] = *reinterpret_cast<const h8 *>(us + REGION / 2 + i * 256);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ul[i], vh[j], acc[i][j], 0, 0, 0);
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[i], vl[j], acc[i][j], 0, 0, 0);
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[i], vh[j], acc[i][j], 0, 0, 0);
+            }
+        us += 4 * PAD * 16;
+        vs += 4 * PAD * 16;
+    }
+}
+
+// f(i, j, row, col) for this lane's fragments: rows row .. row + 3 of column col
+template <typename F> __device__ __forceinline__ void narrow_each(F &&f)
+{
+    const int row = (threadIdx.x >> 8) * 64 + 4 * ((threadIdx.x & 63) >> 4), col = (threadIdx.x >> 6 & 3) * 32 + (threadIdx.x & 15);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            f(i, j, row + 16 * i, col + 16 * j);
+}
+
+__device__ __forceinline__ void zero(f32x4 (&acc)[4][2])
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+}
+
+// a symmetric matrix into a region, each value at its mirror image, where a lane's 4 are neighbours
+__device__ __forceinline__ void narrow_put_square(char *region, const f32x4 (&m)[4][2])
+{
+    narrow_each([&](int i, int j, int row, int col) {
+        unsigned x[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            x[q] = split_word(m[i][j][q]);
+        put4((_Float16 *)region + ((row >> 3) * PAD + col) * 8 + (row & 7), REGION / 4, x[0], x[1], x[2], x[3]);
+    });
+}
+
+// an operand's 128 rows and 128 k into a region, 8 pieces a wave
+__device__ __forceinline__ void narrow_stage(const _Float16 *p, size_t plane, int rows, const char *region)
+{
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const unsigned to = lds_address(region) + wave * 4 * PAD * 16;
+    const _Float16 *src = p + (wave >> 2) * plane + ((size_t)(wave & 3) * 4 * rows + lane) * 8;
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+        copy_words(src + ((size_t)(c >> 1) * rows + (c & 1) * 64) * 8, to + ((c >> 1) * PAD + (c & 1) * 64) * 16);
+}
+
+// step -1: only the first A.  The last step writes the result, and no A.
+template <typename T> __global__ __launch_bounds__(NARROW_THREADS) void k_ns_narrow(const NsTable *__restrict__ tp, int step)
+{
+    const NsTable &t = *tp;
+    extern __shared__ __align__(16) char lds[];
+    char *square = lds, *columns = lds + REGION;
+    int index, local;
+    const NsItem it = find_item(t, t.narrow, die_order(), index, local);
+    const NsDims d = ns_dims(it.m, it.n);
+    NsSpace s;
+    ns_space(it.ws, d, it.split, s);
+    const size_t rect = (size_t)PAD * d.kp, share = PAD * PAD;
+    const int tiles = d.kp / PAD, last = step + 1 == t.steps;
+    f32x4 next[4][2];
+    zero(next);
+    if (step < 0) {
+        for (int c = local; c < tiles; c += it.split) {
+            narrow_stage(s.xk[0] + (size_t)c * (PAD / 8) * PAD * 8, rect, PAD, columns);
+            gemm_wait();
+            narrow_gemm(next, columns, columns);
+            __syncthreads();
+        }
+    } else {
+        narrow_stage(s.xr[0] + (size_t)local * PAD * 8, rect, d.kp, columns);
+        narrow_stage(s.a, share, PAD, square);
+        gemm_wait();
+        f32x4 v[4][2];
+        zero(v);
+        narrow_gemm(v, square, square);
+        const float ca = t.c * dance::pow2f(-2 * X_EXP) * t.q_mul, ba = t.b * dance::pow2f(-X_EXP) * t.q_mul, one = t.a * t.q_mul;
+        narrow_each([&](int i, int j, int row, int col) {
+            // A is symmetric: 4 rows of a column are 4 neighbours of that column's row
+            const _Float16 *p = (const _Float16 *)square + ((row >> 3) * PAD + col) * 8 + (row & 7);
+            const h4 hi = *reinterpret_cast<const h4 *>(p), lo = *reinterpret_cast<const h4 *>(p + REGION / 4);
+            const int diagonal = col < d.r ? col - row : -1;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                v[i][j][q] = fmaf(ca, v[i][j][q], ba * ((float)hi[q] + (float)lo[q])) + (q == diagonal ? one : 0.0f);
+        });
+        __syncthreads();
+        narrow_put_square(square, v);
+        const float mul = 1.0f / t.q_mul;
+#pragma unroll 1
+        for (int c = local; c < tiles; c += it.split) {
+            __syncthreads();                                  // Q is there, and the columns before have been read
+            if (c != local) {
+                narrow_stage(s.xr[0] + (size_t)c * PAD * 8, rect, d.kp, columns);
+                gemm_wait();
+            }
+            zero(v);
+            narrow_gemm(v, square, columns);
+            __syncthreads();
+            if (!last) {
+                // in place, and with k along the columns for the share of A
+                _Float16 *to = s.xr[0] + (size_t)c * PAD * 8;
+                narrow_each([&](int i, int j, int row, int col) {
+                    unsigned x[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        x[q] = split_word(v[i][j][q] * mul);
+                    put4(to + ((size_t)(row >> 3) * d.kp + col) * 8 + (row & 7), rect, x[0], x[1], x[2], x[3]);
+                    transpose4(x);                            // 4 columns of row row + lane % 4
+                    put4((_Float16 *)columns + ((col >> 3) * PAD + row + (threadIdx.x & 3)) * 8 + (col & 4), REGION / 4, x[0],
+                         x[1], x[2], x[3]);
+                });
+                __syncthreads();
+                narrow_gemm(next, columns, columns);
+            } else {
+                const float out = mul * dance::pow2f(-X_EXP);
+                const int step_row = d.tall ? 1 : it.n, step_col = d.tall ? it.n : 1;
+                T *to = (T *)it.dst + (long long)c * PAD * step_col;
+                f32x4 old[4][2];
+                if (t.muon)
+                    narrow_each([&](int i, int j, int row, int col) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            if (row + q < d.r && c * PAD + col < d.k)
+                                old[i][j][q] = (float)to[(long long)(row + q) * step_row + (long long)col * step_col];
+                    });
+                narrow_each([&](int i, int j, int row, int col) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        if (row + q < d.r && c * PAD + col < d.k) {
+                            const float x = v[i][j][q] * out;
+                            to[(long long)(row + q) * step_row + (long long)col * step_col] =
+                                (T)(t.muon ? fmaf(-it.scale, x, old[i][j][q] * t.keep) : x);
+                        }
+                });
+            }
+        }
+    }
+    if (last)
+        return;
+    // where k_ns_sum looks for them: quarter by quarter of the tile, 4 x 4 fragments each
+    const int wave = threadIdx.x >> 6, quarter = (wave >> 2) * 2 + (wave >> 1 & 1);
+    f32x4 *out = reinterpret_cast<f32x4 *>(s.part + local * share) + (quarter * 16 + (wave & 1) * 2) * 64 + (threadIdx.x & 63);
+    narrow_each([&](int i, int j, int, int) { out[(i * 4 + j) * 64] = next[i][j]; });
+}
+
+// ------------------------------------------------------------------------------- small matrices
+// The whole chain of a matrix in one workgroup, X, A and Q in LDS: [plane][k / 8][row][8] as above, padded to 32.
+// 16 waves; a fragment of 16 x 16 of a product is one wave's.
+constexpr int SMALL_THREADS = 1024, SMALL_WAVES = SMALL_THREADS / 64, SMALL_PAD = 32;
+constexpr size_t SMALL_LDS = 160 * 1024;
+constexpr size_t SMALL_MOST = SMALL_LDS - 1024;
+constexpr int SMALL_SQUARE = 3;                     // fragments of Q a wave, and steps of 32 over the rows, at most:
+static_assert(12 * 128 * 128 > SMALL_MOST && 96 * 96 / 256 <= SMALL_SQUARE * SMALL_WAVES, "12 rp^2 bytes at least: rp <= 96");
+
+struct SmallDims {
+    int r, k, rp, kp, tall;
+    size_t bytes;
+};
+
+__host__ __device__ inline SmallDims small_dims(int m, int n)
+{
+    SmallDims d;
+    d.tall = m > n;
+    d.r = d.tall ? n : m;
+    d.k = d.tall ? m : n;
+    d.rp = (d.r + SMALL_PAD - 1) / SMALL_PAD * SMALL_PAD;
+    d.kp = (d.k + SMALL_PAD - 1) / SMALL_PAD * SMALL_PAD;
+    d.bytes = 8 * (size_t)d.rp * d.kp + 4 * (size_t)d.rp * d.rp;        // X both ways; A, which Q replaces
+    return d;
+}
+
+// acc += a fragment of U V' at rows i0 of U, j0 of V, k from 0 to k; operands in LDS, their planes `plane` halves apart
+__device__ __forceinline__ f32x4 small_gemm(const _Float16 *u, int u_rows, int u_plane, int i0, const _Float16 *v, int v_rows,
+                                            int v_plane, int j0, int k)
+{
+    const int lane = threadIdx.x & 63, kb = lane >> 4, row = lane & 15;
+    const _Float16 *up = u + (kb * u_rows + i0 + row) * 8, *vp = v + (kb * v_rows + j0 + row) * 8;
+    // three sums, so that a product does not wait for the one before it
+    f32x4 hh = {0.0f, 0.0f, 0.0f, 0.0f}, hl = hh, lh = hh;
+#pragma unroll 1
+    for (int s = 0; s < k; s += 32) {
+        const h8 uh = *reinterpret_cast<const h8 *>(up), ul = *reinterpret_cast<const h8 *>(up + u_plane);
+        const h8 vh = *reinterpret_cast<const h8 *>(vp), vl = *reinterpret_cast<const h8 *>(vp + v_plane);
+        lh = __builtin_amdgcn_mfma_f32_16x16x32_f16(ul, vh, lh, 0, 0, 0);
+        hl = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh, vl, hl, 0, 0, 0);
+        hh = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh, vh, hh, 0, 0, 0);
+        up += 32 * u_rows;
+        vp += 32 * v_rows;
+    }
+    return hh + (hl + lh);
+}
+
+template <typename T, bool DENSE> __global__ __launch_bounds__(SMALL_THREADS) void k_ns_small(NsTable t)
+{
+    constexpr int N = 16 / sizeof(T), WORDS = (int)(SMALL_MOST / 8 / N / SMALL_THREADS) + 1;      // vectors of M a thread
+    extern __shared__ __align__(16) char lds[];
+    __shared__ double red[SMALL_WAVES];
+    const NsItem it = t.it[blockIdx.x];
+    const SmallDims d = small_dims(it.m, it.n);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int rect = d.rp * d.kp, square = d.rp * d.rp;
+    _Float16 *xk = (_Float16 *)lds, *xr = xk + 2 * rect, *a = xr + 2 * rect;
+
+    // M (Muon: the update) once from memory, its norm on the way, then unscaled into LDS, as fp32 [i][j] where X with k
+    // along its rows and A will be
+    float *tile = reinterpret_cast<float *>(xr);
+    const int ld = d.kp + 1;                        // odd; rp (kp + 1) floats are inside xr and A
+    const int total = it.m * it.n, step_col = d.tall ? ld : 1, step_row = d.tall ? 1 : ld;
+#pragma unroll 1
+    for (int e = threadIdx.x; e < d.rp * ld; e += SMALL_THREADS)
+        tile[e] = 0.0f;
+    __syncthreads();
+    double acc = 0.0;
+    auto enter = [&](int e, float x) {
+        acc = fma((double)x, (double)x, acc);
+        const int row = (int)((unsigned)e / (unsigned)it.n), col = e - row * it.n;
+        tile[row * step_row + col * step_col] = x;
+    };
+    const int vectors = DENSE ? total / N : 0;
+    if (DENSE) {
+        Word<T> g[WORDS], m[WORDS];
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) {           // every load is issued before the first is waited for
+            const int v = threadIdx.x + w * SMALL_THREADS;
+            if (v < vectors)
+                load_words<T>(t, it, (long long)v * N, g[w], m[w]);
+        }
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) {
+            const int v = threadIdx.x + w * SMALL_THREADS;
+            if (v < vectors) {
+                float x[N];
+                elements<T>(t, g[w], m[w], x);
+#pragma unroll
+                for (int q = 0; q < N; ++q)
+                    enter(v * N + q, x[q]);
+                if (t.muon)
+                    reinterpret_cast<Word<T> *>(it.momentum)[v] = m[w];
+            }
+        }
+    }
+#pragma unroll 1
+    for (int e = vectors * N + threadIdx.x; e < total; e += SMALL_THREADS) {
+        float mom;
+        const int row = (int)((unsigned)e / (unsigned)it.n);
+        const float x = element<T>(t, it, row, e - row * it.n, mom);
         if (t.muon)
-            v = fmaf(-it.scale, v, load_as_float(it.dst, t.dtype, at) * t.keep);
-        store_as(it.dst, t.dtype, at, v);
+            ((T *)it.momentum)[e] = (T)mom;
+        enter(e, x);
+    }
+    acc = wave_sum(acc);
+    if (lane == 0)
+        red[wave] = acc;
+    __syncthreads();
+    double sum = red[0];
+#pragma unroll
+    for (int w = 1; w < SMALL_WAVES; ++w)
+        sum += red[w];
+    const Scale scaled = scale_of(sum, t.eps);
+    // X both ways.  The words that replace the tile wait in registers until everybody has read it.
+    constexpr int HELD = (int)(SMALL_MOST / 64 / SMALL_THREADS) + 1;
+    unsigned held[HELD][8];
+#pragma unroll
+    for (int n = 0; n < HELD; ++n) {
+        const int w = threadIdx.x + n * SMALL_THREADS, ib = w / d.kp, j = w - ib * d.kp;
+        if (w < rect / 8)
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                held[n][q] = split_word(scaled(tile[(ib * 8 + q) * ld + j]));
+    }
+#pragma unroll 1
+    for (int w = threadIdx.x; w < rect / 8; w += SMALL_THREADS) {
+        const int jb = w / d.rp, i = w - jb * d.rp;
+        unsigned x[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            x[q] = split_word(scaled(tile[i * ld + jb * 8 + q]));
+        put8(xk + w * 8, rect, x);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < HELD; ++n) {
+        const int w = threadIdx.x + n * SMALL_THREADS;
+        if (w < rect / 8)
+            put8(xr + w * 8, rect, held[n]);
+    }
+    __syncthreads();
+
+    const int fr = d.rp / 16, fk = d.kp / 16;
+    const int i4 = 4 * (lane >> 4), j1 = lane & 15;               // a lane's rows and column in a fragment
+    const float ca = t.c * dance::pow2f(-2 * X_EXP), ba = t.b * dance::pow2f(-X_EXP), mul = 1.0f / t.q_mul;
+    // a fragment of a symmetric matrix at (i0, j0): entered at its mirror image, where a lane's 4 values are neighbours
+    auto put_square = [&](const f32x4 &v, int i0, int j0) {
+        put4(a + (((i0 + i4) >> 3) * d.rp + j0 + j1) * 8 + (i4 & 7), square, split_word(v[0]), split_word(v[1]), split_word(v[2]),
+             split_word(v[3]));
+    };
+#pragma unroll 1
+    for (int step = 0; step < t.steps; ++step) {
+#pragma unroll 1
+        for (int f = wave; f < fr * fr; f += SMALL_WAVES) {
+            const int i0 = f / fr * 16, j0 = f % fr * 16;
+            put_square(small_gemm(xk, d.rp, rect, i0, xk, d.rp, rect, j0, d.kp) * dance::pow2f(-X_EXP), i0, j0);
+        }
+        __syncthreads();
+        f32x4 q[SMALL_SQUARE];
+#pragma unroll
+        for (int n = 0; n < SMALL_SQUARE; ++n) {
+            const int f = wave + n * SMALL_WAVES, i0 = f / fr * 16, j0 = f % fr * 16;
+            if (f >= fr * fr)
+                break;
+            q[n] = small_gemm(a, d.rp, square, i0, a, d.rp, square, j0, d.rp);
+            const _Float16 *p = a + (((i0 + i4) >> 3) * d.rp + j0 + j1) * 8 + (i4 & 7);
+            const h4 ah = *reinterpret_cast<const h4 *>(p), al = *reinterpret_cast<const h4 *>(p + square);
+            const int diagonal = j0 + j1 < d.r ? j0 + j1 - i0 - i4 : -1;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                q[n][e] = (fmaf(ca, q[n][e], ba * ((float)ah[e] + (float)al[e])) + (e == diagonal ? t.a : 0.0f)) * t.q_mul;
+        }
+        __syncthreads();                                          // every wave has read A: Q takes its place
+#pragma unroll
+        for (int n = 0; n < SMALL_SQUARE; ++n) {
+            const int f = wave + n * SMALL_WAVES;
+            if (f >= fr * fr)
+                break;
+            put_square(q[n], f / fr * 16, f % fr * 16);
+        }
+        __syncthreads();
+        // X <- Q X: a wave owns 16 columns of X at a time, holds them in registers and replaces them
+#pragma unroll 1
+        for (int f = wave; f < fk; f += SMALL_WAVES) {
+            const int j0 = f * 16, kb = lane >> 4;
+            h8 vh[SMALL_SQUARE], vl[SMALL_SQUARE];                // rp / 32 <= 3 steps of 32 rows
+#pragma unroll
+            for (int n = 0; n < SMALL_SQUARE; ++n)
+                if (n * 32 < d.rp) {
+                    const _Float16 *p = xr + ((n * 4 + kb) * d.kp + j0 + j1) * 8;
+                    vh[n] = *reinterpret_cast<const h8 *>(p);
+                    vl[n] = *reinterpret_cast<const h8 *>(p + rect);
+                }
+#pragma unroll 1
+            for (int i0 = 0; i0 < d.rp; i0 += 16) {
+                f32x4 hh = {0.0f, 0.0f, 0.0f, 0.0f}, hl = hh, lh = hh;
+#pragma unroll
+                for (int n = 0; n < SMALL_SQUARE; ++n)
+                    if (n * 32 < d.rp) {
+                        const _Float16 *p = a + ((n * 4 + kb) * d.rp + i0 + j1) * 8;
+                        const h8 uh = *reinterpret_cast<const h8 *>(p), ul = *reinterpret_cast<const h8 *>(p + square);
+                        lh = __builtin_amdgcn_mfma_f32_16x16x32_f16(ul, vh[n], lh, 0, 0, 0);
+                        hl = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh, vl[n], hl, 0, 0, 0);
+                        hh = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh, vh[n], hh, 0, 0, 0);
+                    }
+                const f32x4 x = (hh + (hl + lh)) * mul;
+                const int i = i0 + i4, j = j0 + j1;
+                if (step + 1 < t.steps) {
+                    unsigned y[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        y[e] = split_word(x[e]);
+                    put4(xr + ((i >> 3) * d.kp + j) * 8 + (i & 7), rect, y[0], y[1], y[2], y[3]);
+                    transpose4(y);                                // 4 columns of row i + lane % 4
+                    put4(xk + ((j >> 3) * d.rp + i + (lane & 3)) * 8 + (j & 4), rect, y[0], y[1], y[2], y[3]);
+                } else {
+                    const int step_i = d.tall ? 1 : it.n;
+                    T *to = (T *)it.dst + (d.tall ? j * it.n + i : i * it.n + j);
+                    const float out = dance::pow2f(-X_EXP);
+                    float old[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        old[e] = t.muon && i + e < d.r && j < d.k ? (float)to[e * step_i] * t.keep : 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (i + e < d.r && j < d.k)
+                            to[e * step_i] = (T)(t.muon ? fmaf(-it.scale, x[e] * out, old[e]) : x[e] * out);
+                }
+            }
+        }
+        __syncthreads();
     }
 }
 
 // ------------------------------------------------------------------------------------------- host
 bool known_dtype(int t) { return t == DANCE_F32 || t == DANCE_F16 || t == DANCE_BF16; }
 
-int64_t space_of(int m, int n)
+bool is_small(int m, int n) { return small_dims(m, n).bytes <= SMALL_MOST; }
+
+// Workgroups along k that a tile of A is shared by: about 256 a matrix, each with 8 steps of the GEMM at least; more
+// shares are more partial sums to add.  By the matrix alone, so that one of a batch gives the bits it gives alone.
+int split_of(const NsDims &d)
 {
-    NsSpace s;
-    return (int64_t)ns_space(nullptr, ns_dims(m, n), s);
+    if (narrow(d)) {
+        // of the column tiles, T: a share is about 1000 clocks to add, a tile 16 times that
+        const int tiles = d.kp / PAD, each = (int)sqrt(tiles / 16.0);
+        return each <= 1 ? tiles : (tiles + each - 1) / each;
+    }
+    const int want = 256 / lower_tiles(d, PAD), most = d.kp / STEP / 8, split = want < most ? want : most;
+    return split < 1 ? 1 : split > 32 ? 32 : split;
+}
+
+// the tiles' side for a launch of `tiles` tiles of 128: those where every compute unit gets one of them
+int side_for(long long tiles) { return tiles >= 256 ? 128 : 64; }
+
+// Lays out the items' shares of the workspace -> its size.  t.it[].m, n set; ws may be NULL.
+int64_t lay_out(NsTable &t, char *ws)
+{
+    bool small = true;
+    for (int i = 0; i < t.count; ++i)
+        small = small && is_small(t.it[i].m, t.it[i].n);
+    if (small)
+        return 0;
+    int64_t at = (sizeof(NsTable) + 15) & ~(size_t)15;       // the table itself comes first
+    for (int i = 0; i < t.count; ++i) {
+        const NsDims d = ns_dims(t.it[i].m, t.it[i].n);
+        NsSpace s;
+        t.it[i].split = split_of(d);
+        t.it[i].ws = ws + at;
+        at += (int64_t)ns_space(nullptr, d, t.it[i].split, s);
+    }
+    return at;
 }
 
 // the largest power of two that keeps Q's entries, |Q| <= |a| + 1.5 |b| + 2.25 |c|, within fp16
@@ -469,44 +1192,134 @@ float q_scale(float a, float b, float c)
     return most > 0.0 ? (float)exp2(fmin(14.0, floor(log2(60000.0 / most)))) : 1.0f;
 }
 
-// the chain over the items of a table whose sizes, pointers and settings are set
-int run_chain(NsTable &t, int steps, hipStream_t st, const char *fn)
+template <typename F> int with_type(int dtype, bool dense, F &&f)
 {
-    int square = 0, rect = 0, slices = 0;
+    if (dtype == DANCE_F32)
+        return dense ? f((float)0, std::true_type{}) : f((float)0, std::false_type{});
+    if (dtype == DANCE_F16)
+        return dense ? f((_Float16)0, std::true_type{}) : f((_Float16)0, std::false_type{});
+    return dense ? f((__bf16)0.0f, std::true_type{}) : f((__bf16)0.0f, std::false_type{});
+}
+
+// The chain over the items of a table whose sizes, pointers and settings are set.  Matrices that all fit a compute
+// unit's LDS are done in one launch, a workgroup each.
+int run_chain(NsTable &t, char *ws, hipStream_t st, const char *fn)
+{
+    bool dense = true;
+    for (int i = 0; i < t.count; ++i)
+        dense = dense && (t.muon || (t.col_stride == 1 && (t.row_stride == t.it[i].n || t.it[i].m == 1)));
+    if (lay_out(t, ws) == 0) {
+        size_t lds = 0;
+        for (int i = 0; i < t.count; ++i) {
+            const size_t bytes = small_dims(t.it[i].m, t.it[i].n).bytes;
+            lds = bytes > lds ? bytes : lds;
+        }
+        return with_type(t.dtype, dense, [&](auto type, auto is_dense) {
+            using T = decltype(type);
+            constexpr bool D = decltype(is_dense)::value;
+            if (int rc = dance::allow_lds((const void *)k_ns_small<T, D>, lds, fn))
+                return rc;
+            hipLaunchKernelGGL((k_ns_small<T, D>), dim3(t.count), dim3(SMALL_THREADS), lds, st, t);
+            return launch_check(fn);
+        });
+    }
+    long long slices = 0, pack = 0, narrows = 0, gram = 0, sum = 0, poly = 0, rect = 0;
     for (int i = 0; i < t.count; ++i) {
         const NsDims d = ns_dims(t.it[i].m, t.it[i].n);
-        const int down = d.rp / TILE, across = d.kp / TILE;
-        const long long total = (long long)t.it[i].m * t.it[i].n, want = (total + 4095) / 4096;
-        if ((long long)rect + (long long)down * across >= (1ll << 31) || (long long)square + (long long)down * (down + 1) / 2 >= (1ll << 31))
+        if (!narrow(d)) {
+            gram += (long long)lower_tiles(d, PAD) * t.it[i].split;
+            poly += lower_tiles(d, PAD);
+            rect += (long long)(d.rp / PAD) * (d.kp / PAD);
+        }
+    }
+    const int gram_side = t.gram_side = side_for(gram), poly_side = side_for(poly), rect_side = side_for(rect);
+    gram = poly = rect = 0;
+    for (int i = t.count; i < NS_ITEMS; ++i)
+        t.slices[i] = t.pack[i] = t.narrow[i] = t.gram[i] = t.sum[i] = t.poly[i] = t.rect[i] = INT_MAX;
+    for (int i = 0; i < t.count; ++i) {
+        const NsDims d = ns_dims(t.it[i].m, t.it[i].n);
+        const long long want = ((long long)t.it[i].m * t.it[i].n + 8191) / 8192;
+        slices += want < NS_SLICES ? want : NS_SLICES;
+        pack += (long long)(d.rp / PACK) * (d.kp / PACK);
+        if (narrow(d)) {
+            narrows += t.it[i].split;
+            sum += 4;
+        } else {
+            gram += (long long)lower_tiles(d, gram_side) * t.it[i].split;
+            sum += (long long)lower_tiles(d, gram_side) * (gram_side == PAD ? 4 : 1);
+            poly += lower_tiles(d, poly_side);
+            rect += (long long)(d.rp / rect_side) * (d.kp / rect_side);
+        }
+        if (pack >= (1ll << 31) || gram >= (1ll << 31) || sum >= (1ll << 31) || rect >= (1ll << 31) || narrows >= (1ll << 31))
             return dance::fail((int)hipErrorInvalidValue, fn, "too many tiles");
-        square += down * (down + 1) / 2;
-        rect += down * across;
-        slices += (int)(want < NS_SLICES ? want : NS_SLICES);
-        t.square[i] = square;
-        t.rect[i] = rect;
-        t.slices[i] = slices;
+        t.slices[i] = (int)slices;
+        t.pack[i] = (int)pack;
+        t.narrow[i] = (int)narrows;
+        t.gram[i] = (int)gram;
+        t.sum[i] = (int)sum;
+        t.poly[i] = (int)poly;
+        t.rect[i] = (int)rect;
     }
-    const size_t gram_lds = GRAM_WK * TILE * LDT * sizeof(float), poly_lds = 2 * TILE * LDT * sizeof(float);
-    if (int rc = dance::allow_lds((const void *)k_ns_gram, gram_lds, fn))
-        return rc;
-    hipLaunchKernelGGL(k_ns_norm, dim3(slices), dim3(256), 0, st, t);
-    if (int rc = launch_check(fn))
-        return rc;
-    hipLaunchKernelGGL(k_ns_pack, dim3(rect), dim3(256), 0, st, t);
-    if (int rc = launch_check(fn))
-        return rc;
-    for (int s = 0; s < steps; ++s) {
-        hipLaunchKernelGGL(k_ns_gram, dim3(square), dim3(64 * GRAM_WK), gram_lds, st, t, s);
-        if (int rc = launch_check(fn))
-            return rc;
-        hipLaunchKernelGGL(k_ns_poly, dim3(square), dim3(512), poly_lds, st, t);
-        if (int rc = launch_check(fn))
-            return rc;
-        hipLaunchKernelGGL(k_ns_apply, dim3(rect), dim3(256), 0, st, t, s, (int)(s + 1 == steps));
-        if (int rc = launch_check(fn))
-            return rc;
-    }
-    return 0;
+    NsTable *kept = (NsTable *)ws;
+    auto with_side = [&](int side, auto &&f) {
+        return side == 128 ? f(std::integral_constant<int, 4>{}) : f(std::integral_constant<int, 2>{});
+    };
+    return with_type(t.dtype, dense, [&](auto type, auto is_dense) {
+        using T = decltype(type);
+        constexpr bool D = decltype(is_dense)::value;
+        hipLaunchKernelGGL((k_ns_norm<T, D>), dim3((unsigned)slices), dim3(256), 0, st, t, kept);
+        if (int e = launch_check(fn))
+            return e;
+        hipLaunchKernelGGL((k_ns_pack<T, D>), dim3((unsigned)pack), dim3(256), 0, st, (const NsTable *)kept);
+        if (int e = launch_check(fn))
+            return e;
+        if (int e = dance::allow_lds((const void *)k_ns_narrow<T>, NARROW_LDS, fn))
+            return e;
+        // step s of the X of all matrices, and the A of the next step; X itself is the -1st
+        for (int s = -1; s < t.steps; ++s) {
+            const int last = s + 1 == t.steps;
+            int e = 0;
+            if (narrows > 0) {
+                hipLaunchKernelGGL(k_ns_narrow<T>, dim3((unsigned)narrows), dim3(NARROW_THREADS), NARROW_LDS, st,
+                                   (const NsTable *)kept, s);
+                e = launch_check(fn);
+            }
+            if (e == 0 && rect > 0 && s >= 0)
+                e = with_side(poly_side, [&](auto f) {
+                    constexpr int F = decltype(f)::value;
+                    if (int r = dance::allow_lds((const void *)k_ns_poly<F>, Tile<F>::LDS, fn))
+                        return r;
+                    hipLaunchKernelGGL(k_ns_poly<F>, dim3((unsigned)poly), dim3(GEMM_THREADS), Tile<F>::LDS, st,
+                                       (const NsTable *)kept);
+                    return launch_check(fn);
+                });
+            if (e == 0 && rect > 0 && s >= 0)
+                e = with_side(rect_side, [&](auto f) {
+                    constexpr int F = decltype(f)::value;
+                    if (int r = dance::allow_lds((const void *)k_ns_apply<F>, Tile<F>::LDS, fn))
+                        return r;
+                    hipLaunchKernelGGL(k_ns_apply<F>, dim3((unsigned)rect), dim3(GEMM_THREADS), Tile<F>::LDS, st,
+                                       (const NsTable *)kept, s, last);
+                    return launch_check(fn);
+                });
+            if (e == 0 && rect > 0 && !last)
+                e = with_side(gram_side, [&](auto f) {
+                    constexpr int F = decltype(f)::value;
+                    if (int r = dance::allow_lds((const void *)k_ns_gram<F>, Tile<F>::LDS, fn))
+                        return r;
+                    hipLaunchKernelGGL(k_ns_gram<F>, dim3((unsigned)gram), dim3(GEMM_THREADS), Tile<F>::LDS, st,
+                                       (const NsTable *)kept, s + 1);
+                    return launch_check(fn);
+                });
+            if (e == 0 && !last) {
+                hipLaunchKernelGGL(k_ns_sum, dim3((unsigned)sum), dim3(256), 0, st, (const NsTable *)kept);
+                e = launch_check(fn);
+            }
+            if (e)
+                return e;
+        }
+        return 0;
+    });
 }
 
 bool usable(double a, double b, double c) { return isfinite(a) && isfinite(b) && isfinite(c); }
@@ -517,7 +1330,13 @@ extern "C" int64_t dance_orthogonalize_workspace_bytes(int batch, int m, int n)
 {
     if (batch <= 0 || m <= 0 || n <= 0 || (long long)m * n >= (1ll << 31))
         return 0;
-    return (batch < NS_ITEMS ? batch : NS_ITEMS) * space_of(m, n);
+    NsTable t;
+    t.count = batch < NS_ITEMS ? batch : NS_ITEMS;
+    for (int i = 0; i < t.count; ++i) {
+        t.it[i].m = m;
+        t.it[i].n = n;
+    }
+    return lay_out(t, nullptr);
 }
 
 extern "C" int dance_orthogonalize(const void *x, int64_t batch_stride, int64_t row_stride, int64_t col_stride,
@@ -529,9 +1348,10 @@ extern "C" int dance_orthogonalize(const void *x, int64_t batch_stride, int64_t 
     DANCE_REQUIRE(batch_stride >= 0 && row_stride >= 0 && col_stride >= 0);
     if (batch == 0 || m == 0 || n == 0)
         return 0;
-    DANCE_REQUIRE(x && out && ws && ((uintptr_t)ws & 15) == 0);
-    DANCE_REQUIRE(ws_bytes >= dance_orthogonalize_workspace_bytes(batch, m, n));
-    const int64_t size = dtype == DANCE_F32 ? 4 : 2, space = space_of(m, n);
+    const int64_t need = dance_orthogonalize_workspace_bytes(batch, m, n);
+    DANCE_REQUIRE(x && out && ((uintptr_t)ws & 15) == 0);
+    DANCE_REQUIRE(ws_bytes >= need && (ws || need == 0));
+    const int64_t size = dtype == DANCE_F32 ? 4 : 2;
     for (int b0 = 0; b0 < batch; b0 += NS_ITEMS) {
         NsTable t;
         memset(&t, 0, sizeof t);
@@ -539,17 +1359,17 @@ extern "C" int dance_orthogonalize(const void *x, int64_t batch_stride, int64_t 
         t.dtype = dtype;
         t.row_stride = row_stride;
         t.col_stride = col_stride;
+        t.steps = steps;
         t.a = a; t.b = b; t.c = c;
         t.q_mul = q_scale(a, b, c);
         t.eps = (double)eps;
         for (int i = 0; i < t.count; ++i) {
             t.it[i].src = (const char *)x + (b0 + i) * batch_stride * size;
             t.it[i].dst = (char *)out + (int64_t)(b0 + i) * m * n * size;
-            t.it[i].ws = (char *)ws + i * space;
             t.it[i].m = m;
             t.it[i].n = n;
         }
-        if (int rc = run_chain(t, steps, (hipStream_t)stream, __func__))
+        if (int rc = run_chain(t, (char *)ws, (hipStream_t)stream, __func__))
             return rc;
     }
     return 0;
@@ -561,14 +1381,17 @@ extern "C" int64_t dance_muon_workspace_bytes(const dance_muon_item *items_host,
         return 0;
     int64_t most = 0;
     for (int b0 = 0; b0 < count; b0 += NS_ITEMS) {
-        int64_t sum = 0;
-        for (int i = b0; i < count && i < b0 + NS_ITEMS; ++i) {
-            const int m = items_host[i].rows, n = items_host[i].cols;
+        NsTable t;
+        t.count = count - b0 < NS_ITEMS ? count - b0 : NS_ITEMS;
+        for (int i = 0; i < t.count; ++i) {
+            const int m = items_host[b0 + i].rows, n = items_host[b0 + i].cols;
             if (m <= 0 || n <= 0 || (long long)m * n >= (1ll << 31))
                 return 0;
-            sum += space_of(m, n);
+            t.it[i].m = m;
+            t.it[i].n = n;
         }
-        most = sum > most ? sum : most;
+        const int64_t bytes = lay_out(t, nullptr);
+        most = bytes > most ? bytes : most;
     }
     return most;
 }
@@ -581,13 +1404,14 @@ extern "C" int dance_muon_step(const dance_muon_item *items_host, int count, int
     DANCE_REQUIRE(usable(lr, momentum, weight_decay));
     if (count == 0)
         return 0;
-    DANCE_REQUIRE(items_host && ws && ((uintptr_t)ws & 15) == 0);
+    DANCE_REQUIRE(items_host && ((uintptr_t)ws & 15) == 0);
     for (int i = 0; i < count; ++i) {
         DANCE_REQUIRE(items_host[i].param && items_host[i].grad && items_host[i].momentum);
         DANCE_REQUIRE(items_host[i].rows >= 1 && items_host[i].cols >= 1);
         DANCE_REQUIRE((long long)items_host[i].rows * items_host[i].cols < (1ll << 31));
     }
-    DANCE_REQUIRE(ws_bytes >= dance_muon_workspace_bytes(items_host, count));
+    const int64_t need = dance_muon_workspace_bytes(items_host, count);
+    DANCE_REQUIRE(ws_bytes >= need && (ws || need == 0));
     for (int b0 = 0; b0 < count; b0 += NS_ITEMS) {
         NsTable t;
         memset(&t, 0, sizeof t);
@@ -598,23 +1422,21 @@ extern "C" int dance_muon_step(const dance_muon_item *items_host, int count, int
         t.momentum = (float)momentum;
         t.fresh = (float)(1.0 - momentum);
         t.keep = (float)(1.0 - lr * weight_decay);
+        t.steps = steps;
         t.a = a; t.b = b; t.c = c;
         t.q_mul = q_scale(a, b, c);
         t.eps = (double)eps;
-        int64_t at = 0;
         for (int i = 0; i < t.count; ++i) {
             const dance_muon_item &h = items_host[b0 + i];
             t.it[i].src = h.grad;
             t.it[i].momentum = h.momentum;
             t.it[i].dst = h.param;
-            t.it[i].ws = (char *)ws + at;
             t.it[i].m = h.rows;
             t.it[i].n = h.cols;
             const double shape = h.rows > h.cols ? sqrt((double)h.rows / (double)h.cols) : 1.0;
             t.it[i].scale = (float)(lr * shape);
-            at += space_of(h.rows, h.cols);
         }
-        if (int rc = run_chain(t, steps, (hipStream_t)stream, __func__))
+        if (int rc = run_chain(t, (char *)ws, (hipStream_t)stream, __func__))
             return rc;
     }
     return 0;
