@@ -117,7 +117,7 @@ SIGNATURES = {
                                     c_float, c_float, P, c_int64, P]),
     "dance_muon_workspace_bytes": (c_int64, [POINTER(MuonItemStruct), c_int]),
     "dance_muon_step": (c_int, [POINTER(MuonItemStruct), c_int, c_int, c_double, c_double, c_int, c_double, c_int, c_float,
-                                c_float, c_float, c_float, P, c_int64, P]),
+                                c_float, c_float, c_float, P, c_int64, P, P]),
     "dance_nms_sorted": (c_int, [P, c_int, c_float, P, P, P, P]),
     "dance_nms_sorted_plain": (c_int, [P, c_int, c_float, P, P, P, P]),
     "dance_nms_sorted_plain_static": (c_int, [P, c_int, c_float, P, P, P]),

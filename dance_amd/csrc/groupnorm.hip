@@ -26,6 +26,12 @@ template <typename T> struct Vec { static constexpr int N = 16 / (int)sizeof(T);
 // channel slice): the hardware takes unaligned 128-bit accesses
 template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Word { T v[16 / sizeof(T)]; };
 
+// Reads and writes of maps larger than the 256 MB cache can serve twice bypass it (STREAM): what is read for the last
+// time and what is written would only push out what is read again.  (8, 256, 200, 304) fp32, us: statistics 124 -> 86,
+// because they no longer wait for the outputs of the call before to be written back, apply 176 -> 158.  Not where in-
+// and output fit: there the next layer finds its input in the cache.
+typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+
 __device__ __forceinline__ float load_affine(const void *p, int dtype, int i, float otherwise)
 {
     if (p == nullptr)
@@ -62,9 +68,12 @@ template <typename T, bool WHOLE> __device__ __forceinline__ int channel_of(cons
 }
 
 // pixel: the slab's first channel
-template <typename T, bool WHOLE>
+template <typename T, bool WHOLE, bool STREAM = false>
 __device__ __forceinline__ Word<T> load_word(const T *pixel, const GnDims &d, int v)
 {
+    if (WHOLE && STREAM)
+        return __builtin_bit_cast(
+            Word<T>, __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(pixel + v * Vec<T>::N)));
     if (WHOLE)
         return *reinterpret_cast<const Word<T> *>(pixel + v * Vec<T>::N);
     Word<T> w;
@@ -76,9 +85,13 @@ __device__ __forceinline__ Word<T> load_word(const T *pixel, const GnDims &d, in
     return w;
 }
 
-template <typename T, bool WHOLE>
+template <typename T, bool WHOLE, bool STREAM = false>
 __device__ __forceinline__ void store_word(T *pixel, const Word<T> &w, const GnDims &d, int v)
 {
+    if (WHOLE && STREAM) {
+        __builtin_nontemporal_store(__builtin_bit_cast(u32x4_any, w), reinterpret_cast<u32x4_any *>(pixel + v * Vec<T>::N));
+        return;
+    }
     if (WHOLE) {
         *reinterpret_cast<Word<T> *>(pixel + v * Vec<T>::N) = w;
         return;
@@ -207,7 +220,7 @@ template <bool WHOLE> constexpr int IN_FLIGHT = WHOLE ? 8 : 2;
 
 // FL pixels of a thread from pixel p on, rows apart; those past the chunk are its last one again, so that
 // every load is issued
-template <typename T, bool WHOLE, int FL>
+template <typename T, bool WHOLE, bool STREAM, int FL>
 __device__ __forceinline__ void load_batch(Word<T> (&w)[FL], const T *x, long long pixel_stride, long long p, long long p1,
                                            const GnDims &d, int v)
 {
@@ -216,11 +229,11 @@ __device__ __forceinline__ void load_batch(Word<T> (&w)[FL], const T *x, long lo
         const long long step = d.rows * pixel_stride;
 #pragma unroll
         for (int u = 0; u < FL; ++u)
-            w[u] = load_word<T, WHOLE>(xp + u * step, d, v);
+            w[u] = load_word<T, WHOLE, STREAM>(xp + u * step, d, v);
     } else {
 #pragma unroll
         for (int u = 0; u < FL; ++u)
-            w[u] = load_word<T, WHOLE>(x + min(p + u * d.rows, p1 - 1) * pixel_stride, d, v);
+            w[u] = load_word<T, WHOLE, STREAM>(x + min(p + u * d.rows, p1 - 1) * pixel_stride, d, v);
     }
 }
 
@@ -254,10 +267,10 @@ __global__ __launch_bounds__(MAX_THREADS) void k_gn_stats(const T *__restrict__ 
         const T *xp = x + b * image_stride;
         Word<T> w[FL], next[FL];
         long long p = p0 + row;
-        load_batch<T, WHOLE>(w, xp, pixel_stride, p, p1, d, v);
+        load_batch<T, WHOLE, false>(w, xp, pixel_stride, p, p1, d, v);
         for (; p < p1; p += FL * d.rows) {
             if (p + FL * d.rows < p1)
-                load_batch<T, WHOLE>(next, xp, pixel_stride, p + FL * d.rows, p1, d, v);
+                load_batch<T, WHOLE, false>(next, xp, pixel_stride, p + FL * d.rows, p1, d, v);
             for_batch<FL>(p, p1, d.rows, [&](int u) { add_word<T>(s, q, w[u]); });
 #pragma unroll
             for (int u = 0; u < FL; ++u)
@@ -385,7 +398,7 @@ template <typename T> __device__ __forceinline__ Word<T> apply_word(const Word<T
 }
 
 // grid: b * nch workgroups, slab = the whole map
-template <typename T, bool WHOLE, int ACT>
+template <typename T, bool WHOLE, int ACT, bool STREAM>
 __global__ __launch_bounds__(MAX_THREADS) void k_gn_apply(const T *__restrict__ x, long long image_stride,
                                                           long long pixel_stride, const Channel *__restrict__ channels,
                                                           T *__restrict__ y, GnDims d)
@@ -400,7 +413,7 @@ __global__ __launch_bounds__(MAX_THREADS) void k_gn_apply(const T *__restrict__ 
     T *yp = y + b * d.hw * d.c;
     Word<T> w[FL], next[FL];
     long long p = p0 + row;
-    load_batch<T, WHOLE>(w, xp, pixel_stride, p, p1, d, v);        // in flight while the constants arrive
+    load_batch<T, WHOLE, STREAM>(w, xp, pixel_stride, p, p1, d, v);        // in flight while the constants arrive
     Channel k[N];
 #pragma unroll
     for (int j = 0; j < N; ++j)
@@ -408,9 +421,9 @@ __global__ __launch_bounds__(MAX_THREADS) void k_gn_apply(const T *__restrict__ 
     const long long step = (long long)d.rows * d.c;
     for (; p < p1; p += FL * d.rows) {
         if (p + FL * d.rows < p1)
-            load_batch<T, WHOLE>(next, xp, pixel_stride, p + FL * d.rows, p1, d, v);
+            load_batch<T, WHOLE, STREAM>(next, xp, pixel_stride, p + FL * d.rows, p1, d, v);
         T *yq = yp + p * d.c;
-        for_batch<FL>(p, p1, d.rows, [&](int u) { store_word<T, WHOLE>(yq + u * step, apply_word<T>(w[u], k, ACT), d, v); });
+        for_batch<FL>(p, p1, d.rows, [&](int u) { store_word<T, WHOLE, STREAM>(yq + u * step, apply_word<T>(w[u], k, ACT), d, v); });
 #pragma unroll
         for (int u = 0; u < FL; ++u)
             w[u] = next[u];
@@ -527,8 +540,8 @@ __global__ __launch_bounds__(MAX_THREADS) void k_gn_grad_sums(const T *__restric
         const T *xp = x + b * image_stride, *dp = dy + b * dy_image;
         Word<T> w[FL], g[FL];
         long long p = p0 + row;
-        load_batch<T, WHOLE>(w, xp, pixel_stride, p, p1, d, v);
-        load_batch<T, WHOLE>(g, dp, dy_pixel, p, p1, d, v);
+        load_batch<T, WHOLE, false>(w, xp, pixel_stride, p, p1, d, v);
+        load_batch<T, WHOLE, false>(g, dp, dy_pixel, p, p1, d, v);
         Channel k[N];
         float s[N], q[N];
 #pragma unroll
@@ -550,8 +563,8 @@ __global__ __launch_bounds__(MAX_THREADS) void k_gn_grad_sums(const T *__restric
             });
             p += FL * d.rows;
             if (p < p1) {
-                load_batch<T, WHOLE>(w, xp, pixel_stride, p, p1, d, v);
-                load_batch<T, WHOLE>(g, dp, dy_pixel, p, p1, d, v);
+                load_batch<T, WHOLE, false>(w, xp, pixel_stride, p, p1, d, v);
+                load_batch<T, WHOLE, false>(g, dp, dy_pixel, p, p1, d, v);
             }
         }
 #pragma unroll
@@ -567,53 +580,48 @@ __global__ __launch_bounds__(MAX_THREADS) void k_gn_grad_sums(const T *__restric
         *reinterpret_cast<float2 *>(out + c * 2) = float2{redf[c][0], redf[c][1] * (float)st[c / d.gc * 2 + 1]};
 }
 
-// partial (b, nch, c, 2) -> sums (b, c, 2) in fp64 and a group's a1, a2 of grad_x.  grid: (groups, b).
-__global__ __launch_bounds__(256) void k_gn_grad_finish(const float *__restrict__ partial, Saved saved,
-                                                        double *__restrict__ sums, float2 *__restrict__ means, GnDims d)
+// partial (b, nch, c, 2) -> sums (b, c, 2) in fp64 and a group's a1, a2 of grad_x.  grid: (groups, b).  Neighbouring
+// threads read neighbouring channels of a chunk, the chunks are dealt to rows of threads.
+__global__ __launch_bounds__(MAX_THREADS) void k_gn_grad_finish(const float *__restrict__ partial, Saved saved,
+                                                                double *__restrict__ sums, float2 *__restrict__ means,
+                                                                GnDims d)
 {
-    __shared__ double red[256 * 2];
+    __shared__ __align__(16) double red[MAX_THREADS][2];
     const int g = blockIdx.x, b = blockIdx.y;
-    double m1 = 0.0, m2 = 0.0;
-    // a channel is folded by `lanes` threads (a power of two), the block takes 256 / lanes channels at once
-    int lanes = 64;
-    while (lanes > 1 && lanes * d.gc > 256)
-        lanes >>= 1;
-    const int sub = threadIdx.x / lanes, lane = threadIdx.x - sub * lanes;
-    for (int c0 = 0; c0 < d.gc; c0 += 256 / lanes) {
-        const int cl = c0 + sub, c = g * d.gc + cl;
-        double s = 0.0, q = 0.0;
-        if (cl < d.gc)
+    double m1 = 0.0, m2 = 0.0;                            // thread 0's
+    for (int c0 = 0; c0 < d.gc; c0 += MAX_THREADS) {
+        const int width = min(d.gc - c0, MAX_THREADS), rows = MAX_THREADS / width;
+        const int row = threadIdx.x / width, cl = threadIdx.x - row * width, c = g * d.gc + c0 + cl;
+        __syncthreads();                                  // (the channels before have been read)
+        if (row < rows) {
+            double s = 0.0, q = 0.0;
 #pragma unroll 8
-            for (int i = lane; i < d.nch; i += lanes) {
+            for (int i = row; i < d.nch; i += rows) {
                 const float2 p = *reinterpret_cast<const float2 *>(partial + (((long long)b * d.nch + i) * d.c + c) * 2);
                 s += (double)p.x;
                 q += (double)p.y;
             }
-        for (int m = lanes >> 1; m >= 1; m >>= 1) {
-            s += __shfl_xor(s, m, 64);
-            q += __shfl_xor(q, m, 64);
+            red[row * width + cl][0] = s;
+            red[row * width + cl][1] = q;
         }
-        if (cl < d.gc && lane == 0) {
+        fold_rows(red, rows, width);
+        if (row == 0) {
+            const double s = red[cl][0], q = red[cl][1], w = (double)saved.weight[c];
             sums[((long long)b * d.c + c) * 2] = s;
             sums[((long long)b * d.c + c) * 2 + 1] = q;
-            const double w = (double)saved.weight[c];
-            m1 += w * s;
-            m2 += w * q;
-        }
-    }
-    red[threadIdx.x * 2] = m1;
-    red[threadIdx.x * 2 + 1] = m2;
-    __syncthreads();
-    for (int h = 128; h >= 1; h >>= 1) {
-        if ((int)threadIdx.x < h) {
-            red[threadIdx.x * 2] += red[(threadIdx.x + h) * 2];
-            red[threadIdx.x * 2 + 1] += red[(threadIdx.x + h) * 2 + 1];
+            red[cl][0] = w * s;
+            red[cl][1] = w * q;
         }
         __syncthreads();
+        const double (*weighted)[2] = red;
+        for_group_sums(weighted, 1, width, [&](int, double s, double q) {
+            m1 += s;
+            m2 += q;
+        });
     }
     if (threadIdx.x == 0) {
         const double count = (double)d.gc * (double)d.hw, rstd = saved.stats[((long long)b * d.groups + g) * 2 + 1];
-        means[(long long)b * d.groups + g] = float2{(float)(rstd * red[0] / count), (float)(rstd * rstd * red[1] / count)};
+        means[(long long)b * d.groups + g] = float2{(float)(rstd * m1 / count), (float)(rstd * rstd * m2 / count)};
     }
 }
 
@@ -642,7 +650,7 @@ __global__ __launch_bounds__(64) void k_gn_grad_affine(const double *__restrict_
 
 // grid: b * nch workgroups, slab = the whole map; dx may be NULL (only dw, dbeta wanted: one workgroup then).
 // The last workgroups write dw and dbeta, too: no launch of their own.
-template <typename T, bool WHOLE, int ACT>
+template <typename T, bool WHOLE, int ACT, bool STREAM>
 __global__ __launch_bounds__(MAX_THREADS) void k_gn_grad_apply(const T *__restrict__ dy, long long dy_image,
                                                                long long dy_pixel, const T *__restrict__ x,
                                                                long long image_stride, long long pixel_stride, Saved saved,
@@ -664,8 +672,8 @@ __global__ __launch_bounds__(MAX_THREADS) void k_gn_grad_apply(const T *__restri
     T *op = dx + b * d.hw * d.c;
     Word<T> w[FL], g[FL];
     long long p = p0 + row;
-    load_batch<T, WHOLE>(w, xp, pixel_stride, p, p1, d, v);
-    load_batch<T, WHOLE>(g, dp, dy_pixel, p, p1, d, v);
+    load_batch<T, WHOLE, STREAM>(w, xp, pixel_stride, p, p1, d, v);
+    load_batch<T, WHOLE, STREAM>(g, dp, dy_pixel, p, p1, d, v);
     const double *st = saved.stats + (long long)b * d.groups * 2;
     Channel k[N];
     float2 a[N];
@@ -687,12 +695,12 @@ __global__ __launch_bounds__(MAX_THREADS) void k_gn_grad_apply(const T *__restri
                 const float dz = grad_z((float)g[u].v[j], (float)w[u].v[j], k[j], st + c / d.gc * 2, saved.weight + c, ACT, e);
                 r.v[j] = (T)grad_x(dz, e, k[j], a[j]);
             }
-            store_word<T, WHOLE>(oq + u * step, r, d, v);
+            store_word<T, WHOLE, STREAM>(oq + u * step, r, d, v);
         });
         p += FL * d.rows;
         if (p < p1) {
-            load_batch<T, WHOLE>(w, xp, pixel_stride, p, p1, d, v);
-            load_batch<T, WHOLE>(g, dp, dy_pixel, p, p1, d, v);
+            load_batch<T, WHOLE, STREAM>(w, xp, pixel_stride, p, p1, d, v);
+            load_batch<T, WHOLE, STREAM>(g, dp, dy_pixel, p, p1, d, v);
         }
     }
 }
@@ -803,8 +811,10 @@ int vectors_of(int c, int dtype) { return ceil_div(c, vector_of(dtype)); }
 
 int threads_of(int cv) { return cv <= 256 ? 256 : MAX_THREADS; }
 
-// The two-pass form.  Workgroups of an image: about 2048 over the whole batch (eight a compute unit), each
-// with 8 pixels a thread at least, so that a workgroup's reduction is paid by enough reading.
+// The two-pass form.  A workgroup takes 16 pixels a thread, so that its reduction is paid by enough reading, where that
+// still gives every compute unit a workgroup, else 8 or 4; no more than 2048 workgroups (eight a compute unit).  us of
+// statistics and apply pass with 16 / 8 pixels: (1, 256, 200, 304) bf16 10.0 + 12.9 / 10.9 + 15.4; with 8 / 4:
+// (3, 96, 67, 101) fp16 6.6 + 6.9 / 5.7 + 5.0.
 GnDims dims_of(int b, int c, long long hw, int groups, int dtype)
 {
     GnDims d;
@@ -814,7 +824,11 @@ GnDims dims_of(int b, int c, long long hw, int groups, int dtype)
     d.rows = threads_of(d.cv) / d.cv;
     d.groups = groups;
     d.gc = c / groups;
-    const long long most = (hw + 8 * d.rows - 1) / (8 * d.rows);
+    int pixels = 16;
+    auto most_of = [&] { return (hw + (long long)pixels * d.rows - 1) / ((long long)pixels * d.rows); };
+    while (pixels > 4 && b * most_of() < 256)
+        pixels /= 2;
+    const long long most = most_of();
     long long nch = (2048 + b - 1) / b;
     nch = nch < 1 ? 1 : (nch > most ? most : nch);
     d.chunk = (hw + nch - 1) / nch;
@@ -865,6 +879,11 @@ template <typename F> int with_type(int dtype, bool whole, F &&f)
         return whole ? f((_Float16)0, std::true_type{}) : f((_Float16)0, std::false_type{});
     return whole ? f((__bf16)0.0f, std::true_type{}) : f((__bf16)0.0f, std::false_type{});
 }
+
+// Does a map (in- and output) go past the cache?
+bool streams(int b, int c, long long hw, int dtype) { return (double)b * c * hw * (dtype == DANCE_F32 ? 4 : 2) >= 64e6; }
+
+template <typename F> int with_flag(bool on, F &&f) { return on ? f(std::true_type{}) : f(std::false_type{}); }
 
 template <typename F> int with_act(int act, F &&f)
 {
@@ -960,9 +979,12 @@ extern "C" int dance_group_norm_act(const void *x, int64_t image_stride, int64_t
         if (int rc = launch_check(fn))
             return rc;
         return with_act(act, [&](auto a) {
-            hipLaunchKernelGGL((k_gn_apply<T, W, decltype(a)::value>), grid, dim3(threads), 0, st, (const T *)x,
-                               (long long)image_stride, (long long)pixel_stride, (const Channel *)out.channels, (T *)y, d);
-            return launch_check(fn);
+            return with_flag(W && streams(b, c, hw, dtype), [&](auto stream) {
+                hipLaunchKernelGGL((k_gn_apply<T, W, decltype(a)::value, W && decltype(stream)::value>), grid, dim3(threads), 0,
+                                   st, (const T *)x, (long long)image_stride, (long long)pixel_stride,
+                                   (const Channel *)out.channels, (T *)y, d);
+                return launch_check(fn);
+            });
         });
     });
 }
@@ -1031,14 +1053,17 @@ extern "C" int dance_group_norm_act_backward(const void *dy, int64_t dy_image_st
                                (long long)image_stride, (long long)pixel_stride, sv, partial, d);
             if (int rc = launch_check(fn))
                 return rc;
-            hipLaunchKernelGGL(k_gn_grad_finish, dim3(groups, b), dim3(256), 0, st, (const float *)partial, sv, sums, means, d);
+            hipLaunchKernelGGL(k_gn_grad_finish, dim3(groups, b), dim3(MAX_THREADS), 0, st, (const float *)partial, sv, sums, means, d);
             if (int rc = launch_check(fn))
                 return rc;
-            hipLaunchKernelGGL((k_gn_grad_apply<T, W, ACT>), dx ? grid : dim3(1), dim3(threads), 0, st, (const T *)dy,
-                               (long long)dy_image_stride, (long long)dy_pixel_stride, (const T *)x,
-                               (long long)image_stride, (long long)pixel_stride, sv, (const float2 *)means,
-                               (const double *)sums, (T *)dx, dweight, dbias, affine_dtype, b, d);
-            return launch_check(fn);
+            return with_flag(W && streams(b, c, hw, dtype), [&](auto stream) {
+                hipLaunchKernelGGL((k_gn_grad_apply<T, W, ACT, W && decltype(stream)::value>), dx ? grid : dim3(1),
+                                   dim3(threads), 0, st, (const T *)dy, (long long)dy_image_stride,
+                                   (long long)dy_pixel_stride, (const T *)x, (long long)image_stride,
+                                   (long long)pixel_stride, sv, (const float2 *)means, (const double *)sums, (T *)dx, dweight,
+                                   dbias, affine_dtype, b, d);
+                return launch_check(fn);
+            });
         });
     });
 }

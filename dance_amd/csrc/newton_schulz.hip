@@ -260,6 +260,12 @@ __device__ __forceinline__ unsigned split_word(float x)
     return __builtin_bit_cast(unsigned, p);
 }
 
+// c v + b A of an entry, A from its halves
+__device__ __forceinline__ float poly_of(float c, float v, float b, _Float16 hi, _Float16 lo)
+{
+    return fmaf((float)hi, b, fmaf((float)lo, b, c * v));
+}
+
 __device__ __forceinline__ unsigned hi_pair(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ __forceinline__ unsigned lo_pair(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
@@ -295,11 +301,12 @@ __device__ __forceinline__ void transpose4(unsigned (&x)[4])
 }
 
 // tile [I][J] of split words in LDS, row stride J + 1 (odd: conflict-free both ways) -> operand with rows i (from i0
-// of `rows`) and k along j (from j0).  T threads.
+// of `rows`) and k along j (from j0).  By T threads.
 template <int I, int J, int T>
-__device__ __forceinline__ void put_rows(_Float16 *out, size_t plane, int rows, int i0, int j0, const unsigned *tile)
+__device__ __forceinline__ void put_rows(_Float16 *out, size_t plane, int rows, int i0, int j0, const unsigned *tile,
+                                         int thread = threadIdx.x)
 {
-    const int i = threadIdx.x % I, jb0 = threadIdx.x / I;
+    const int i = thread % I, jb0 = thread / I;
     const unsigned *from = tile + i * (J + 1) + jb0 * 8;
     _Float16 *to = out + ((size_t)(j0 / 8 + jb0) * rows + i0 + i) * 8;
     const size_t step = (size_t)(T / I) * rows * 8;
@@ -316,9 +323,10 @@ __device__ __forceinline__ void put_rows(_Float16 *out, size_t plane, int rows, 
 
 // the same tile -> operand with rows j (from j0 of `rows`) and k along i (from i0)
 template <int I, int J, int T>
-__device__ __forceinline__ void put_cols(_Float16 *out, size_t plane, int rows, int i0, int j0, const unsigned *tile)
+__device__ __forceinline__ void put_cols(_Float16 *out, size_t plane, int rows, int i0, int j0, const unsigned *tile,
+                                         int thread = threadIdx.x)
 {
-    const int j = threadIdx.x % J, ib0 = threadIdx.x / J;
+    const int j = thread % J, ib0 = thread / J;
     const unsigned *from = tile + ib0 * 8 * (J + 1) + j;
     _Float16 *to = out + ((size_t)(i0 / 8 + ib0) * rows + j0 + j) * 8;
     const size_t step = (size_t)(T / J) * rows * 8;
@@ -390,9 +398,9 @@ template <typename T, bool DENSE> __global__ __launch_bounds__(256) void k_ns_pa
                 tile[(rr + w * (256 / (PACK / N))) * step_i + (cc + q) * step_j] = split_word(scaled(x[q]));
         }
     } else {
-#pragma unroll 8
-        for (int w = threadIdx.x; w < PACK * PACK; w += 256) {
-            const int rr = w / PACK, cc = w % PACK, row = row0 + rr, col = col0 + cc;
+#pragma unroll 4
+        for (int n = 0; n < PACK * PACK / 256; ++n) {
+            const int rr = threadIdx.x / PACK + n * (256 / PACK), cc = threadIdx.x % PACK, row = row0 + rr, col = col0 + cc;
             float x = 0.0f;
             if (row < it.m && col < it.n) {
                 float mom;
@@ -412,17 +420,19 @@ template <typename T, bool DENSE> __global__ __launch_bounds__(256) void k_ns_pa
 // ------------------------------------------------------------------------------------------- GEMM
 // A square tile of side S = 32 F by 4 waves of F x F fragments of 16 x 16, three products each, k in steps of 32.  A
 // step's operands, S rows of each side, are copied from L2 to LDS without passing registers (global_load_lds_dwordx4),
-// the next step's while this one's are multiplied.
+// DEPTH - 1 steps ahead.
 //   F = 4 (128): per step and wave 48 MFMAs (768 clocks) stand against 16 KB read from LDS (512 clocks for all four
-//     waves); two workgroups share a compute unit, one multiplies while the other waits: 820 clocks a step.
-//   F = 2 (64): 192 against 256 clocks, so less of the chip's rate, but four times the workgroups: where 128-tiles do
-//     not give every compute unit one, a step of theirs lasts 1550 clocks, four of these 600 each.
+//     waves); two buffers, so that two workgroups share a compute unit and one multiplies while the other waits: 820
+//     clocks a step.
+//   F = 2 (64): 192 against 256 clocks, so less of the chip's rate, but four times the workgroups: for launches whose
+//     128-tiles would not give every compute unit one, where a step of those lasts 1550 clocks.  Four buffers: alone on
+//     its compute unit a workgroup has to cover the copies' latency itself.
 constexpr int STEP = 32;
 template <int F> struct Tile {
-    static constexpr int SIDE = 32 * F, LD = SIDE + 1;
+    static constexpr int SIDE = 32 * F, LD = SIDE + 1, DEPTH = F == 2 ? 4 : 2;
     static constexpr int SIDE_BYTES = 2 * (STEP / 8) * SIDE * 16;        // [plane][k block][row] words of 16 bytes
-    static constexpr int BUFFER = 2 * SIDE_BYTES;
-    static constexpr int LDS = 2 * BUFFER > SIDE * LD * 4 ? 2 * BUFFER : SIDE * LD * 4;      // two buffers, then the tile in 32 bits
+    static constexpr int BUFFER = 2 * SIDE_BYTES, COPIES = STEP / 8 * F / 2;      // COPIES: of a wave and step
+    static constexpr int LDS = DEPTH * BUFFER > SIDE * LD * 4 ? DEPTH * BUFFER : SIDE * LD * 4;       // then the tile in 32 bits
 };
 constexpr int GEMM_THREADS = 256;
 
@@ -461,9 +471,14 @@ template <int F> __device__ __forceinline__ void stage_plane(const Side &s, int 
             copy_words(src + ((size_t)kb * s.rows + part * 64) * 8, lds + (kb * Tile<F>::SIDE + part * 64) * 16);
 }
 
-__device__ __forceinline__ void gemm_wait()
+// until at most LEFT of this wave's copies are under way (they end in order); in all waves
+template <int LEFT = 0> __device__ __forceinline__ void gemm_wait()
 {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    static_assert(LEFT == 0 || LEFT == 8, "the waits that occur");
+    if (LEFT == 8)
+        asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    else
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
 }
 
@@ -496,12 +511,20 @@ __device__ __forceinline__ void tile_gemm(f32x4 (&acc)[F][F], char *lds, const S
     const int word = (lane >> 4) * SIDE + (lane & 15);
     const char *us = lds + ((wave >> 1) * 16 * F + word) * 16;
     const char *vs = lds + (same ? 0 : SIDE_BYTES) + ((wave & 1) * 16 * F + word) * 16;
-    stage(0, 0);
-    gemm_wait();
+    constexpr int DEPTH = Tile<F>::DEPTH, AHEAD = DEPTH - 1;
+#pragma unroll
+    for (int b = 0; b < AHEAD; ++b)
+        if (b < steps)
+            stage(b, b);
     for (int s = 0; s < steps; ++s) {
-        const int now = (s & 1) * Tile<F>::BUFFER;
-        if (s + 1 < steps)
-            stage(s + 1, (s + 1) & 1);
+        // step s has arrived; and what step s - 1 was read from is free, after the barrier, for step s + AHEAD
+        if (s + AHEAD <= steps)
+            gemm_wait<(AHEAD - 1) * Tile<F>::COPIES>();
+        else
+            gemm_wait();
+        const int now = s % DEPTH * Tile<F>::BUFFER;
+        if (s + AHEAD < steps)
+            stage(s + AHEAD, (s + AHEAD) % DEPTH);
         h8 uh[F], ul[F], vh[F], vl[F];
         auto load_u = [&](int i) {
             uh[i] = *reinterpret_cast<const h8 *>(us + now + i * 256);
@@ -524,8 +547,8 @@ __device__ __forceinline__ void tile_gemm(f32x4 (&acc)[F][F], char *lds, const S
                 acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[i], vl[j], acc[i][j], 0, 0, 0);
                 acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[i], vh[j], acc[i][j], 0, 0, 0);
             }
-        gemm_wait();
     }
+    __syncthreads();
 }
 
 // this lane's first value of the tile: acc[i][j][q] lies 16 i + q rows and 16 j columns from it
@@ -582,8 +605,10 @@ template <int F> __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_gram(co
             out[(i * F + j) * 64] = acc[i][j];
 }
 
-// the shares added in order, split, mirrored: 64 x 64 of A a workgroup, a quarter of a tile of 128 or a tile of 64
-__global__ __launch_bounds__(256) void k_ns_sum(const NsTable *__restrict__ tp)
+// the shares added in order, split, mirrored: 64 x 64 of A a workgroup, a quarter of a tile of 128 or a tile of 64.
+// 16 bytes of a share a thread, eight shares at once: one or two trips to memory.
+constexpr int SUM_THREADS = 1024;
+__global__ __launch_bounds__(SUM_THREADS) void k_ns_sum(const NsTable *__restrict__ tp)
 {
     const NsTable &t = *tp;
     constexpr int UNIT = 64, LD = UNIT + 1;
@@ -598,30 +623,30 @@ __global__ __launch_bounds__(256) void k_ns_sum(const NsTable *__restrict__ tp)
     lower_tile(local / parts, ti, tj);
     const size_t share = (size_t)lower_tiles(d, side) * side * side / 4;
     const f32x4 *in = reinterpret_cast<const f32x4 *>(s.part + (size_t)(local / parts) * side * side) + part * 16 * 64 + threadIdx.x;
-    f32x4 v[4];
+    f32x4 v = in[0];
+    for (int k = 1; k < it.split; k += 8) {
+        f32x4 w[8];
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
-        v[w] = in[256 * w];
-#pragma unroll 2
-    for (int k = 1; k < it.split; ++k)
+        for (int u = 0; u < 8; ++u)
+            w[u] = in[min(k + u, it.split - 1) * share];
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
-            v[w] += in[k * share + 256 * w];
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        // fragment f of the unit: 4 x 4 of a wave, or 2 x 2 of each of 4 waves
-        const int f = 4 * w + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-        const int i = parts == 4 ? f >> 2 : (f >> 3) * 2 + (f >> 1 & 1), j = parts == 4 ? f & 3 : (f >> 2 & 1) * 2 + (f & 1);
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            tile[(16 * i + 4 * (lane >> 4) + q) * LD + 16 * j + (lane & 15)] = split_word(v[w][q] * dance::pow2f(-X_EXP));
+        for (int u = 0; u < 8; ++u)
+            if (k + u < it.split)
+                v += w[u];
     }
+    // fragment f of the unit: 4 x 4 of a wave, or 2 x 2 of each of 4 waves
+    const int f = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int i = parts == 4 ? f >> 2 : (f >> 3) * 2 + (f >> 1 & 1), j = parts == 4 ? f & 3 : (f >> 2 & 1) * 2 + (f & 1);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        tile[(16 * i + 4 * (lane >> 4) + q) * LD + 16 * j + (lane & 15)] = split_word(v[q] * dance::pow2f(-X_EXP));
     __syncthreads();
     const size_t plane = (size_t)d.rp * d.rp;
     const int i0 = ti * side + (part >> 1) * UNIT, j0 = tj * side + (part & 1) * UNIT;
-    put_rows<UNIT, UNIT, 256>(s.a, plane, d.rp, i0, j0, tile);
-    if (ti != tj)
-        put_cols<UNIT, UNIT, 256>(s.a, plane, d.rp, i0, j0, tile);
+    if (threadIdx.x < SUM_THREADS / 2)
+        put_rows<UNIT, UNIT, SUM_THREADS / 2>(s.a, plane, d.rp, i0, j0, tile);
+    else if (ti != tj)
+        put_cols<UNIT, UNIT, SUM_THREADS / 2>(s.a, plane, d.rp, i0, j0, tile, threadIdx.x - SUM_THREADS / 2);
 }
 
 // Q = a I + b A + c A A, lower tiles and their mirror images
@@ -654,10 +679,14 @@ template <int F> __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_poly(co
     tile_gemm<F>(acc, lds, side_of(s.a, plane, d.rp, i0, 0), side_of(s.a, plane, d.rp, j0, 0), ti == tj, d.rp / STEP);
     const float ca = t.c * dance::pow2f(-2 * X_EXP) * t.q_mul, ba = t.b * dance::pow2f(-X_EXP) * t.q_mul, a = t.a * t.q_mul;
     const unsigned *tile = tile_to_lds<unsigned>(acc, lds, [&](int i, int j, f32x4 v) {
-        const int diagonal = col + 16 * j < d.r ? col + 16 * j - row - 16 * i : -1;
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            v[q] = fmaf(ca, v[q], ba * ((float)hi[i][j][q] + (float)lo[i][j][q])) + (q == diagonal ? a : 0.0f);
+            v[q] = poly_of(ca, v[q], ba, hi[i][j][q], lo[i][j][q]);
+        if (ti == tj && i == j) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                v[q] += row + 16 * i + q == col + 16 * j && col + 16 * j < d.r ? a : 0.0f;
+        }
         return v;
     });
     put_rows<SIDE, SIDE, GEMM_THREADS>(s.q, plane, d.rp, i0, j0, tile);
@@ -666,7 +695,7 @@ template <int F> __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_poly(co
 }
 
 // a tile of the result, rows i and columns j of X from (i0, j0) on; Muon: the parameter's update
-template <typename T, int SIDE>
+template <typename T, int SIDE, int THREADS>
 __device__ __forceinline__ void put_result(const NsTable &t, const NsItem &it, const NsDims &d, int i0, int j0, const float *tile)
 {
     const int row0 = d.tall ? j0 : i0, col = (d.tall ? i0 : j0) + (int)threadIdx.x % SIDE;
@@ -675,21 +704,21 @@ __device__ __forceinline__ void put_result(const NsTable &t, const NsItem &it, c
     if (col >= it.n)
         return;
 #pragma unroll 1
-    for (int r = threadIdx.x / SIDE; r < SIDE && row0 + r < it.m; r += 8 * (GEMM_THREADS / SIDE)) {
+    for (int r = threadIdx.x / SIDE; r < SIDE && row0 + r < it.m; r += 8 * (THREADS / SIDE)) {
         T *to = (T *)it.dst + (long long)(row0 + r) * it.n + col;
         T old[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            const int rr = r + u * (GEMM_THREADS / SIDE);
+            const int rr = r + u * (THREADS / SIDE);
             if (t.muon && row0 + rr < it.m)
-                old[u] = to[(long long)u * (GEMM_THREADS / SIDE) * it.n];
+                old[u] = to[(long long)u * (THREADS / SIDE) * it.n];
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            const int rr = r + u * (GEMM_THREADS / SIDE);
+            const int rr = r + u * (THREADS / SIDE);
             const float v = from[rr * step_row];
             if (row0 + rr < it.m)
-                to[(long long)u * (GEMM_THREADS / SIDE) * it.n] = (T)(t.muon ? fmaf(-it.scale, v, (float)old[u] * t.keep) : v);
+                to[(long long)u * (THREADS / SIDE) * it.n] = (T)(t.muon ? fmaf(-it.scale, v, (float)old[u] * t.keep) : v);
         }
     }
 }
@@ -721,11 +750,11 @@ template <int F> __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_apply(c
     const float *tile = tile_to_lds<float>(acc, lds, [&](int, int, f32x4 v) { return v * out; });
     // neighbouring threads write neighbours of a row of M
     if (t.dtype == DANCE_F32)
-        put_result<float, SIDE>(t, it, d, i0, j0, tile);
+        put_result<float, SIDE, GEMM_THREADS>(t, it, d, i0, j0, tile);
     else if (t.dtype == DANCE_F16)
-        put_result<_Float16, SIDE>(t, it, d, i0, j0, tile);
+        put_result<_Float16, SIDE, GEMM_THREADS>(t, it, d, i0, j0, tile);
     else
-        put_result<__bf16, SIDE>(t, it, d, i0, j0, tile);
+        put_result<__bf16, SIDE, GEMM_THREADS>(t, it, d, i0, j0, tile);
 }
 
 // ------------------------------------------------------------------------------ narrow matrices
@@ -824,6 +853,7 @@ template <typename T> __global__ __launch_bounds__(NARROW_THREADS) void k_ns_nar
     ns_space(it.ws, d, it.split, s);
     const size_t rect = (size_t)PAD * d.kp, share = PAD * PAD;
     const int tiles = d.kp / PAD, last = step + 1 == t.steps;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     f32x4 next[4][2];
     zero(next);
     if (step < 0) {
@@ -845,17 +875,24 @@ template <typename T> __global__ __launch_bounds__(NARROW_THREADS) void k_ns_nar
             // A is symmetric: 4 rows of a column are 4 neighbours of that column's row
             const _Float16 *p = (const _Float16 *)square + ((row >> 3) * PAD + col) * 8 + (row & 7);
             const h4 hi = *reinterpret_cast<const h4 *>(p), lo = *reinterpret_cast<const h4 *>(p + REGION / 4);
-            const int diagonal = col < d.r ? col - row : -1;
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                v[i][j][q] = fmaf(ca, v[i][j][q], ba * ((float)hi[q] + (float)lo[q])) + (q == diagonal ? one : 0.0f);
+                v[i][j][q] = poly_of(ca, v[i][j][q], ba, hi[q], lo[q]);
+            if (wave / 4 * 4 + i == (wave & 3) * 2 + j) {         // (a fragment of the diagonal, in every lane)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    v[i][j][q] += row + q == col && col < d.r ? one : 0.0f;
+            }
         });
-        __syncthreads();
-        narrow_put_square(square, v);
+        f32x4 q[4][2];
+        narrow_each([&](int i, int j, int, int) { q[i][j] = v[i][j]; });
         const float mul = 1.0f / t.q_mul;
 #pragma unroll 1
         for (int c = local; c < tiles; c += it.split) {
-            __syncthreads();                                  // Q is there, and the columns before have been read
+            __syncthreads();                                  // A, and the columns before, have been read
+            if (c == local || last)
+                narrow_put_square(square, q);
+            __syncthreads();
             if (c != local) {
                 narrow_stage(s.xr[0] + (size_t)c * PAD * 8, rect, d.kp, columns);
                 gemm_wait();
@@ -879,33 +916,22 @@ template <typename T> __global__ __launch_bounds__(NARROW_THREADS) void k_ns_nar
                 __syncthreads();
                 narrow_gemm(next, columns, columns);
             } else {
-                const float out = mul * dance::pow2f(-X_EXP);
-                const int step_row = d.tall ? 1 : it.n, step_col = d.tall ? it.n : 1;
-                T *to = (T *)it.dst + (long long)c * PAD * step_col;
-                f32x4 old[4][2];
-                if (t.muon)
-                    narrow_each([&](int i, int j, int row, int col) {
-#pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            if (row + q < d.r && c * PAD + col < d.k)
-                                old[i][j][q] = (float)to[(long long)(row + q) * step_row + (long long)col * step_col];
-                    });
+                // the tile in fp32 over both regions; Q is needed again if there are more columns
+                float *tile = reinterpret_cast<float *>(lds);
                 narrow_each([&](int i, int j, int row, int col) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
-                        if (row + q < d.r && c * PAD + col < d.k) {
-                            const float x = v[i][j][q] * out;
-                            to[(long long)(row + q) * step_row + (long long)col * step_col] =
-                                (T)(t.muon ? fmaf(-it.scale, x, old[i][j][q] * t.keep) : x);
-                        }
+                        tile[(row + q) * (PAD + 1) + col] = v[i][j][q] * (mul * dance::pow2f(-X_EXP));
                 });
+                __syncthreads();
+                put_result<T, PAD, NARROW_THREADS>(t, it, d, 0, c * PAD, tile);
             }
         }
     }
     if (last)
         return;
     // where k_ns_sum looks for them: quarter by quarter of the tile, 4 x 4 fragments each
-    const int wave = threadIdx.x >> 6, quarter = (wave >> 2) * 2 + (wave >> 1 & 1);
+    const int quarter = (wave >> 2) * 2 + (wave >> 1 & 1);
     f32x4 *out = reinterpret_cast<f32x4 *>(s.part + local * share) + (quarter * 16 + (wave & 1) * 2) * 64 + (threadIdx.x & 63);
     narrow_each([&](int i, int j, int, int) { out[(i * 4 + j) * 64] = next[i][j]; });
 }
@@ -1055,7 +1081,8 @@ template <typename T, bool DENSE> __global__ __launch_bounds__(SMALL_THREADS) vo
 
     const int fr = d.rp / 16, fk = d.kp / 16;
     const int i4 = 4 * (lane >> 4), j1 = lane & 15;               // a lane's rows and column in a fragment
-    const float ca = t.c * dance::pow2f(-2 * X_EXP), ba = t.b * dance::pow2f(-X_EXP), mul = 1.0f / t.q_mul;
+    const float ca = t.c * dance::pow2f(-2 * X_EXP) * t.q_mul, ba = t.b * dance::pow2f(-X_EXP) * t.q_mul, one = t.a * t.q_mul;
+    const float mul = 1.0f / t.q_mul;
     // a fragment of a symmetric matrix at (i0, j0): entered at its mirror image, where a lane's 4 values are neighbours
     auto put_square = [&](const f32x4 &v, int i0, int j0) {
         put4(a + (((i0 + i4) >> 3) * d.rp + j0 + j1) * 8 + (i4 & 7), square, split_word(v[0]), split_word(v[1]), split_word(v[2]),
@@ -1078,10 +1105,14 @@ template <typename T, bool DENSE> __global__ __launch_bounds__(SMALL_THREADS) vo
             q[n] = small_gemm(a, d.rp, square, i0, a, d.rp, square, j0, d.rp);
             const _Float16 *p = a + (((i0 + i4) >> 3) * d.rp + j0 + j1) * 8 + (i4 & 7);
             const h4 ah = *reinterpret_cast<const h4 *>(p), al = *reinterpret_cast<const h4 *>(p + square);
-            const int diagonal = j0 + j1 < d.r ? j0 + j1 - i0 - i4 : -1;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                q[n][e] = (fmaf(ca, q[n][e], ba * ((float)ah[e] + (float)al[e])) + (e == diagonal ? t.a : 0.0f)) * t.q_mul;
+                q[n][e] = poly_of(ca, q[n][e], ba, ah[e], al[e]);
+            if (i0 == j0) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    q[n][e] += i4 + e == j1 && j0 + j1 < d.r ? one : 0.0f;
+            }
         }
         __syncthreads();                                          // every wave has read A: Q takes its place
 #pragma unroll
@@ -1192,135 +1223,151 @@ float q_scale(float a, float b, float c)
     return most > 0.0 ? (float)exp2(fmin(14.0, floor(log2(60000.0 / most)))) : 1.0f;
 }
 
-template <typename F> int with_type(int dtype, bool dense, F &&f)
-{
-    if (dtype == DANCE_F32)
-        return dense ? f((float)0, std::true_type{}) : f((float)0, std::false_type{});
-    if (dtype == DANCE_F16)
-        return dense ? f((_Float16)0, std::true_type{}) : f((_Float16)0, std::false_type{});
-    return dense ? f((__bf16)0.0f, std::true_type{}) : f((__bf16)0.0f, std::false_type{});
-}
+// A chain over the items of a table whose sizes, pointers and settings are set, in pieces: prepare, then step(-1),
+// step(0), ... step(t.steps - 1).  Matrices that all fit a compute unit's LDS are done in one launch, a workgroup each,
+// by prepare.
+struct Chain {
+    NsTable t;
+    NsTable *kept;
+    hipStream_t st;
+    const char *fn;
+    bool dense, done;
+    long long narrows, gram, sum, poly, rect;
+    int poly_side, rect_side;
 
-// The chain over the items of a table whose sizes, pointers and settings are set.  Matrices that all fit a compute
-// unit's LDS are done in one launch, a workgroup each.
-int run_chain(NsTable &t, char *ws, hipStream_t st, const char *fn)
-{
-    bool dense = true;
-    for (int i = 0; i < t.count; ++i)
-        dense = dense && (t.muon || (t.col_stride == 1 && (t.row_stride == t.it[i].n || t.it[i].m == 1)));
-    if (lay_out(t, ws) == 0) {
+    template <typename F> int with_type(F &&f) const
+    {
+        if (t.dtype == DANCE_F32)
+            return dense ? f((float)0, std::true_type{}) : f((float)0, std::false_type{});
+        if (t.dtype == DANCE_F16)
+            return dense ? f((_Float16)0, std::true_type{}) : f((_Float16)0, std::false_type{});
+        return dense ? f((__bf16)0.0f, std::true_type{}) : f((__bf16)0.0f, std::false_type{});
+    }
+
+    int launched() const { return launch_check(fn); }
+
+    int small() const
+    {
         size_t lds = 0;
         for (int i = 0; i < t.count; ++i) {
             const size_t bytes = small_dims(t.it[i].m, t.it[i].n).bytes;
             lds = bytes > lds ? bytes : lds;
         }
-        return with_type(t.dtype, dense, [&](auto type, auto is_dense) {
+        return with_type([&](auto type, auto is_dense) {
             using T = decltype(type);
             constexpr bool D = decltype(is_dense)::value;
             if (int rc = dance::allow_lds((const void *)k_ns_small<T, D>, lds, fn))
                 return rc;
             hipLaunchKernelGGL((k_ns_small<T, D>), dim3(t.count), dim3(SMALL_THREADS), lds, st, t);
-            return launch_check(fn);
+            return launched();
         });
     }
-    long long slices = 0, pack = 0, narrows = 0, gram = 0, sum = 0, poly = 0, rect = 0;
-    for (int i = 0; i < t.count; ++i) {
-        const NsDims d = ns_dims(t.it[i].m, t.it[i].n);
-        if (!narrow(d)) {
-            gram += (long long)lower_tiles(d, PAD) * t.it[i].split;
-            poly += lower_tiles(d, PAD);
-            rect += (long long)(d.rp / PAD) * (d.kp / PAD);
-        }
-    }
-    const int gram_side = t.gram_side = side_for(gram), poly_side = side_for(poly), rect_side = side_for(rect);
-    gram = poly = rect = 0;
-    for (int i = t.count; i < NS_ITEMS; ++i)
-        t.slices[i] = t.pack[i] = t.narrow[i] = t.gram[i] = t.sum[i] = t.poly[i] = t.rect[i] = INT_MAX;
-    for (int i = 0; i < t.count; ++i) {
-        const NsDims d = ns_dims(t.it[i].m, t.it[i].n);
-        const long long want = ((long long)t.it[i].m * t.it[i].n + 8191) / 8192;
-        slices += want < NS_SLICES ? want : NS_SLICES;
-        pack += (long long)(d.rp / PACK) * (d.kp / PACK);
-        if (narrow(d)) {
-            narrows += t.it[i].split;
-            sum += 4;
-        } else {
-            gram += (long long)lower_tiles(d, gram_side) * t.it[i].split;
-            sum += (long long)lower_tiles(d, gram_side) * (gram_side == PAD ? 4 : 1);
-            poly += lower_tiles(d, poly_side);
-            rect += (long long)(d.rp / rect_side) * (d.kp / rect_side);
-        }
-        if (pack >= (1ll << 31) || gram >= (1ll << 31) || sum >= (1ll << 31) || rect >= (1ll << 31) || narrows >= (1ll << 31))
-            return dance::fail((int)hipErrorInvalidValue, fn, "too many tiles");
-        t.slices[i] = (int)slices;
-        t.pack[i] = (int)pack;
-        t.narrow[i] = (int)narrows;
-        t.gram[i] = (int)gram;
-        t.sum[i] = (int)sum;
-        t.poly[i] = (int)poly;
-        t.rect[i] = (int)rect;
-    }
-    NsTable *kept = (NsTable *)ws;
-    auto with_side = [&](int side, auto &&f) {
-        return side == 128 ? f(std::integral_constant<int, 4>{}) : f(std::integral_constant<int, 2>{});
-    };
-    return with_type(t.dtype, dense, [&](auto type, auto is_dense) {
-        using T = decltype(type);
-        constexpr bool D = decltype(is_dense)::value;
-        hipLaunchKernelGGL((k_ns_norm<T, D>), dim3((unsigned)slices), dim3(256), 0, st, t, kept);
-        if (int e = launch_check(fn))
-            return e;
-        hipLaunchKernelGGL((k_ns_pack<T, D>), dim3((unsigned)pack), dim3(256), 0, st, (const NsTable *)kept);
-        if (int e = launch_check(fn))
-            return e;
-        if (int e = dance::allow_lds((const void *)k_ns_narrow<T>, NARROW_LDS, fn))
-            return e;
-        // step s of the X of all matrices, and the A of the next step; X itself is the -1st
-        for (int s = -1; s < t.steps; ++s) {
-            const int last = s + 1 == t.steps;
-            int e = 0;
-            if (narrows > 0) {
-                hipLaunchKernelGGL(k_ns_narrow<T>, dim3((unsigned)narrows), dim3(NARROW_THREADS), NARROW_LDS, st,
-                                   (const NsTable *)kept, s);
-                e = launch_check(fn);
+
+    int prepare(char *ws, hipStream_t stream, const char *name)
+    {
+        st = stream;
+        fn = name;
+        kept = (NsTable *)ws;
+        dense = true;
+        for (int i = 0; i < t.count; ++i)
+            dense = dense && (t.muon || (t.col_stride == 1 && (t.row_stride == t.it[i].n || t.it[i].m == 1)));
+        done = lay_out(t, ws) == 0;
+        if (done)
+            return t.count > 0 ? small() : 0;
+        gram = poly = rect = 0;
+        for (int i = 0; i < t.count; ++i) {
+            const NsDims d = ns_dims(t.it[i].m, t.it[i].n);
+            if (!narrow(d)) {
+                gram += (long long)lower_tiles(d, PAD) * t.it[i].split;
+                poly += lower_tiles(d, PAD);
+                rect += (long long)(d.rp / PAD) * (d.kp / PAD);
             }
-            if (e == 0 && rect > 0 && s >= 0)
-                e = with_side(poly_side, [&](auto f) {
-                    constexpr int F = decltype(f)::value;
-                    if (int r = dance::allow_lds((const void *)k_ns_poly<F>, Tile<F>::LDS, fn))
-                        return r;
-                    hipLaunchKernelGGL(k_ns_poly<F>, dim3((unsigned)poly), dim3(GEMM_THREADS), Tile<F>::LDS, st,
-                                       (const NsTable *)kept);
-                    return launch_check(fn);
-                });
-            if (e == 0 && rect > 0 && s >= 0)
-                e = with_side(rect_side, [&](auto f) {
-                    constexpr int F = decltype(f)::value;
-                    if (int r = dance::allow_lds((const void *)k_ns_apply<F>, Tile<F>::LDS, fn))
-                        return r;
-                    hipLaunchKernelGGL(k_ns_apply<F>, dim3((unsigned)rect), dim3(GEMM_THREADS), Tile<F>::LDS, st,
-                                       (const NsTable *)kept, s, last);
-                    return launch_check(fn);
-                });
-            if (e == 0 && rect > 0 && !last)
-                e = with_side(gram_side, [&](auto f) {
-                    constexpr int F = decltype(f)::value;
-                    if (int r = dance::allow_lds((const void *)k_ns_gram<F>, Tile<F>::LDS, fn))
-                        return r;
-                    hipLaunchKernelGGL(k_ns_gram<F>, dim3((unsigned)gram), dim3(GEMM_THREADS), Tile<F>::LDS, st,
-                                       (const NsTable *)kept, s + 1);
-                    return launch_check(fn);
-                });
-            if (e == 0 && !last) {
-                hipLaunchKernelGGL(k_ns_sum, dim3((unsigned)sum), dim3(256), 0, st, (const NsTable *)kept);
-                e = launch_check(fn);
+        }
+        t.gram_side = side_for(gram);
+        poly_side = side_for(poly);
+        rect_side = side_for(rect);
+        long long slices = 0, pack = 0;
+        narrows = gram = sum = poly = rect = 0;
+        for (int i = t.count; i < NS_ITEMS; ++i)
+            t.slices[i] = t.pack[i] = t.narrow[i] = t.gram[i] = t.sum[i] = t.poly[i] = t.rect[i] = INT_MAX;
+        for (int i = 0; i < t.count; ++i) {
+            const NsDims d = ns_dims(t.it[i].m, t.it[i].n);
+            const long long want = ((long long)t.it[i].m * t.it[i].n + 8191) / 8192;
+            slices += want < NS_SLICES ? want : NS_SLICES;
+            pack += (long long)(d.rp / PACK) * (d.kp / PACK);
+            if (narrow(d)) {
+                narrows += t.it[i].split;
+                sum += 4;
+            } else {
+                gram += (long long)lower_tiles(d, t.gram_side) * t.it[i].split;
+                sum += (long long)lower_tiles(d, t.gram_side) * (t.gram_side == PAD ? 4 : 1);
+                poly += lower_tiles(d, poly_side);
+                rect += (long long)(d.rp / rect_side) * (d.kp / rect_side);
             }
-            if (e)
+            if (pack >= (1ll << 31) || gram >= (1ll << 31) || sum >= (1ll << 31) || rect >= (1ll << 31) || narrows >= (1ll << 31))
+                return dance::fail((int)hipErrorInvalidValue, fn, "too many tiles");
+            t.slices[i] = (int)slices;
+            t.pack[i] = (int)pack;
+            t.narrow[i] = (int)narrows;
+            t.gram[i] = (int)gram;
+            t.sum[i] = (int)sum;
+            t.poly[i] = (int)poly;
+            t.rect[i] = (int)rect;
+        }
+        return with_type([&](auto type, auto is_dense) {
+            using T = decltype(type);
+            constexpr bool D = decltype(is_dense)::value;
+            if (int e = dance::allow_lds((const void *)k_ns_narrow<T>, NARROW_LDS, fn))
                 return e;
+            hipLaunchKernelGGL((k_ns_norm<T, D>), dim3((unsigned)slices), dim3(256), 0, st, t, kept);
+            if (int e = launched())
+                return e;
+            hipLaunchKernelGGL((k_ns_pack<T, D>), dim3((unsigned)pack), dim3(256), 0, st, (const NsTable *)kept);
+            return launched();
+        });
+    }
+
+    // kernel<F> on `tiles` tiles of side `side`, F = side / 32
+    template <typename K, typename... Args> int tiled(int side, long long tiles, K &&kernel, Args... args) const
+    {
+        auto go = [&](auto f) {
+            constexpr int F = decltype(f)::value;
+            auto k = kernel(f);
+            if (int r = dance::allow_lds((const void *)k, Tile<F>::LDS, fn))
+                return r;
+            hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(GEMM_THREADS), Tile<F>::LDS, st, (const NsTable *)kept, args...);
+            return launched();
+        };
+        return side == 128 ? go(std::integral_constant<int, 4>{}) : go(std::integral_constant<int, 2>{});
+    }
+
+    // step s of the X of all matrices, and the A of the next step; X itself is the -1st
+    int step(int s) const
+    {
+        const int last = s + 1 == t.steps;
+        int e = 0;
+        if (done)
+            return 0;
+        if (narrows > 0) {
+            e = with_type([&](auto type, auto) {
+                hipLaunchKernelGGL(k_ns_narrow<decltype(type)>, dim3((unsigned)narrows), dim3(NARROW_THREADS), NARROW_LDS, st,
+                                   (const NsTable *)kept, s);
+                return launched();
+            });
         }
-        return 0;
-    });
-}
+        if (e == 0 && rect > 0 && s >= 0)
+            e = tiled(poly_side, poly, [](auto f) { return k_ns_poly<decltype(f)::value>; });
+        if (e == 0 && rect > 0 && s >= 0)
+            e = tiled(rect_side, rect, [](auto f) { return k_ns_apply<decltype(f)::value>; }, s, last);
+        if (e == 0 && rect > 0 && !last)
+            e = tiled(t.gram_side, gram, [](auto f) { return k_ns_gram<decltype(f)::value>; }, s + 1);
+        if (e == 0 && !last) {
+            hipLaunchKernelGGL(k_ns_sum, dim3((unsigned)sum), dim3(SUM_THREADS), 0, st, (const NsTable *)kept);
+            e = launched();
+        }
+        return e;
+    }
+};
 
 bool usable(double a, double b, double c) { return isfinite(a) && isfinite(b) && isfinite(c); }
 
@@ -1353,7 +1400,8 @@ extern "C" int dance_orthogonalize(const void *x, int64_t batch_stride, int64_t 
     DANCE_REQUIRE(ws_bytes >= need && (ws || need == 0));
     const int64_t size = dtype == DANCE_F32 ? 4 : 2;
     for (int b0 = 0; b0 < batch; b0 += NS_ITEMS) {
-        NsTable t;
+        Chain chain;
+        NsTable &t = chain.t;
         memset(&t, 0, sizeof t);
         t.count = batch - b0 < NS_ITEMS ? batch - b0 : NS_ITEMS;
         t.dtype = dtype;
@@ -1369,36 +1417,58 @@ extern "C" int dance_orthogonalize(const void *x, int64_t batch_stride, int64_t 
             t.it[i].m = m;
             t.it[i].n = n;
         }
-        if (int rc = run_chain(t, (char *)ws, (hipStream_t)stream, __func__))
+        if (int rc = chain.prepare((char *)ws, (hipStream_t)stream, __func__))
             return rc;
+        for (int s = -1; s < steps; ++s)
+            if (int rc = chain.step(s))
+                return rc;
     }
     return 0;
 }
+
+namespace {
+// the next matrices of a kind, narrow or not, from items[at] on into a table -> where to go on
+int take(const dance_muon_item *items, int count, bool wide, int at, NsTable &t)
+{
+    t.count = 0;
+    for (; at < count && t.count < NS_ITEMS; ++at) {
+        const dance_muon_item &h = items[at];
+        if (narrow(ns_dims(h.rows, h.cols)) == wide)
+            continue;
+        NsItem &it = t.it[t.count++];
+        it.src = h.grad;
+        it.momentum = h.momentum;
+        it.dst = h.param;
+        it.m = h.rows;
+        it.n = h.cols;
+    }
+    return at;
+}
+}  // namespace
 
 extern "C" int64_t dance_muon_workspace_bytes(const dance_muon_item *items_host, int count)
 {
     if (count <= 0 || !items_host)
         return 0;
+    for (int i = 0; i < count; ++i)
+        if (items_host[i].rows <= 0 || items_host[i].cols <= 0 || (long long)items_host[i].rows * items_host[i].cols >= (1ll << 31))
+            return 0;
     int64_t most = 0;
-    for (int b0 = 0; b0 < count; b0 += NS_ITEMS) {
-        NsTable t;
-        t.count = count - b0 < NS_ITEMS ? count - b0 : NS_ITEMS;
-        for (int i = 0; i < t.count; ++i) {
-            const int m = items_host[b0 + i].rows, n = items_host[b0 + i].cols;
-            if (m <= 0 || n <= 0 || (long long)m * n >= (1ll << 31))
-                return 0;
-            t.it[i].m = m;
-            t.it[i].n = n;
+    for (int at[2] = {0, 0}; at[0] < count || at[1] < count;) {
+        int64_t sum = 0;
+        for (int wide = 0; wide < 2; ++wide) {
+            NsTable t;
+            at[wide] = take(items_host, count, wide, at[wide], t);
+            sum += lay_out(t, nullptr);
         }
-        const int64_t bytes = lay_out(t, nullptr);
-        most = bytes > most ? bytes : most;
+        most = sum > most ? sum : most;
     }
     return most;
 }
 
 extern "C" int dance_muon_step(const dance_muon_item *items_host, int count, int dtype, double lr, double momentum,
                                int nesterov, double weight_decay, int steps, float a, float b, float c, float eps, void *ws,
-                               int64_t ws_bytes, void *stream)
+                               int64_t ws_bytes, void *stream, void *side_stream)
 {
     DANCE_REQUIRE(count >= 0 && known_dtype(dtype) && steps >= 1 && steps <= 100 && usable(a, b, c) && eps > 0.0f);
     DANCE_REQUIRE(usable(lr, momentum, weight_decay));
@@ -1412,32 +1482,37 @@ extern "C" int dance_muon_step(const dance_muon_item *items_host, int count, int
     }
     const int64_t need = dance_muon_workspace_bytes(items_host, count);
     DANCE_REQUIRE(ws_bytes >= need && (ws || need == 0));
-    for (int b0 = 0; b0 < count; b0 += NS_ITEMS) {
-        NsTable t;
-        memset(&t, 0, sizeof t);
-        t.count = count - b0 < NS_ITEMS ? count - b0 : NS_ITEMS;
-        t.dtype = dtype;
-        t.muon = 1;
-        t.nesterov = nesterov != 0;
-        t.momentum = (float)momentum;
-        t.fresh = (float)(1.0 - momentum);
-        t.keep = (float)(1.0 - lr * weight_decay);
-        t.steps = steps;
-        t.a = a; t.b = b; t.c = c;
-        t.q_mul = q_scale(a, b, c);
-        t.eps = (double)eps;
-        for (int i = 0; i < t.count; ++i) {
-            const dance_muon_item &h = items_host[b0 + i];
-            t.it[i].src = h.grad;
-            t.it[i].momentum = h.momentum;
-            t.it[i].dst = h.param;
-            t.it[i].m = h.rows;
-            t.it[i].n = h.cols;
-            const double shape = h.rows > h.cols ? sqrt((double)h.rows / (double)h.cols) : 1.0;
-            t.it[i].scale = (float)(lr * shape);
+    for (int at[2] = {0, 0}; at[0] < count || at[1] < count;) {
+        // the narrow matrices and the others: two chains, launched in turn so that two streams run beside each other
+        Chain chains[2];
+        char *space = (char *)ws;
+        for (int wide = 1; wide >= 0; --wide) {
+            NsTable &t = chains[wide].t;
+            memset(&t, 0, sizeof t);
+            at[wide] = take(items_host, count, wide, at[wide], t);
+            t.dtype = dtype;
+            t.muon = 1;
+            t.nesterov = nesterov != 0;
+            t.momentum = (float)momentum;
+            t.fresh = (float)(1.0 - momentum);
+            t.keep = (float)(1.0 - lr * weight_decay);
+            t.steps = steps;
+            t.a = a; t.b = b; t.c = c;
+            t.q_mul = q_scale(a, b, c);
+            t.eps = (double)eps;
+            for (int i = 0; i < t.count; ++i) {
+                const double m = t.it[i].m, n = t.it[i].n;
+                t.it[i].scale = (float)(lr * (m > n ? sqrt(m / n) : 1.0));
+            }
+            const int64_t bytes = lay_out(t, space);
+            if (int rc = chains[wide].prepare(space, (hipStream_t)(wide && side_stream ? side_stream : stream), __func__))
+                return rc;
+            space += bytes;
         }
-        if (int rc = run_chain(t, (char *)ws, (hipStream_t)stream, __func__))
-            return rc;
+        for (int s = -1; s < steps; ++s)
+            for (int wide = 1; wide >= 0; --wide)
+                if (int rc = chains[wide].step(s))
+                    return rc;
     }
     return 0;
 }

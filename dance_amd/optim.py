@@ -7,10 +7,23 @@ is one chain of launches for all matrices of one type and device, whatever their
 
 The reference trains with Detectron2's SGD (train_net.py:22-70) and has no counterpart.
 """
+import struct
+
 import torch
 
-from ._lib import MuonItemStruct, check, lib, on_device, stream_of
+from ._lib import MuonItemStruct, check, lib, on_device, ptr, stream_of
 from .ops import DTYPE_CODES, NS_COEFFICIENTS, _need_gpu, _scratch, check_newton_schulz
+
+
+NARROW_ROWS = 128           # up to so many rows (of the smaller side) a step of the chain is a launch of its own
+
+_SIDE = {}
+
+
+def _side_stream(dev):
+    if dev not in _SIDE:
+        _SIDE[dev] = torch.cuda.Stream(dev)
+    return _SIDE[dev]
 
 
 def _rows_outermost(t):
@@ -24,6 +37,17 @@ def _rows_outermost(t):
             return False
         dense *= size
     return t.size(0) == 1 or t.stride(0) == dense
+
+
+def _refuse(what, p, g, m):
+    _need_gpu(p, g, m)
+    if p.dim() < 2 or p.dtype not in DTYPE_CODES:
+        raise RuntimeError("%s: matrices of fp32, fp16 or bf16 expected, got a %s parameter of shape %s"
+                           % (what, p.dtype, tuple(p.shape)))
+    for name, t in (("gradient", g), ("momentum buffer", m)):
+        if t.shape != p.shape or t.dtype != p.dtype or t.device != p.device:
+            raise RuntimeError("%s: a %s %s %s on %s for a parameter %s %s on %s"
+                               % (what, name, tuple(t.shape), t.dtype, t.device, tuple(p.shape), p.dtype, p.device))
 
 
 @torch.no_grad()
@@ -42,41 +66,53 @@ def muon_step(params, grads, momentum_buffers, *, lr, momentum=0.95, nesterov=Tr
     if not len(params) == len(grads) == len(momentum_buffers):
         raise RuntimeError("%s: %d params, %d grads, %d momentum buffers"
                            % (what, len(params), len(grads), len(momentum_buffers)))
-    chains, seen = {}, set()
+    # {(device, type): [device, dance_muon_item's fields one after the other, a narrow matrix among them?, a wide one?]}
+    chains, written, kept = {}, [], []
     for p, g, m in zip(params, grads, momentum_buffers):
-        _need_gpu(p, g, m)
-        if p.dim() < 2 or p.dtype not in DTYPE_CODES:
-            raise RuntimeError("%s: matrices of fp32, fp16 or bf16 expected, got a %s parameter of shape %s"
-                               % (what, p.dtype, tuple(p.shape)))
-        for name, t in (("gradient", g), ("momentum buffer", m)):
-            if t.shape != p.shape or t.dtype != p.dtype or t.device != p.device:
-                raise RuntimeError("%s: a %s %s %s on %s for a parameter %s %s on %s"
-                                   % (what, name, tuple(t.shape), t.dtype, t.device, tuple(p.shape), p.dtype, p.device))
-        if p.numel() == 0:
+        shape, dtype, index = p.shape, p.dtype, p.get_device()
+        if index < 0 or g.get_device() != index or m.get_device() != index or g.shape != shape or m.shape != shape or \
+                g.dtype is not dtype or m.dtype is not dtype or len(shape) < 2 or dtype not in DTYPE_CODES:
+            _refuse(what, p, g, m)
+        size = p.numel()
+        if size == 0:
             continue
-        if m.stride() != p.stride() or not _rows_outermost(p):
+        strides = p.stride()
+        if m.stride() != strides or not (p.is_contiguous() or _rows_outermost(p)):
             raise RuntimeError("%s: parameter and momentum buffer must be dense, rows outermost, with equal strides, got %s "
-                               "and %s of shape %s" % (what, p.stride(), m.stride(), tuple(p.shape)))
-        for t in (p, m):
-            if t.data_ptr() in seen:
-                raise RuntimeError("%s: a parameter or momentum buffer appears twice" % what)
-            seen.add(t.data_ptr())
-        if g.stride() != p.stride():
-            g = torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device).copy_(g)
-        chains.setdefault((p.device, p.dtype), []).append((p, g, m))
+                               "and %s of shape %s" % (what, strides, m.stride(), tuple(shape)))
+        if g.stride() != strides:
+            g = torch.empty_strided(shape, strides, dtype=dtype, device=p.device).copy_(g)
+            kept.append(g)
+        at, m_at, rows = p.data_ptr(), m.data_ptr(), shape[0]
+        cols = size // rows
+        key = (index, dtype)
+        chain = chains.get(key)
+        if chain is None:
+            chain = chains[key] = [p.device, [], False, False]
+        chain[1] += (at, g.data_ptr(), m_at, rows, cols)
+        chain[3 if rows > NARROW_ROWS and cols > NARROW_ROWS else 2] = True
+        written += (p, m)
+    places = [at for chain in chains.values() for k in (0, 2) for at in chain[1][k::5]]
+    if len(set(places)) != len(places):
+        raise RuntimeError("%s: a parameter or momentum buffer appears twice" % what)
     h = lib()
-    for (dev, dtype), chain in chains.items():
-        items = (MuonItemStruct * len(chain))()
-        for it, (p, g, m) in zip(items, chain):
-            it.param, it.grad, it.momentum = p.data_ptr(), g.data_ptr(), m.data_ptr()
-            it.rows, it.cols = p.size(0), p.numel() // p.size(0)
-        nbytes = h.dance_muon_workspace_bytes(items, len(chain))
-        ws = _scratch(nbytes, dev)
+    for (_, dtype), (dev, fields, narrow, wide) in chains.items():
+        count = len(fields) // 5
+        items = (MuonItemStruct * count).from_buffer_copy(struct.pack("@" + "PPPii" * count, *fields))
+        nbytes = h.dance_muon_workspace_bytes(items, count)
         with on_device(dev):
-            check(h.dance_muon_step(items, len(chain), DTYPE_CODES[dtype], lr, momentum, int(bool(nesterov)), weight_decay,
-                                    steps, a, b, c, eps, ws.data_ptr() if nbytes else None, nbytes, stream_of(dev)), what)
-        # written behind autograd's back: what caches by version (saved tensors, the modules' packed weights) must see it
-        torch.autograd.graph.increment_version([t for p, _, m in chain for t in (p, m)])
+            ws, cur, side = _scratch(nbytes, dev), None, None
+            if narrow and wide:                  # they leave each other room on the chip: beside each other on two streams
+                cur, side = torch.cuda.current_stream(dev), _side_stream(dev)
+                side.wait_stream(cur)
+            check(h.dance_muon_step(items, count, DTYPE_CODES[dtype], lr, momentum, int(bool(nesterov)), weight_decay, steps, a,
+                                    b, c, eps, ptr(ws), nbytes, stream_of(dev), None if side is None else side.cuda_stream),
+                  what)
+            if side is not None:
+                cur.wait_stream(side)
+    # written behind autograd's back: what caches by version (saved tensors, the modules' packed weights) must see it
+    if written:
+        torch.autograd.graph.increment_version(written)
 
 
 class Muon(torch.optim.Optimizer):

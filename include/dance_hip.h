@@ -702,7 +702,9 @@ int dance_orthogonalize(const void *x, int64_t batch_stride, int64_t row_stride,
  * parameter, gradient and momentum each:
  *   m <- momentum m + (1 - momentum) g;   u = nesterov ? momentum m + (1 - momentum) g : m
  *   p <- p (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) O,   O = orthogonalize(u)
- * in fp32, m and p rounded to the type once each.  items_host is read during the call only. */
+ * in fp32, m and p rounded to the type once each.  items_host is read during the call only.  side_stream: NULL,
+ * or a stream that matrices of more than 128 rows and columns run on beside the others; the caller makes it wait
+ * for `stream` before the call and `stream` for it afterwards. */
 typedef struct dance_muon_item {
     void *param;
     const void *grad;
@@ -712,7 +714,7 @@ typedef struct dance_muon_item {
 int64_t dance_muon_workspace_bytes(const dance_muon_item *items_host, int count);
 int dance_muon_step(const dance_muon_item *items_host, int count, int dtype, double lr, double momentum,
                     int nesterov, double weight_decay, int steps, float a, float b, float c, float eps,
-                    void *ws, int64_t ws_bytes, void *stream);
+                    void *ws, int64_t ws_bytes, void *stream, void *side_stream);
 
 #ifdef __cplusplus
 }

@@ -99,7 +99,7 @@ def test_orthogonalize_empty_and_workspace():
 
 def _muon(items, **over):
     a = dict(items=items, count=1, dtype=0, lr=0.1, momentum=0.9, nesterov=1, wd=0.0, steps=5, a=3.4445, b=-4.775, c=2.0315,
-             eps=1e-7, ws=None, ws_bytes=0, stream=None)
+             eps=1e-7, ws=None, ws_bytes=0, stream=None, side=None)
     a.update(over)
     return _lib.lib().dance_muon_step(*a.values())
 
