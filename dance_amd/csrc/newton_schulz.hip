@@ -621,6 +621,11 @@ __global__ __launch_bounds__(SUM_THREADS) void k_ns_sum(const NsTable *__restric
     const int side = narrow(d) ? PAD : t.gram_side, parts = side == PAD ? 4 : 1;
     const int part = local & (parts - 1);
     lower_tile(local / parts, ti, tj);
+    // A unit above the diagonal is the mirror image of the one below it, at either side of the tiles: the two products
+    // differ in their last bits, and a matrix gets the same bits whatever the launch holds besides it
+    const int i0 = ti * side + (part >> 1) * UNIT, j0 = tj * side + (part & 1) * UNIT;
+    if (i0 < j0)
+        return;
     const size_t share = (size_t)lower_tiles(d, side) * side * side / 4;
     const f32x4 *in = reinterpret_cast<const f32x4 *>(s.part + (size_t)(local / parts) * side * side) + part * 16 * 64 + threadIdx.x;
     f32x4 v = in[0];
@@ -642,10 +647,9 @@ __global__ __launch_bounds__(SUM_THREADS) void k_ns_sum(const NsTable *__restric
         tile[(16 * i + 4 * (lane >> 4) + q) * LD + 16 * j + (lane & 15)] = split_word(v[q] * dance::pow2f(-X_EXP));
     __syncthreads();
     const size_t plane = (size_t)d.rp * d.rp;
-    const int i0 = ti * side + (part >> 1) * UNIT, j0 = tj * side + (part & 1) * UNIT;
     if (threadIdx.x < SUM_THREADS / 2)
         put_rows<UNIT, UNIT, SUM_THREADS / 2>(s.a, plane, d.rp, i0, j0, tile);
-    else if (ti != tj)
+    else if (i0 != j0)
         put_cols<UNIT, UNIT, SUM_THREADS / 2>(s.a, plane, d.rp, i0, j0, tile, threadIdx.x - SUM_THREADS / 2);
 }
 
@@ -689,6 +693,14 @@ template <int F> __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_poly(co
         }
         return v;
     });
+    if (F == 4 && ti == tj) {
+        // the quarter above the diagonal from the one below it, as tiles of 64 have it
+        unsigned *w = reinterpret_cast<unsigned *>(lds);
+#pragma unroll 4
+        for (int e = threadIdx.x; e < 64 * 64; e += GEMM_THREADS)
+            w[(e & 63) * Tile<F>::LD + 64 + (e >> 6)] = w[(64 + (e >> 6)) * Tile<F>::LD + (e & 63)];
+        __syncthreads();
+    }
     put_rows<SIDE, SIDE, GEMM_THREADS>(s.q, plane, d.rp, i0, j0, tile);
     if (ti != tj)
         put_cols<SIDE, SIDE, GEMM_THREADS>(s.q, plane, d.rp, i0, j0, tile);

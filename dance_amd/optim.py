@@ -8,6 +8,7 @@ is one chain of launches for all matrices of one type and device, whatever their
 The reference trains with Detectron2's SGD (train_net.py:22-70) and has no counterpart.
 """
 import struct
+import threading
 
 import torch
 
@@ -17,13 +18,14 @@ from .ops import DTYPE_CODES, NS_COEFFICIENTS, _need_gpu, _scratch, check_newton
 
 NARROW_ROWS = 128           # up to so many rows (of the smaller side) a step of the chain is a launch of its own
 
-_SIDE = {}
+_SIDE = threading.local()    # a thread may be capturing its stream into a graph while another one steps
 
 
 def _side_stream(dev):
-    if dev not in _SIDE:
-        _SIDE[dev] = torch.cuda.Stream(dev)
-    return _SIDE[dev]
+    streams = _SIDE.__dict__
+    if dev not in streams:
+        streams[dev] = torch.cuda.Stream(dev)
+    return streams[dev]
 
 
 def _rows_outermost(t):
@@ -105,11 +107,11 @@ def muon_step(params, grads, momentum_buffers, *, lr, momentum=0.95, nesterov=Tr
             if narrow and wide:                  # they leave each other room on the chip: beside each other on two streams
                 cur, side = torch.cuda.current_stream(dev), _side_stream(dev)
                 side.wait_stream(cur)
-            check(h.dance_muon_step(items, count, DTYPE_CODES[dtype], lr, momentum, int(bool(nesterov)), weight_decay, steps, a,
-                                    b, c, eps, ptr(ws), nbytes, stream_of(dev), None if side is None else side.cuda_stream),
-                  what)
+            code = h.dance_muon_step(items, count, DTYPE_CODES[dtype], lr, momentum, int(bool(nesterov)), weight_decay, steps, a,
+                                     b, c, eps, ptr(ws), nbytes, stream_of(dev), None if side is None else side.cuda_stream)
             if side is not None:
-                cur.wait_stream(side)
+                cur.wait_stream(side)            # also where the call failed half way: the workspace is freed next
+            check(code, what)
     # written behind autograd's back: what caches by version (saved tensors, the modules' packed weights) must see it
     if written:
         torch.autograd.graph.increment_version(written)

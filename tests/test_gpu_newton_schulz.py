@@ -109,6 +109,36 @@ def test_orthogonal_it_is(device):
     assert float((got - u @ v).abs().max()) < 48 * 2.0 ** -22 * 4
 
 
+@pytest.mark.parametrize("shape", [(96, 150), (90, 100), (32, 500), (33, 34), (1, 3000), (16, 1500), (17, 17)])
+def test_around_one_workgroup(device, shape):
+    """sizes on both sides of what one workgroup keeps in its LDS, and of its 16 and 32 wide tiles"""
+    for dtype in (torch.float32, torch.bfloat16):
+        for x in (_matrix(*shape, 31).to(dtype), _matrix(*shape, 32, "gradient").to(dtype).t()):
+            _check(ops.orthogonalize(x.to(device)), x.double(), dtype, "%s %s" % (tuple(x.shape), dtype))
+
+
+@pytest.mark.parametrize("shape", [(100, 9000), (128, 20011), (20000, 65)])
+def test_long_narrow(device, shape):
+    """up to 128 rows and so many columns that a workgroup has several tiles of them; the Muon step too"""
+    x = _matrix(*shape, 33)
+    _check(ops.orthogonalize(x.to(device), steps=2), x.double(), torch.float32, str(shape), steps=2)
+    p, g, m = (_matrix(*shape, 34 + i).to(device) for i in range(3))
+    before = [(p.clone(), m.clone())]
+    optim.muon_step([p], [g], [m], lr=0.1)
+    _muon_check([p], [g], [m], before, torch.float32, 0.1, 0.95, True, 0.0, "long")
+
+
+@pytest.mark.parametrize("batch,shape", [(2, (600, 5000)), (18, (600, 640)), (3, (1100, 1100))])
+def test_enough_for_large_tiles(device, batch, shape):
+    """batches whose products have tiles enough of 128 x 128 for the whole chip: the bits of single calls, whose tiles
+    are of 64 x 64"""
+    x = torch.stack([_matrix(*shape, 40 + i, "gradient" if i % 2 else "noise") for i in range(batch)])
+    got = ops.orthogonalize(x.to(device), steps=2)
+    for i in (0, batch - 1):
+        assert torch.equal(ops.orthogonalize(x[i].to(device), steps=2), got[i]), i
+    _check(got[batch - 1], x[batch - 1].double(), torch.float32, "%d of %s" % (batch, shape), steps=2)
+
+
 def test_identities_to_the_bit(device):
     """a transposed matrix, a power of two, one of a batch, any strides: the same bits"""
     x = _matrix(96, 200, 5).to(device)
@@ -354,6 +384,69 @@ def test_streams_and_captured_graphs(device):
         optim.muon_step(*eager, lr=0.1)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(params + buffers, eager[0] + eager[2])), seed
+
+
+BOTH = [(64, 200), (150, 140), (20, 30), (200, 9, 3, 3), (128, 700), (300, 301), (257, 129)]
+
+
+@pytest.mark.parametrize("repeat", [1, 9])
+def test_narrow_and_wide_matrices_beside_each_other(device, repeat):
+    """both sides of 128 rows in one step, which then runs on two streams; also more of each than one launch takes.  Each
+    matrix gets the bits it has alone, but for the two that alone fit one workgroup's LDS, where the order of the sums
+    is another (_muon_check holds for all)"""
+    shapes = BOTH * repeat + [(140, 150)] * (repeat * repeat // 2)
+    def lists():
+        return [[_matrix(s[0], math.prod(s[1:]), 1000 * k + i).reshape(s).to(device) for i, s in enumerate(shapes)] for k in range(3)]
+    params, grads, buffers = lists()
+    optim.muon_step(params, grads, buffers, lr=0.1)
+    alone = lists()
+    before = [(p.clone(), m.clone()) for p, m in zip(alone[0], alone[2])]
+    for i in range(len(shapes)):
+        optim.muon_step(*[[t[i]] for t in alone], lr=0.1)
+    for i, s in enumerate(shapes):
+        assert s in ((20, 30), (64, 200)) or torch.equal(params[i], alone[0][i]), (i, s)
+        assert torch.equal(buffers[i], alone[2][i]), (i, s)
+    _muon_check(params[:7], grads, buffers, before, torch.float32, 0.1, 0.95, True, 0.0, "both")
+
+
+def test_captured_on_two_streams(device):
+    """the fork into the step's own stream and the join are part of a captured graph; two graphs and eager steps in turn,
+    captured and replayed on a stream of the caller's"""
+    def state():
+        return [[_matrix(s[0], math.prod(s[1:]), 100 * k + i).reshape(s).to(device) for i, s in enumerate(BOTH)] for k in range(3)]
+    captured, eager = [state(), state()], [state(), state()]
+    stream = torch.cuda.Stream(device)
+    graphs = [torch.cuda.CUDAGraph() for _ in captured]
+    for graph, s in zip(graphs, captured):
+        stream.wait_stream(torch.cuda.current_stream(device))
+        with torch.cuda.graph(graph, stream=stream):
+            optim.muon_step(*s, lr=0.1)
+    for turn in range(4):
+        for k in (0, 1):
+            for a, b in zip(captured[k][1], eager[k][1]):
+                new = _matrix(a.size(0), a.numel() // a.size(0), 10000 * turn + a.numel() + k).reshape(a.shape).to(device)
+                a.copy_(new)
+                b.copy_(new)
+            stream.wait_stream(torch.cuda.current_stream(device))
+            with torch.cuda.stream(stream):
+                graphs[k].replay()
+            optim.muon_step(*eager[k], lr=0.1)
+            torch.cuda.synchronize()
+        for k in (0, 1):
+            assert all(torch.equal(a, b) for a, b in zip(captured[k][0] + captured[k][2], eager[k][0] + eager[k][2])), (turn, k)
+
+
+def test_a_failing_step_is_joined(device):
+    """an error from the library is raised with the step's own stream joined, and the next step is right"""
+    params, grads, buffers = ([_matrix(s[0], math.prod(s[1:]), 100 * k + i).reshape(s).to(device) for i, s in enumerate(BOTH[:2])]
+                              for k in range(3))
+    kept = [p.clone() for p in params]
+    with pytest.raises(RuntimeError, match="requirement failed"):
+        optim.muon_step(params, grads, buffers, lr=float("nan"))
+    assert all(torch.equal(a, b) for a, b in zip(params, kept))
+    before = [(p.clone(), m.clone()) for p, m in zip(params, buffers)]
+    optim.muon_step(params, grads, buffers, lr=0.1)
+    _muon_check(params, grads, buffers, before, torch.float32, 0.1, 0.95, True, 0.0, "after an error")
 
 
 def test_training_a_norm_layer_stack(device):
