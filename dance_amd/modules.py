@@ -79,7 +79,9 @@ class _ConvNormAct(nn.Conv2d):
     (C -> C, C % 128 == 0, GroupNorm(32), no bias, dilation 1) runs on the feature-prep kernels
     (conv3x3 as split-half f16 MFMA implicit GEMM + GroupNorm + ReLU; output in
     channels_last memory); anything else, `DANCE_FEATPREP=torch`, or `use_hip = False` runs
-    the stock torch.nn ops."""
+    the stock torch.nn ops.  With `DANCE_GROUPNORM=hip` the norm and the activation of that path run on
+    ops.group_norm_act, in training mode and under autograd too, where the convolution's output is
+    channels_last."""
 
     use_hip = True
 
@@ -111,6 +113,9 @@ class _ConvNormAct(nn.Conv2d):
             if layer is not None:
                 return ops.bottom_out16(x, 0, [layer], groups=32, eps=self.norm.eps, measure=False).permute(0, 3, 1, 2)
         x = super().forward(x)
+        if (self.norm is not None and x.is_cuda and os.environ.get("DANCE_GROUPNORM", "torch") == "hip"
+                and ops.is_channels_last(x)):
+            return ops.group_norm_act(x, self.norm.num_groups, self.norm.weight, self.norm.bias, eps=self.norm.eps)
         if self.norm is not None:
             x = self.norm(x)
         return F.relu(x)

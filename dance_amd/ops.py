@@ -516,6 +516,11 @@ def _channels_last_strides(t):
     return (t.stride(0) if t.size(0) > 1 else 0), (t.size(1) if pixel is None else pixel)
 
 
+def is_channels_last(t):
+    """Does group_norm_act read this GPU tensor in place?"""
+    return t.is_cuda and t.dim() >= 2 and t.dtype in DTYPE_CODES and _channels_last_strides(t) is not None
+
+
 def _nhwc_view(t):
     """t itself when the kernels can walk its memory, else a dense channels-last copy."""
     strides = _channels_last_strides(t)

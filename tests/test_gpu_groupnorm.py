@@ -11,7 +11,7 @@ magnitudes.  On top comes half a step of the output's type."""
 import pytest
 import torch
 
-from dance_amd import ops
+from dance_amd import modules, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -353,3 +353,52 @@ def test_offsets_past_32_bits(device):
     dense = x.contiguous().reshape(1, 1, pixels, c).permute(0, 3, 1, 2)
     assert torch.equal(y, ops.group_norm_act(dense, 2, w, be))
     assert float(y[..., -4096:].float().abs().max()) > 0.5
+
+
+def test_conv_layers_use_it_when_asked(device, monkeypatch):
+    """modules._ConvNormAct under autograd with DANCE_GROUPNORM=hip against the stock path; a channels-first map stays on
+    the stock path.  The sums of both are of at most 960 fp32 terms (576 * 2^-24 = 3.4e-5 of their absolute sum for the
+    convolution alone, forward and backward), and where |z| is below 1e-3, which the two may see on either side of the
+    ReLU's border, the gradient is zero: 1e-4 of the norms, 1e-3 of the weight's (sums of cancelling terms)."""
+    g = torch.Generator().manual_seed(3)
+    layer = modules._ConvNormAct(64, 96, 1, "GN").to(device).to(memory_format=torch.channels_last)
+    with torch.no_grad():
+        for p in layer.parameters():
+            p.copy_(torch.randn(p.shape, generator=g) * (0.05 if p.dim() == 4 else 0.3) + (p.dim() == 1))
+    x = torch.randn((2, 64, 20, 24), generator=g).to(device)
+    dy = torch.randn((2, 96, 20, 24), generator=g).to(device)
+    with torch.no_grad():
+        z = layer.norm.to(device)(torch.nn.functional.conv2d(x, layer.weight, layer.bias, padding=1))
+    dy = dy * (z.abs() > 1e-3)
+    calls = []
+    real = ops.group_norm_act
+    monkeypatch.setattr(ops, "group_norm_act", lambda *a, **k: calls.append(1) or real(*a, **k))
+    results = {}
+    for knob in ("torch", "hip"):
+        monkeypatch.setenv("DANCE_GROUPNORM", knob)
+        xr = x.to(memory_format=torch.channels_last).requires_grad_(True)
+        y = layer(xr)
+        results[knob] = (y,) + torch.autograd.grad(y, [xr] + list(layer.parameters()), dy)
+        assert len(calls) == (knob == "hip")
+    for i, (a, b) in enumerate(zip(results["hip"], results["torch"])):
+        assert a.shape == b.shape and float((a - b).norm()) <= (1e-4 if i < 2 else 1e-3) * float(b.norm())
+    monkeypatch.setattr(ops, "is_channels_last", lambda t: False)
+    assert layer(x).shape == dy.shape
+    assert len(calls) == 1
+
+
+@pytest.mark.parametrize("dtype,c,lo,hi", [(torch.float32, 72, 0, 72), (torch.float32, 75, 1, 73), (torch.bfloat16, 143, 3, 139)])
+def test_maps_larger_than_the_cache(device, dtype, c, lo, hi):
+    """maps of more than 64 MB are read and written past the cache: aligned, and at odd elements with channels around
+    them, which get a gradient of zero.  (A thread sums 16 pixels at these sizes, half of N_T.)"""
+    full = _map((2, c, 257, 463), dtype, device, c).permute(0, 2, 3, 1).contiguous().requires_grad_(True)
+    x = full.permute(0, 3, 1, 2)[:, lo:hi]
+    assert x.numel() * x.element_size() >= 64e6
+    w, be = (t.requires_grad_(True) for t in _affine(hi - lo, torch.float32, device, c))
+    y = ops.group_norm_act(x, 8, w, be)
+    dy = _map(tuple(x.shape), dtype, device, c + 1)
+    dfull, dw, db = torch.autograd.grad(y, (full, w, be), dy)
+    want = _oracle(x, 8, w, be, "relu", dy)
+    for name, got in (("y", y), ("dx", dfull.permute(0, 3, 1, 2)[:, lo:hi]), ("dweight", dw), ("dbias", db)):
+        _check(got, want[name], name)
+    assert not bool(dfull[..., :lo].any()) and not bool(dfull[..., hi:].any())
