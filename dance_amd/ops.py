@@ -530,8 +530,14 @@ def _nhwc_view(t):
     return (t,) + strides
 
 
-def _empty_nhwc(shape, dtype, device):
-    return torch.empty((shape[0],) + tuple(shape[2:]) + (shape[1],), dtype=dtype, device=device).movedim(-1, 1)
+def _nhwc_strides(shape):
+    """a dense channels-last map's"""
+    strides, dense = [1] * len(shape), shape[1]
+    for i in range(len(shape) - 1, 1, -1):
+        strides[i] = dense
+        dense *= shape[i]
+    strides[0] = dense
+    return tuple(strides)
 
 
 def _scratch(nbytes, device):
@@ -539,14 +545,15 @@ def _scratch(nbytes, device):
 
 
 def _group_norm_forward(x, groups, weight, bias, eps, act):
-    """-> (y, the map as it was read, what the backward call takes)"""
-    shape, dev = x.shape, x.device
+    """-> (y, the map as it was read, what the backward call takes: a tensor, and sizes and strides)"""
+    shape, dev, dtype = x.shape, x.device, x.dtype
     b, c, hw = shape[0], shape[1], math.prod(shape[2:])
     x, image, pixel = _nhwc_view(x)
-    y = _empty_nhwc(shape, x.dtype, dev)
+    strides = _nhwc_strides(shape)
+    y = torch.empty_strided(shape, strides, dtype=dtype, device=dev)
     h = lib()
     saved = torch.empty((h.dance_group_norm_saved_bytes(b, c, groups),), dtype=torch.uint8, device=dev)
-    dt, affine = DTYPE_CODES[x.dtype], weight if weight is not None else bias
+    dt, affine = DTYPE_CODES[dtype], weight if weight is not None else bias
     at = DTYPE_F32 if affine is None else DTYPE_CODES[affine.dtype]
     nbytes = h.dance_group_norm_workspace_bytes(b, c, hw, groups, dt, 0)
     ws = _scratch(nbytes, dev)
@@ -554,15 +561,14 @@ def _group_norm_forward(x, groups, weight, bias, eps, act):
         check(h.dance_group_norm_act(x.data_ptr(), image, pixel, dt, ptr(weight), ptr(bias), at, eps, act, groups,
                                      y.data_ptr(), saved.data_ptr(), ptr(ws), nbytes, b, c, hw, stream_of(dev)),
               "group_norm_act")
-    return y, x, saved
+    return y, x, saved, (strides, image, pixel, dt, at, act, groups, b, c, hw)
 
 
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
-        y, x, saved = _group_norm_forward(x, groups, weight, bias, eps, act)
+        y, x, saved, ctx.sizes = _group_norm_forward(x, groups, weight, bias, eps, act)
         ctx.save_for_backward(x, weight, bias, saved)
-        ctx.groups, ctx.act = groups, act
         return y
 
     @staticmethod
@@ -570,23 +576,22 @@ class _GroupNormAct(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, bias, saved = ctx.saved_tensors
         want_x, want_w, want_b = ctx.needs_input_grad[:3]
-        shape, dev = x.shape, x.device
-        b, c, hw = shape[0], shape[1], math.prod(shape[2:])
-        dx = _empty_nhwc(shape, x.dtype, dev) if want_x else None
+        strides, image, pixel, dt, at, act, groups, b, c, hw = ctx.sizes
+        dev = x.device
+        dx = torch.empty_strided(x.shape, strides, dtype=x.dtype, device=dev) if want_x else None
         dw = torch.empty_like(weight) if want_w else None
         db = torch.empty_like(bias) if want_b else None
         if b == 0 or hw == 0:                        # empty sums
             return dx, dw if dw is None else dw.zero_(), db if db is None else db.zero_(), None, None, None
-        dy, dy_image, dy_pixel = _nhwc_view(dy)
-        image, pixel = _channels_last_strides(x)
-        dt, affine = DTYPE_CODES[x.dtype], weight if weight is not None else bias
-        at = DTYPE_F32 if affine is None else DTYPE_CODES[affine.dtype]
+        dy_image, dy_pixel = c * hw, c
+        if dy.stride() != strides:
+            dy, dy_image, dy_pixel = _nhwc_view(dy)
         h = lib()
-        nbytes = h.dance_group_norm_workspace_bytes(b, c, hw, ctx.groups, dt, 1)
+        nbytes = h.dance_group_norm_workspace_bytes(b, c, hw, groups, dt, 1)
         ws = _scratch(nbytes, dev)
         with on_device(dev):
             check(h.dance_group_norm_act_backward(dy.data_ptr(), dy_image, dy_pixel, x.data_ptr(), image, pixel, dt,
-                                                  at, ctx.act, ctx.groups, saved.data_ptr(), ptr(dx), ptr(dw), ptr(db),
+                                                  at, act, groups, saved.data_ptr(), ptr(dx), ptr(dw), ptr(db),
                                                   ptr(ws), nbytes, b, c, hw, stream_of(dev)),
                   "group_norm_act backward")
         return dx, dw, db, None, None, None
