@@ -31,6 +31,7 @@ namespace {
 using dance::launch_check;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
 constexpr int PAD = 128;                            // rows and columns are padded to whole tiles of the GEMM
@@ -250,14 +251,49 @@ template <typename T, bool DENSE> __global__ __launch_bounds__(256) void k_ns_no
 }
 
 // ------------------------------------------------------------------------------ tiles in LDS, split
-// hi in the low half, lo in the high one: dance::split_half as one word
-__device__ __forceinline__ unsigned split_word(float x)
+// What hi = fp16(x) leaves of x, exactly: one v_fma_mix_f32, which reads the half as it lies (with a constant factor
+// the compiler makes a conversion and a subtraction of it).  With the two conversions of v_cvt_pk_f16_f32 a pair of
+// values is split by four instructions; the epilogues of the products are bound by them.
+__device__ __forceinline__ float rest_of(_Float16 hi, float x)
+{
+    float minus = -1.0f;
+    asm("" : "+s"(minus));
+    return fmaf((float)hi, minus, x);
+}
+
+__device__ __forceinline__ unsigned pack2(float a, float b) { return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{a, b}, h2)); }
+
+// x as a value of its own: out of a product the compiler would else round hi in one go (v_fma_mixlo_f16), and for one of
+// its two uses only
+__device__ __forceinline__ float settled(float x)
 {
     asm("" : "+v"(x));
-    h2 p;
-    p[0] = (_Float16)x;
-    p[1] = (_Float16)(x - (float)p[0]);
-    return __builtin_bit_cast(unsigned, p);
+    return x;
+}
+
+// hi in the low half, lo in the high one: dance::split_half as one word
+__device__ __forceinline__ unsigned split_word(float value)
+{
+    const float x = settled(value);
+    return pack2(x, rest_of((_Float16)x, x));
+}
+
+// four values' halves, two of one plane a word
+struct Quad {
+    unsigned hi[2], lo[2];
+};
+
+__device__ __forceinline__ Quad split4(const f32x4 &x)
+{
+    Quad r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float a = settled(x[2 * i]), b = settled(x[2 * i + 1]);
+        const h2 h = __builtin_convertvector(f32x2{a, b}, h2);
+        r.hi[i] = __builtin_bit_cast(unsigned, h);
+        r.lo[i] = pack2(rest_of(h[0], a), rest_of(h[1], b));
+    }
+    return r;
 }
 
 // c v + b A of an entry, A from its halves
@@ -276,28 +312,33 @@ __device__ __forceinline__ void put8(_Float16 *p, size_t plane, const unsigned (
     *reinterpret_cast<uint4 *>(p + plane) = uint4{lo_pair(x[0], x[1]), lo_pair(x[2], x[3]), lo_pair(x[4], x[5]), lo_pair(x[6], x[7])};
 }
 
-__device__ __forceinline__ void put4(_Float16 *p, size_t plane, unsigned a, unsigned b, unsigned c, unsigned d)
+__device__ __forceinline__ void put4(_Float16 *p, size_t plane, const Quad &x)
 {
-    *reinterpret_cast<uint2 *>(p) = uint2{hi_pair(a, b), hi_pair(c, d)};
-    *reinterpret_cast<uint2 *>(p + plane) = uint2{lo_pair(a, b), lo_pair(c, d)};
+    *reinterpret_cast<uint2 *>(p) = uint2{x.hi[0], x.hi[1]};
+    *reinterpret_cast<uint2 *>(p + plane) = uint2{x.lo[0], x.lo[1]};
 }
 
-// 4 x 4 words over 4 neighbouring lanes transposed: lane l's word q becomes lane q's word l
-__device__ __forceinline__ void transpose4(unsigned (&x)[4])
+// 4 x 4 halves over 4 neighbouring lanes transposed: lane l's half q becomes lane q's half l
+__device__ __forceinline__ void transpose4(unsigned (&x)[2])
 {
     const bool odd = threadIdx.x & 1, upper = threadIdx.x & 2;
-    auto swap = [](unsigned &a, unsigned &b, bool second, auto pattern) {       // b of the first lane against a of the second
-        const unsigned sent = second ? a : b;
-        const unsigned got = (unsigned)__builtin_amdgcn_mov_dpp((int)sent, decltype(pattern)::value, 0xf, 0xf, true);
-        a = second ? got : a;
-        b = second ? b : got;
-    };
-    constexpr std::integral_constant<int, 0xB1> by1{};                   // quad_perm 1 0 3 2
-    constexpr std::integral_constant<int, 0x4E> by2{};                   // quad_perm 2 3 0 1
-    swap(x[0], x[1], odd, by1);
-    swap(x[2], x[3], odd, by1);
-    swap(x[0], x[2], upper, by2);
-    swap(x[1], x[3], upper, by2);
+    // the second word of a lane against the first of the one two further
+    const unsigned got = (unsigned)__builtin_amdgcn_mov_dpp((int)(upper ? x[0] : x[1]), 0x4E, 0xf, 0xf, true);     // 2 3 0 1
+    x[0] = upper ? got : x[0];
+    x[1] = upper ? x[1] : got;
+    // both words' low halves of an even lane and its neighbour, or their high ones
+    const unsigned pick = odd ? 0x03020706u : 0x05040100u;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const unsigned other = (unsigned)__builtin_amdgcn_mov_dpp((int)x[i], 0xB1, 0xf, 0xf, true);                // 1 0 3 2
+        x[i] = __builtin_amdgcn_perm(other, x[i], pick);
+    }
+}
+
+__device__ __forceinline__ void transpose4(Quad &x)
+{
+    transpose4(x.hi);
+    transpose4(x.lo);
 }
 
 // tile [I][J] of split words in LDS, row stride J + 1 (odd: conflict-free both ways) -> operand with rows i (from i0
@@ -833,11 +874,7 @@ __device__ __forceinline__ void zero(f32x4 (&acc)[4][2])
 __device__ __forceinline__ void narrow_put_square(char *region, const f32x4 (&m)[4][2])
 {
     narrow_each([&](int i, int j, int row, int col) {
-        unsigned x[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            x[q] = split_word(m[i][j][q]);
-        put4((_Float16 *)region + ((row >> 3) * PAD + col) * 8 + (row & 7), REGION / 4, x[0], x[1], x[2], x[3]);
+        put4((_Float16 *)region + ((row >> 3) * PAD + col) * 8 + (row & 7), REGION / 4, split4(m[i][j]));
     });
 }
 
@@ -916,14 +953,10 @@ template <typename T> __global__ __launch_bounds__(NARROW_THREADS) void k_ns_nar
                 // in place, and with k along the columns for the share of A
                 _Float16 *to = s.xr[0] + (size_t)c * PAD * 8;
                 narrow_each([&](int i, int j, int row, int col) {
-                    unsigned x[4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        x[q] = split_word(v[i][j][q] * mul);
-                    put4(to + ((size_t)(row >> 3) * d.kp + col) * 8 + (row & 7), rect, x[0], x[1], x[2], x[3]);
+                    Quad x = split4(v[i][j] * mul);
+                    put4(to + ((size_t)(row >> 3) * d.kp + col) * 8 + (row & 7), rect, x);
                     transpose4(x);                            // 4 columns of row row + lane % 4
-                    put4((_Float16 *)columns + ((col >> 3) * PAD + row + (threadIdx.x & 3)) * 8 + (col & 4), REGION / 4, x[0],
-                         x[1], x[2], x[3]);
+                    put4((_Float16 *)columns + ((col >> 3) * PAD + row + (threadIdx.x & 3)) * 8 + (col & 4), REGION / 4, x);
                 });
                 __syncthreads();
                 narrow_gemm(next, columns, columns);
@@ -1097,8 +1130,7 @@ template <typename T, bool DENSE> __global__ __launch_bounds__(SMALL_THREADS) vo
     const float mul = 1.0f / t.q_mul;
     // a fragment of a symmetric matrix at (i0, j0): entered at its mirror image, where a lane's 4 values are neighbours
     auto put_square = [&](const f32x4 &v, int i0, int j0) {
-        put4(a + (((i0 + i4) >> 3) * d.rp + j0 + j1) * 8 + (i4 & 7), square, split_word(v[0]), split_word(v[1]), split_word(v[2]),
-             split_word(v[3]));
+        put4(a + (((i0 + i4) >> 3) * d.rp + j0 + j1) * 8 + (i4 & 7), square, split4(v));
     };
 #pragma unroll 1
     for (int step = 0; step < t.steps; ++step) {
@@ -1162,13 +1194,10 @@ template <typename T, bool DENSE> __global__ __launch_bounds__(SMALL_THREADS) vo
                 const f32x4 x = (hh + (hl + lh)) * mul;
                 const int i = i0 + i4, j = j0 + j1;
                 if (step + 1 < t.steps) {
-                    unsigned y[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        y[e] = split_word(x[e]);
-                    put4(xr + ((i >> 3) * d.kp + j) * 8 + (i & 7), rect, y[0], y[1], y[2], y[3]);
+                    Quad y = split4(x);
+                    put4(xr + ((i >> 3) * d.kp + j) * 8 + (i & 7), rect, y);
                     transpose4(y);                                // 4 columns of row i + lane % 4
-                    put4(xk + ((j >> 3) * d.rp + i + (lane & 3)) * 8 + (j & 4), rect, y[0], y[1], y[2], y[3]);
+                    put4(xk + ((j >> 3) * d.rp + i + (lane & 3)) * 8 + (j & 4), rect, y);
                 } else {
                     const int step_i = d.tall ? 1 : it.n;
                     T *to = (T *)it.dst + (d.tall ? j * it.n + i : i * it.n + j);
