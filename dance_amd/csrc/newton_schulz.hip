@@ -987,8 +987,7 @@ template <typename T> __global__ __launch_bounds__(NARROW_THREADS) void k_ns_nar
 constexpr int SMALL_THREADS = 1024, SMALL_WAVES = SMALL_THREADS / 64, SMALL_PAD = 32;
 constexpr size_t SMALL_LDS = 160 * 1024;
 constexpr size_t SMALL_MOST = SMALL_LDS - 1024;
-constexpr int SMALL_SQUARE = 3;                     // fragments of Q a wave, and steps of 32 over the rows, at most:
-static_assert(12 * 128 * 128 > SMALL_MOST && 96 * 96 / 256 <= SMALL_SQUARE * SMALL_WAVES, "12 rp^2 bytes at least: rp <= 96");
+static_assert(12 * 128 * 128 > SMALL_MOST, "12 rp^2 bytes at least: rp <= 96");
 
 struct SmallDims {
     int r, k, rp, kp, tall;
@@ -1007,25 +1006,196 @@ __host__ __device__ inline SmallDims small_dims(int m, int n)
     return d;
 }
 
-// acc += a fragment of U V' at rows i0 of U, j0 of V, k from 0 to k; operands in LDS, their planes `plane` halves apart
-__device__ __forceinline__ f32x4 small_gemm(const _Float16 *u, int u_rows, int u_plane, int i0, const _Float16 *v, int v_rows,
-                                            int v_plane, int j0, int k)
+// A fragment of U V': this lane's first words of U and V, `rows` words from one block of 8 k to the next, planes `plane`
+// halves apart, over `steps` steps of 32 k.  A step's words are read while the one before is multiplied, into the other
+// of two sets of registers (the compiler does not unroll the loop, matrix instructions are convergent).
+__device__ __forceinline__ f32x4 small_gemm(const _Float16 *u, const _Float16 *v, int rows, int plane, int steps)
 {
-    const int lane = threadIdx.x & 63, kb = lane >> 4, row = lane & 15;
-    const _Float16 *up = u + (kb * u_rows + i0 + row) * 8, *vp = v + (kb * v_rows + j0 + row) * 8;
     // three sums, so that a product does not wait for the one before it
     f32x4 hh = {0.0f, 0.0f, 0.0f, 0.0f}, hl = hh, lh = hh;
+    h8 uh[2], ul[2], vh[2], vl[2];
+    auto load = [&](int set, int step) {
+        const _Float16 *us = u + step * 32 * rows, *vs = v + step * 32 * rows;
+        uh[set] = *reinterpret_cast<const h8 *>(us);
+        ul[set] = *reinterpret_cast<const h8 *>(us + plane);
+        vh[set] = *reinterpret_cast<const h8 *>(vs);
+        vl[set] = *reinterpret_cast<const h8 *>(vs + plane);
+    };
+    auto multiply = [&](int set) {
+        lh = __builtin_amdgcn_mfma_f32_16x16x32_f16(ul[set], vh[set], lh, 0, 0, 0);
+        hl = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[set], vl[set], hl, 0, 0, 0);
+        hh = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[set], vh[set], hh, 0, 0, 0);
+    };
+    load(0, 0);
 #pragma unroll 1
-    for (int s = 0; s < k; s += 32) {
-        const h8 uh = *reinterpret_cast<const h8 *>(up), ul = *reinterpret_cast<const h8 *>(up + u_plane);
-        const h8 vh = *reinterpret_cast<const h8 *>(vp), vl = *reinterpret_cast<const h8 *>(vp + v_plane);
-        lh = __builtin_amdgcn_mfma_f32_16x16x32_f16(ul, vh, lh, 0, 0, 0);
-        hl = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh, vl, hl, 0, 0, 0);
-        hh = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh, vh, hh, 0, 0, 0);
-        up += 32 * u_rows;
-        vp += 32 * v_rows;
+    for (int s = 1; s < steps; s += 2) {
+        load(1, s);
+        multiply(0);
+        load(0, min(s + 1, steps - 1));
+        multiply(1);
     }
+    if (steps & 1)
+        multiply(0);
     return hh + (hl + lh);
+}
+
+// a / b of small numbers (a < 2^20) by the reciprocal 1 / b: a + 1/2 is at least 1/2 from a multiple of b, the error of
+// the product at most 2^-23 (a + 1/2) / b
+__device__ __forceinline__ int small_div(int a, float reciprocal) { return (int)(((float)a + 0.5f) * reciprocal); }
+
+struct SmallSettings {
+    float ca, ba, one, mul;
+    int steps;
+};
+
+// The unscaled M in LDS as fp32 [i][j], behind xk -> the result, for rp = 32 R
+template <int R, typename T>
+__device__ __forceinline__ void small_steps(const NsTable &t, const NsItem &it, const SmallDims &d, const SmallSettings &c,
+                                            Scale scaled, _Float16 *xk)
+{
+    constexpr int RP = 32 * R, FR = 2 * R, LOWER = FR * (FR + 1) / 2, MINE = (LOWER + SMALL_WAVES - 1) / SMALL_WAVES, SQUARE = RP * RP;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int rect = RP * d.kp, ld = d.kp + 1;
+    _Float16 *xr = xk + 2 * rect, *a = xr + 2 * rect;
+    const float *tile = reinterpret_cast<const float *>(xr);
+    // X both ways.  The words that replace the tile wait in registers until everybody has read it.
+    constexpr int HELD = (int)(SMALL_MOST / 64 / SMALL_THREADS) + 1;
+    Quad held[HELD][2];
+    const float per_k = 1.0f / (float)d.kp;
+#pragma unroll
+    for (int n = 0; n < HELD; ++n) {
+        const int w = threadIdx.x + n * SMALL_THREADS, ib = small_div(w, per_k), j = w - ib * d.kp;
+        if (w < rect / 8) {
+            const float *from = tile + ib * 8 * ld + j;
+#pragma unroll
+            for (int h = 0; h < 2; ++h, from += 4 * ld)
+                held[n][h] = split4(f32x4{scaled(from[0]), scaled(from[ld]), scaled(from[2 * ld]), scaled(from[3 * ld])});
+        }
+    }
+#pragma unroll 1
+    for (int w = threadIdx.x; w < rect / 8; w += SMALL_THREADS) {
+        const float *from = tile + w % RP * ld + w / RP * 8;
+#pragma unroll
+        for (int h = 0; h < 2; ++h, from += 4)
+            put4(xk + w * 8 + 4 * h, rect, split4(f32x4{scaled(from[0]), scaled(from[1]), scaled(from[2]), scaled(from[3])}));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < HELD; ++n) {
+        const int w = threadIdx.x + n * SMALL_THREADS;
+        if (w < rect / 8)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                put4(xr + w * 8 + 4 * h, rect, held[n][h]);
+    }
+    __syncthreads();
+
+    const int i4 = 4 * (lane >> 4), j1 = lane & 15;               // a lane's rows and column in a fragment
+    const int word = ((lane >> 4) * RP + j1) * 8;                 // its first word of a side, at row 0
+    int i0[MINE], j0[MINE];                                       // the wave's fragments on and below the diagonal
+#pragma unroll
+    for (int n = 0; n < MINE; ++n) {
+        lower_tile(wave + n * SMALL_WAVES, i0[n], j0[n]);
+        i0[n] = __builtin_amdgcn_readfirstlane(i0[n]) * 16;
+        j0[n] = __builtin_amdgcn_readfirstlane(j0[n]) * 16;
+    }
+    // a fragment of a symmetric matrix: its mirror image, where a lane's 4 values are neighbours, and itself
+    auto put_square = [&](const f32x4 &v, int i0, int j0) {
+        Quad x = split4(v);
+        put4(a + (((i0 + i4) >> 3) * RP + j0 + j1) * 8 + (i4 & 7), SQUARE, x);
+        if (i0 != j0) {
+            transpose4(x);                                        // 4 columns of row i + lane % 4
+            put4(a + (((j0 + j1) >> 3) * RP + i0 + i4 + (lane & 3)) * 8 + (j1 & 4), SQUARE, x);
+        }
+    };
+#pragma unroll 1
+    for (int step = 1;; ++step) {
+#pragma unroll
+        for (int n = 0; n < MINE; ++n)
+            if (wave + n * SMALL_WAVES < LOWER)
+                put_square(small_gemm(xk + word + i0[n] * 8, xk + word + j0[n] * 8, RP, rect, d.kp / 32) * dance::pow2f(-X_EXP), i0[n],
+                           j0[n]);
+        __syncthreads();
+        f32x4 q[MINE];
+#pragma unroll
+        for (int n = 0; n < MINE; ++n) {
+            if (wave + n * SMALL_WAVES >= LOWER)
+                continue;
+            q[n] = small_gemm(a + word + i0[n] * 8, a + word + j0[n] * 8, RP, SQUARE, R);
+            const _Float16 *p = a + (((i0[n] + i4) >> 3) * RP + j0[n] + j1) * 8 + (i4 & 7);
+            const h4 ah = *reinterpret_cast<const h4 *>(p), al = *reinterpret_cast<const h4 *>(p + SQUARE);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                q[n][e] = poly_of(c.ca, q[n][e], c.ba, ah[e], al[e]);
+            if (i0[n] == j0[n]) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    q[n][e] += i4 + e == j1 && j0[n] + j1 < d.r ? c.one : 0.0f;
+            }
+        }
+        __syncthreads();                                          // every wave has read A: Q takes its place
+#pragma unroll
+        for (int n = 0; n < MINE; ++n)
+            if (wave + n * SMALL_WAVES < LOWER)
+                put_square(q[n], i0[n], j0[n]);
+        __syncthreads();
+        // X <- Q X: a wave owns 16 columns of X at a time, holds them in registers and replaces them
+        const bool last = step == c.steps;
+#pragma unroll 1
+        for (int f = wave; f < d.kp / 16; f += SMALL_WAVES) {
+            const int j = f * 16 + j1;
+            h8 vh[R], vl[R];
+#pragma unroll
+            for (int n = 0; n < R; ++n) {
+                const _Float16 *p = xr + ((n * 4 + (lane >> 4)) * d.kp + j) * 8;
+                vh[n] = *reinterpret_cast<const h8 *>(p);
+                vl[n] = *reinterpret_cast<const h8 *>(p + rect);
+            }
+            auto fragment = [&](int i0) {
+                f32x4 hh = {0.0f, 0.0f, 0.0f, 0.0f}, hl = hh, lh = hh;
+#pragma unroll
+                for (int n = 0; n < R; ++n) {
+                    const _Float16 *p = a + word + (n * 4 * RP + i0) * 8;
+                    const h8 uh = *reinterpret_cast<const h8 *>(p), ul = *reinterpret_cast<const h8 *>(p + SQUARE);
+                    lh = __builtin_amdgcn_mfma_f32_16x16x32_f16(ul, vh[n], lh, 0, 0, 0);
+                    hl = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh, vl[n], hl, 0, 0, 0);
+                    hh = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh, vh[n], hh, 0, 0, 0);
+                }
+                return (hh + (hl + lh)) * c.mul;
+            };
+            if (!last) {
+                _Float16 *to_r = xr + ((i4 >> 3) * d.kp + j) * 8 + (i4 & 7);
+                _Float16 *to_k = xk + ((j >> 3) * RP + i4 + (lane & 3)) * 8 + (j & 4);
+#pragma unroll
+                for (int i = 0; i < RP; i += 16) {
+                    Quad x = split4(fragment(i));
+                    put4(to_r + i * d.kp, rect, x);
+                    transpose4(x);
+                    put4(to_k + i * 8, rect, x);
+                }
+            } else {
+                const int step_i = d.tall ? 1 : it.n;
+                const float out = dance::pow2f(-X_EXP);
+#pragma unroll 1
+                for (int i0 = 0; i0 < RP; i0 += 16) {
+                    const int i = i0 + i4;
+                    T *to = (T *)it.dst + (d.tall ? j * it.n + i : i * it.n + j);
+                    float old[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        old[e] = t.muon && i + e < d.r && j < d.k ? (float)to[e * step_i] : 0.0f;
+                    const f32x4 x = fragment(i0) * out;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (i + e < d.r && j < d.k)
+                            to[e * step_i] = (T)(t.muon ? fmaf(-it.scale, x[e], old[e] * t.keep) : x[e]);
+                }
+            }
+        }
+        if (last)
+            return;
+        __syncthreads();
+    }
 }
 
 template <typename T, bool DENSE> __global__ __launch_bounds__(SMALL_THREADS) void k_ns_small(NsTable t)
@@ -1036,23 +1206,26 @@ template <typename T, bool DENSE> __global__ __launch_bounds__(SMALL_THREADS) vo
     const NsItem it = t.it[blockIdx.x];
     const SmallDims d = small_dims(it.m, it.n);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int rect = d.rp * d.kp, square = d.rp * d.rp;
-    _Float16 *xk = (_Float16 *)lds, *xr = xk + 2 * rect, *a = xr + 2 * rect;
+    const int rect = d.rp * d.kp;
+    const SmallSettings c = {t.c * dance::pow2f(-2 * X_EXP) * t.q_mul, t.b * dance::pow2f(-X_EXP) * t.q_mul, t.a * t.q_mul,
+                             1.0f / t.q_mul, t.steps};
+    // (here and not where they are used, each a trip to the kernel's arguments in host memory)
+    asm volatile("" : : "v"(c.ca), "v"(c.ba), "v"(c.one), "v"(c.mul), "s"(c.steps));
 
     // M (Muon: the update) once from memory, its norm on the way, then unscaled into LDS, as fp32 [i][j] where X with k
     // along its rows and A will be
-    float *tile = reinterpret_cast<float *>(xr);
+    float *tile = reinterpret_cast<float *>(lds) + rect;
     const int ld = d.kp + 1;                        // odd; rp (kp + 1) floats are inside xr and A
     const int total = it.m * it.n, step_col = d.tall ? ld : 1, step_row = d.tall ? 1 : ld;
-#pragma unroll 1
-    for (int e = threadIdx.x; e < d.rp * ld; e += SMALL_THREADS)
-        tile[e] = 0.0f;
-    __syncthreads();
+    const float per_row = 1.0f / (float)it.n;
     double acc = 0.0;
-    auto enter = [&](int e, float x) {
-        acc = fma((double)x, (double)x, acc);
-        const int row = (int)((unsigned)e / (unsigned)it.n), col = e - row * it.n;
-        tile[row * step_row + col * step_col] = x;
+    auto padding = [&] {                            // while the first loads are under way
+        if (d.r < d.rp || d.k < d.kp) {
+#pragma unroll 1
+            for (int e = threadIdx.x; e < d.rp * ld; e += SMALL_THREADS)
+                tile[e] = 0.0f;
+            __syncthreads();
+        }
     };
     const int vectors = DENSE ? total / N : 0;
     if (DENSE) {
@@ -1063,28 +1236,39 @@ template <typename T, bool DENSE> __global__ __launch_bounds__(SMALL_THREADS) vo
             if (v < vectors)
                 load_words<T>(t, it, (long long)v * N, g[w], m[w]);
         }
+        padding();
 #pragma unroll
         for (int w = 0; w < WORDS; ++w) {
             const int v = threadIdx.x + w * SMALL_THREADS;
             if (v < vectors) {
                 float x[N];
                 elements<T>(t, g[w], m[w], x);
+                const int row = small_div(v * N, per_row);
+                int col = v * N - row * it.n;
+                float *to = tile + row * step_row + col * step_col;
 #pragma unroll
-                for (int q = 0; q < N; ++q)
-                    enter(v * N + q, x[q]);
+                for (int q = 0; q < N; ++q) {
+                    acc = fma((double)x[q], (double)x[q], acc);
+                    *to = x[q];
+                    const bool end = ++col == it.n;
+                    to += end ? step_row - (it.n - 1) * step_col : step_col;
+                    col = end ? 0 : col;
+                }
                 if (t.muon)
                     reinterpret_cast<Word<T> *>(it.momentum)[v] = m[w];
             }
         }
-    }
+    } else
+        padding();
 #pragma unroll 1
     for (int e = vectors * N + threadIdx.x; e < total; e += SMALL_THREADS) {
         float mom;
-        const int row = (int)((unsigned)e / (unsigned)it.n);
-        const float x = element<T>(t, it, row, e - row * it.n, mom);
+        const int row = small_div(e, per_row), col = e - row * it.n;
+        const float x = element<T>(t, it, row, col, mom);
         if (t.muon)
             ((T *)it.momentum)[e] = (T)mom;
-        enter(e, x);
+        acc = fma((double)x, (double)x, acc);
+        tile[row * step_row + col * step_col] = x;
     }
     acc = wave_sum(acc);
     if (lane == 0)
@@ -1095,126 +1279,12 @@ template <typename T, bool DENSE> __global__ __launch_bounds__(SMALL_THREADS) vo
     for (int w = 1; w < SMALL_WAVES; ++w)
         sum += red[w];
     const Scale scaled = scale_of(sum, t.eps);
-    // X both ways.  The words that replace the tile wait in registers until everybody has read it.
-    constexpr int HELD = (int)(SMALL_MOST / 64 / SMALL_THREADS) + 1;
-    unsigned held[HELD][8];
-#pragma unroll
-    for (int n = 0; n < HELD; ++n) {
-        const int w = threadIdx.x + n * SMALL_THREADS, ib = w / d.kp, j = w - ib * d.kp;
-        if (w < rect / 8)
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-                held[n][q] = split_word(scaled(tile[(ib * 8 + q) * ld + j]));
-    }
-#pragma unroll 1
-    for (int w = threadIdx.x; w < rect / 8; w += SMALL_THREADS) {
-        const int jb = w / d.rp, i = w - jb * d.rp;
-        unsigned x[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-            x[q] = split_word(scaled(tile[i * ld + jb * 8 + q]));
-        put8(xk + w * 8, rect, x);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < HELD; ++n) {
-        const int w = threadIdx.x + n * SMALL_THREADS;
-        if (w < rect / 8)
-            put8(xr + w * 8, rect, held[n]);
-    }
-    __syncthreads();
-
-    const int fr = d.rp / 16, fk = d.kp / 16;
-    const int i4 = 4 * (lane >> 4), j1 = lane & 15;               // a lane's rows and column in a fragment
-    const float ca = t.c * dance::pow2f(-2 * X_EXP) * t.q_mul, ba = t.b * dance::pow2f(-X_EXP) * t.q_mul, one = t.a * t.q_mul;
-    const float mul = 1.0f / t.q_mul;
-    // a fragment of a symmetric matrix at (i0, j0): entered at its mirror image, where a lane's 4 values are neighbours
-    auto put_square = [&](const f32x4 &v, int i0, int j0) {
-        put4(a + (((i0 + i4) >> 3) * d.rp + j0 + j1) * 8 + (i4 & 7), square, split4(v));
-    };
-#pragma unroll 1
-    for (int step = 0; step < t.steps; ++step) {
-#pragma unroll 1
-        for (int f = wave; f < fr * fr; f += SMALL_WAVES) {
-            const int i0 = f / fr * 16, j0 = f % fr * 16;
-            put_square(small_gemm(xk, d.rp, rect, i0, xk, d.rp, rect, j0, d.kp) * dance::pow2f(-X_EXP), i0, j0);
-        }
-        __syncthreads();
-        f32x4 q[SMALL_SQUARE];
-#pragma unroll
-        for (int n = 0; n < SMALL_SQUARE; ++n) {
-            const int f = wave + n * SMALL_WAVES, i0 = f / fr * 16, j0 = f % fr * 16;
-            if (f >= fr * fr)
-                break;
-            q[n] = small_gemm(a, d.rp, square, i0, a, d.rp, square, j0, d.rp);
-            const _Float16 *p = a + (((i0 + i4) >> 3) * d.rp + j0 + j1) * 8 + (i4 & 7);
-            const h4 ah = *reinterpret_cast<const h4 *>(p), al = *reinterpret_cast<const h4 *>(p + square);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                q[n][e] = poly_of(ca, q[n][e], ba, ah[e], al[e]);
-            if (i0 == j0) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    q[n][e] += i4 + e == j1 && j0 + j1 < d.r ? one : 0.0f;
-            }
-        }
-        __syncthreads();                                          // every wave has read A: Q takes its place
-#pragma unroll
-        for (int n = 0; n < SMALL_SQUARE; ++n) {
-            const int f = wave + n * SMALL_WAVES;
-            if (f >= fr * fr)
-                break;
-            put_square(q[n], f / fr * 16, f % fr * 16);
-        }
-        __syncthreads();
-        // X <- Q X: a wave owns 16 columns of X at a time, holds them in registers and replaces them
-#pragma unroll 1
-        for (int f = wave; f < fk; f += SMALL_WAVES) {
-            const int j0 = f * 16, kb = lane >> 4;
-            h8 vh[SMALL_SQUARE], vl[SMALL_SQUARE];                // rp / 32 <= 3 steps of 32 rows
-#pragma unroll
-            for (int n = 0; n < SMALL_SQUARE; ++n)
-                if (n * 32 < d.rp) {
-                    const _Float16 *p = xr + ((n * 4 + kb) * d.kp + j0 + j1) * 8;
-                    vh[n] = *reinterpret_cast<const h8 *>(p);
-                    vl[n] = *reinterpret_cast<const h8 *>(p + rect);
-                }
-#pragma unroll 1
-            for (int i0 = 0; i0 < d.rp; i0 += 16) {
-                f32x4 hh = {0.0f, 0.0f, 0.0f, 0.0f}, hl = hh, lh = hh;
-#pragma unroll
-                for (int n = 0; n < SMALL_SQUARE; ++n)
-                    if (n * 32 < d.rp) {
-                        const _Float16 *p = a + ((n * 4 + kb) * d.rp + i0 + j1) * 8;
-                        const h8 uh = *reinterpret_cast<const h8 *>(p), ul = *reinterpret_cast<const h8 *>(p + square);
-                        lh = __builtin_amdgcn_mfma_f32_16x16x32_f16(ul, vh[n], lh, 0, 0, 0);
-                        hl = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh, vl[n], hl, 0, 0, 0);
-                        hh = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh, vh[n], hh, 0, 0, 0);
-                    }
-                const f32x4 x = (hh + (hl + lh)) * mul;
-                const int i = i0 + i4, j = j0 + j1;
-                if (step + 1 < t.steps) {
-                    Quad y = split4(x);
-                    put4(xr + ((i >> 3) * d.kp + j) * 8 + (i & 7), rect, y);
-                    transpose4(y);                                // 4 columns of row i + lane % 4
-                    put4(xk + ((j >> 3) * d.rp + i + (lane & 3)) * 8 + (j & 4), rect, y);
-                } else {
-                    const int step_i = d.tall ? 1 : it.n;
-                    T *to = (T *)it.dst + (d.tall ? j * it.n + i : i * it.n + j);
-                    const float out = dance::pow2f(-X_EXP);
-                    float old[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        old[e] = t.muon && i + e < d.r && j < d.k ? (float)to[e * step_i] * t.keep : 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (i + e < d.r && j < d.k)
-                            to[e * step_i] = (T)(t.muon ? fmaf(-it.scale, x[e] * out, old[e]) : x[e] * out);
-                }
-            }
-        }
-        __syncthreads();
-    }
+    if (d.rp == 32)
+        small_steps<1, T>(t, it, d, c, scaled, (_Float16 *)lds);
+    else if (d.rp == 64)
+        small_steps<2, T>(t, it, d, c, scaled, (_Float16 *)lds);
+    else
+        small_steps<3, T>(t, it, d, c, scaled, (_Float16 *)lds);
 }
 
 // ------------------------------------------------------------------------------------------- host
