@@ -1151,27 +1151,38 @@ __device__ __forceinline__ void small_steps(const NsTable &t, const NsItem &it, 
                 vh[n] = *reinterpret_cast<const h8 *>(p);
                 vl[n] = *reinterpret_cast<const h8 *>(p + rect);
             }
-            auto fragment = [&](int i0) {
+            // Q's rows of a fragment are read while the one before is multiplied and written
+            h8 uh[2][R], ul[2][R];
+            auto load = [&](int set, int i) {
+#pragma unroll
+                for (int n = 0; n < R; ++n) {
+                    const _Float16 *p = a + word + (n * 4 * RP + i) * 8;
+                    uh[set][n] = *reinterpret_cast<const h8 *>(p);
+                    ul[set][n] = *reinterpret_cast<const h8 *>(p + SQUARE);
+                }
+            };
+            auto fragment = [&](int set) {
                 f32x4 hh = {0.0f, 0.0f, 0.0f, 0.0f}, hl = hh, lh = hh;
 #pragma unroll
                 for (int n = 0; n < R; ++n) {
-                    const _Float16 *p = a + word + (n * 4 * RP + i0) * 8;
-                    const h8 uh = *reinterpret_cast<const h8 *>(p), ul = *reinterpret_cast<const h8 *>(p + SQUARE);
-                    lh = __builtin_amdgcn_mfma_f32_16x16x32_f16(ul, vh[n], lh, 0, 0, 0);
-                    hl = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh, vl[n], hl, 0, 0, 0);
-                    hh = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh, vh[n], hh, 0, 0, 0);
+                    lh = __builtin_amdgcn_mfma_f32_16x16x32_f16(ul[set][n], vh[n], lh, 0, 0, 0);
+                    hl = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[set][n], vl[n], hl, 0, 0, 0);
+                    hh = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[set][n], vh[n], hh, 0, 0, 0);
                 }
                 return (hh + (hl + lh)) * c.mul;
             };
+            load(0, 0);
             if (!last) {
                 _Float16 *to_r = xr + ((i4 >> 3) * d.kp + j) * 8 + (i4 & 7);
                 _Float16 *to_k = xk + ((j >> 3) * RP + i4 + (lane & 3)) * 8 + (j & 4);
 #pragma unroll
-                for (int i = 0; i < RP; i += 16) {
-                    Quad x = split4(fragment(i));
-                    put4(to_r + i * d.kp, rect, x);
+                for (int i = 0; i < FR; ++i) {
+                    if (i + 1 < FR)
+                        load((i + 1) & 1, 16 * (i + 1));
+                    Quad x = split4(fragment(i & 1));
+                    put4(to_r + 16 * i * d.kp, rect, x);
                     transpose4(x);
-                    put4(to_k + i * 8, rect, x);
+                    put4(to_k + 16 * i * 8, rect, x);
                 }
             } else {
                 const int step_i = d.tall ? 1 : it.n;
@@ -1184,7 +1195,8 @@ __device__ __forceinline__ void small_steps(const NsTable &t, const NsItem &it, 
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         old[e] = t.muon && i + e < d.r && j < d.k ? (float)to[e * step_i] : 0.0f;
-                    const f32x4 x = fragment(i0) * out;
+                    load(0, i0);
+                    const f32x4 x = fragment(0) * out;
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         if (i + e < d.r && j < d.k)
