@@ -662,30 +662,37 @@ __global__ __launch_bounds__(SUM_THREADS) void k_ns_sum(const NsTable *__restric
     const int side = narrow(d) ? PAD : t.gram_side, parts = side == PAD ? 4 : 1;
     const int part = local & (parts - 1);
     lower_tile(local / parts, ti, tj);
-    // A unit above the diagonal is the mirror image of the one below it, at either side of the tiles: the two products
-    // differ in their last bits, and a matrix gets the same bits whatever the launch holds besides it
+    // A unit or fragment above the diagonal is the mirror image of the one below it: A is symmetric to the bit at either
+    // side of the tiles, and a matrix gets the same bits whatever the launch holds besides it
     const int i0 = ti * side + (part >> 1) * UNIT, j0 = tj * side + (part & 1) * UNIT;
     if (i0 < j0)
         return;
     const size_t share = (size_t)lower_tiles(d, side) * side * side / 4;
     const f32x4 *in = reinterpret_cast<const f32x4 *>(s.part + (size_t)(local / parts) * side * side) + part * 16 * 64 + threadIdx.x;
-    f32x4 v = in[0];
-    for (int k = 1; k < it.split; k += 8) {
-        f32x4 w[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-            w[u] = in[min(k + u, it.split - 1) * share];
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-            if (k + u < it.split)
-                v += w[u];
-    }
     // fragment f of the unit: 4 x 4 of a wave, or 2 x 2 of each of 4 waves
-    const int f = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int f = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int i = parts == 4 ? f >> 2 : (f >> 3) * 2 + (f >> 1 & 1), j = parts == 4 ? f & 3 : (f >> 2 & 1) * 2 + (f & 1);
+    if (i0 > j0 || i >= j) {
+        f32x4 v = in[0];
+        for (int k = 1; k < it.split; k += 8) {
+            f32x4 w[8];
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-        tile[(16 * i + 4 * (lane >> 4) + q) * LD + 16 * j + (lane & 15)] = split_word(v[q] * dance::pow2f(-X_EXP));
+            for (int u = 0; u < 8; ++u)
+                w[u] = in[min(k + u, it.split - 1) * share];
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (k + u < it.split)
+                    v += w[u];
+        }
+        const int row = 16 * i + 4 * (lane >> 4), col = 16 * j + (lane & 15);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const unsigned word = split_word(v[q] * dance::pow2f(-X_EXP));
+            tile[(row + q) * LD + col] = word;
+            if (i0 == j0 && i > j)
+                tile[col * LD + row + q] = word;
+        }
+    }
     __syncthreads();
     const size_t plane = (size_t)d.rp * d.rp;
     if (threadIdx.x < SUM_THREADS / 2)
@@ -870,11 +877,96 @@ __device__ __forceinline__ void zero(f32x4 (&acc)[4][2])
             acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 }
 
-// a symmetric matrix into a region, each value at its mirror image, where a lane's 4 are neighbours
-__device__ __forceinline__ void narrow_put_square(char *region, const f32x4 (&m)[4][2])
+// Symmetric products U U' of 128 rows: the 36 fragments on and below the diagonal, over 8 waves.  The quarter below the
+// diagonal is four waves' (BLOCK, 2 x 2 fragments each), a quarter on the diagonal two waves': (3, 0) (3, 1) (3, 2)
+// (3, 3) (0, 0) of its own rows (LAST_ROW) and (1, 0) (1, 1) (2, 0) (2, 1) (2, 2) (MIDDLE).  A fragment's rows are the
+// same words as a left and as a right operand, so a wave reads four rows of fragments at most.  Each SIMD has a wave of
+// four and one of five fragments: 1728 clocks of MFMAs where all 64 take 3072.
+enum Triangle { BLOCK, LAST_ROW, MIDDLE };
+
+struct Triangular {
+    int kind, row[4];           // rows of fragments, in units of 16
+};
+
+__device__ __forceinline__ Triangular triangular()
 {
-    narrow_each([&](int i, int j, int row, int col) {
-        put4((_Float16 *)region + ((row >> 3) * PAD + col) * 8 + (row & 7), REGION / 4, split4(m[i][j]));
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = wave & 2;
+    if (wave < 4)
+        return {BLOCK, {4 + half, 5 + half, (wave & 1) * 2, (wave & 1) * 2 + 1}};
+    const int q = half * 2;
+    return {wave & 1 ? MIDDLE : LAST_ROW, {q, q + 1, q + 2, q + 3}};
+}
+
+// f(s, i, j) for the wave's fragments: s their place in a wave's five, (i, j) two of its four rows
+template <int KIND, typename F> __device__ __forceinline__ void triangular_of(F &&f)
+{
+    if (KIND == BLOCK) {
+        f(0, 0, 2);
+        f(1, 0, 3);
+        f(2, 1, 2);
+        f(3, 1, 3);
+    } else if (KIND == LAST_ROW) {
+        f(0, 3, 0);
+        f(1, 3, 1);
+        f(2, 3, 2);
+        f(3, 3, 3);
+        f(4, 0, 0);
+    } else {
+        f(0, 1, 0);
+        f(1, 1, 1);
+        f(2, 2, 0);
+        f(3, 2, 1);
+        f(4, 2, 2);
+    }
+}
+
+template <typename F> __device__ __forceinline__ void with_kind(const Triangular &t, F &&f)
+{
+    if (t.kind == BLOCK)
+        f(std::integral_constant<int, BLOCK>{});
+    else if (t.kind == LAST_ROW)
+        f(std::integral_constant<int, LAST_ROW>{});
+    else
+        f(std::integral_constant<int, MIDDLE>{});
+}
+
+// acc += the wave's fragments of U U', 128 k
+template <int KIND> __device__ __forceinline__ void triangular_gemm(f32x4 (&acc)[5], const Triangular &t, const char *u)
+{
+    const int lane = threadIdx.x & 63;
+    const char *at = u + ((lane >> 4) * PAD + (lane & 15)) * 16;
+#pragma unroll 1
+    for (int s = 0; s < PAD / 32; ++s) {
+        h8 h[4], l[4];
+#pragma unroll
+        for (int i = 0; i < (KIND == MIDDLE ? 3 : 4); ++i) {
+            h[i] = *reinterpret_cast<const h8 *>(at + t.row[i] * 256);
+            l[i] = *reinterpret_cast<const h8 *>(at + t.row[i] * 256 + REGION / 2);
+        }
+        triangular_of<KIND>([&](int f, int i, int j) { acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[i], h[j], acc[f], 0, 0, 0); });
+        triangular_of<KIND>([&](int f, int i, int j) { acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h[i], l[j], acc[f], 0, 0, 0); });
+        triangular_of<KIND>([&](int f, int i, int j) { acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h[i], h[j], acc[f], 0, 0, 0); });
+        at += 4 * PAD * 16;
+    }
+}
+
+__device__ __forceinline__ void triangular_gemm(f32x4 (&acc)[5], const Triangular &t, const char *u)
+{
+    with_kind(t, [&](auto kind) { triangular_gemm<decltype(kind)::value>(acc, t, u); });
+}
+
+// a symmetric matrix into a region: each value at its mirror image, where a lane's 4 are neighbours, and in its place
+template <int KIND> __device__ __forceinline__ void put_triangular(char *region, const Triangular &t, const f32x4 (&m)[5])
+{
+    const int row = 4 * ((threadIdx.x & 63) >> 4), col = threadIdx.x & 15;
+    triangular_of<KIND>([&](int f, int i, int j) {
+        const int i0 = 16 * t.row[i], j0 = 16 * t.row[j];
+        Quad x = split4(m[f]);
+        put4((_Float16 *)region + (((i0 + row) >> 3) * PAD + j0 + col) * 8 + (row & 7), REGION / 4, x);
+        if (KIND == BLOCK || i != j) {
+            transpose4(x);                                    // 4 columns of row row + lane % 4
+            put4((_Float16 *)region + (((j0 + col) >> 3) * PAD + i0 + row + (threadIdx.x & 3)) * 8 + (col & 4), REGION / 4, x);
+        }
     });
 }
 
@@ -902,45 +994,51 @@ template <typename T> __global__ __launch_bounds__(NARROW_THREADS) void k_ns_nar
     ns_space(it.ws, d, it.split, s);
     const size_t rect = (size_t)PAD * d.kp, share = PAD * PAD;
     const int tiles = d.kp / PAD, last = step + 1 == t.steps;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    f32x4 next[4][2];
-    zero(next);
+    const Triangular mine = triangular();
+    f32x4 next[5];
+#pragma unroll
+    for (int f = 0; f < 5; ++f)
+        next[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     if (step < 0) {
         for (int c = local; c < tiles; c += it.split) {
             narrow_stage(s.xk[0] + (size_t)c * (PAD / 8) * PAD * 8, rect, PAD, columns);
             gemm_wait();
-            narrow_gemm(next, columns, columns);
+            triangular_gemm(next, mine, columns);
             __syncthreads();
         }
     } else {
-        narrow_stage(s.xr[0] + (size_t)local * PAD * 8, rect, d.kp, columns);
         narrow_stage(s.a, share, PAD, square);
-        gemm_wait();
-        f32x4 v[4][2];
-        zero(v);
-        narrow_gemm(v, square, square);
+        narrow_stage(s.xr[0] + (size_t)local * PAD * 8, rect, d.kp, columns);
+        gemm_wait<8>();                                       // A; the columns are on their way
+        f32x4 q[5];
+#pragma unroll
+        for (int f = 0; f < 5; ++f)
+            q[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        triangular_gemm(q, mine, square);
         const float ca = t.c * dance::pow2f(-2 * X_EXP) * t.q_mul, ba = t.b * dance::pow2f(-X_EXP) * t.q_mul, one = t.a * t.q_mul;
-        narrow_each([&](int i, int j, int row, int col) {
-            // A is symmetric: 4 rows of a column are 4 neighbours of that column's row
-            const _Float16 *p = (const _Float16 *)square + ((row >> 3) * PAD + col) * 8 + (row & 7);
-            const h4 hi = *reinterpret_cast<const h4 *>(p), lo = *reinterpret_cast<const h4 *>(p + REGION / 4);
+        with_kind(mine, [&](auto kind) {
+            constexpr int KIND = decltype(kind)::value;
+            const int row = 4 * ((threadIdx.x & 63) >> 4), col = threadIdx.x & 15;
+            triangular_of<KIND>([&](int f, int i, int j) {
+                const int i0 = 16 * mine.row[i], j0 = 16 * mine.row[j];
+                // A is symmetric: 4 rows of a column are 4 neighbours of that column's row
+                const _Float16 *p = (const _Float16 *)square + (((i0 + row) >> 3) * PAD + j0 + col) * 8 + (row & 7);
+                const h4 hi = *reinterpret_cast<const h4 *>(p), lo = *reinterpret_cast<const h4 *>(p + REGION / 4);
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                v[i][j][q] = poly_of(ca, v[i][j][q], ba, hi[q], lo[q]);
-            if (wave / 4 * 4 + i == (wave & 3) * 2 + j) {         // (a fragment of the diagonal, in every lane)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    v[i][j][q] += row + q == col && col < d.r ? one : 0.0f;
-            }
+                for (int e = 0; e < 4; ++e) {
+                    q[f][e] = poly_of(ca, q[f][e], ba, hi[e], lo[e]);
+                    if (KIND != BLOCK && i == j)
+                        q[f][e] += row + e == col && j0 + col < d.r ? one : 0.0f;
+                }
+            });
         });
-        f32x4 q[4][2];
-        narrow_each([&](int i, int j, int, int) { q[i][j] = v[i][j]; });
+        f32x4 v[4][2];
         const float mul = 1.0f / t.q_mul;
 #pragma unroll 1
         for (int c = local; c < tiles; c += it.split) {
-            __syncthreads();                                  // A, and the columns before, have been read
+            gemm_wait();                                      // A, and the columns before, have been read; the first are here
             if (c == local || last)
-                narrow_put_square(square, q);
+                with_kind(mine, [&](auto kind) { put_triangular<decltype(kind)::value>(square, mine, q); });
             __syncthreads();
             if (c != local) {
                 narrow_stage(s.xr[0] + (size_t)c * PAD * 8, rect, d.kp, columns);
@@ -959,7 +1057,7 @@ template <typename T> __global__ __launch_bounds__(NARROW_THREADS) void k_ns_nar
                     put4((_Float16 *)columns + ((col >> 3) * PAD + row + (threadIdx.x & 3)) * 8 + (col & 4), REGION / 4, x);
                 });
                 __syncthreads();
-                narrow_gemm(next, columns, columns);
+                triangular_gemm(next, mine, columns);
             } else {
                 // the tile in fp32 over both regions; Q is needed again if there are more columns
                 float *tile = reinterpret_cast<float *>(lds);
@@ -976,9 +1074,13 @@ template <typename T> __global__ __launch_bounds__(NARROW_THREADS) void k_ns_nar
     if (last)
         return;
     // where k_ns_sum looks for them: quarter by quarter of the tile, 4 x 4 fragments each
-    const int quarter = (wave >> 2) * 2 + (wave >> 1 & 1);
-    f32x4 *out = reinterpret_cast<f32x4 *>(s.part + local * share) + (quarter * 16 + (wave & 1) * 2) * 64 + (threadIdx.x & 63);
-    narrow_each([&](int i, int j, int, int) { out[(i * 4 + j) * 64] = next[i][j]; });
+    f32x4 *out = reinterpret_cast<f32x4 *>(s.part + local * share) + (threadIdx.x & 63);
+    with_kind(mine, [&](auto kind) {
+        triangular_of<decltype(kind)::value>([&](int f, int i, int j) {
+            const int fi = mine.row[i], fj = mine.row[j];
+            out[(((fi >> 2) * 2 + (fj >> 2)) * 16 + (fi & 3) * 4 + (fj & 3)) * 64] = next[f];
+        });
+    });
 }
 
 // ------------------------------------------------------------------------------- small matrices
@@ -1162,14 +1264,16 @@ __device__ __forceinline__ void small_steps(const NsTable &t, const NsItem &it, 
                 }
             };
             auto fragment = [&](int set) {
-                f32x4 hh = {0.0f, 0.0f, 0.0f, 0.0f}, hl = hh, lh = hh;
+                f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int n = 0; n < R; ++n) {
-                    lh = __builtin_amdgcn_mfma_f32_16x16x32_f16(ul[set][n], vh[n], lh, 0, 0, 0);
-                    hl = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[set][n], vl[n], hl, 0, 0, 0);
-                    hh = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[set][n], vh[n], hh, 0, 0, 0);
+                    x = __builtin_amdgcn_mfma_f32_16x16x32_f16(ul[set][n], vh[n], x, 0, 0, 0);
+                    x = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[set][n], vl[n], x, 0, 0, 0);
                 }
-                return (hh + (hl + lh)) * c.mul;
+#pragma unroll
+                for (int n = 0; n < R; ++n)
+                    x = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[set][n], vh[n], x, 0, 0, 0);
+                return x * c.mul;
             };
             load(0, 0);
             if (!last) {
