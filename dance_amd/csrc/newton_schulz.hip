@@ -92,7 +92,7 @@ struct NsSpace {
     double *sums;               // NS_SLICES partial sums of squares
     float *part;                // [split][lower tile][side * side]: a tile of A summed over a share of k
     _Float16 *a, *q;            // [2][rp / 8][rp][8]
-    _Float16 *xk[2], *xr[2];    // [2][kp / 8][rp][8], [2][rp / 8][kp][8]: this step's and the next one's
+    _Float16 *xk[2], *xr[2];    // [2][kp / 8][rp][8], [2][rp / 8][kp][8]: this step's and the next one's (narrow: xr[0] alone)
 };
 
 __host__ __device__ inline size_t ns_space(char *ws, const NsDims &d, int split, NsSpace &s)
@@ -109,7 +109,7 @@ __host__ __device__ inline size_t ns_space(char *ws, const NsDims &d, int split,
     at += narrow(d) ? 0 : square;
     for (int i = 0; i < (narrow(d) ? 1 : 2); ++i) {
         s.xk[i] = (_Float16 *)(ws + at);
-        at += rect;
+        at += narrow(d) ? 0 : rect;
         s.xr[i] = (_Float16 *)(ws + at);
         at += rect;
     }
@@ -400,59 +400,85 @@ __device__ __forceinline__ Scale scale_of(double sum, double eps)
     return Scale{X_EXP - e, 1.0f / (float)m};
 }
 
-// M / norm -> the first X, a tile of 64 x 64 a workgroup; Muon: the momentum is stored on the way
-template <typename T, bool DENSE> __global__ __launch_bounds__(256) void k_ns_pack(const NsTable *__restrict__ tp)
+// 1 / norm of an item, by all lanes of a wave
+__device__ __forceinline__ Scale item_scale(const NsTable &t, const NsSpace &s, int n_item)
 {
-    const NsTable &t = *tp;
-    constexpr int N = 16 / sizeof(T), LD = PACK + 1;
-    __shared__ unsigned tile[PACK * LD];
-    int n_item, local;
-    const NsItem it = find_item(t, t.pack, blockIdx.x, n_item, local);
-    const NsDims d = ns_dims(it.m, it.n);
-    NsSpace s;
-    ns_space(it.ws, d, it.split, s);
-    const int across = d.kp / PACK, i0 = local / across * PACK, j0 = local % across * PACK;
     const int slices = t.slices[n_item] - (n_item ? t.slices[n_item - 1] : 0);
     double sum = 0.0;
     for (int i = threadIdx.x & 63; i < slices; i += 64)
         sum += s.sums[i];
-    const Scale scaled = scale_of(wave_sum(sum), t.eps);
-    // N neighbours of a row of M at once: along j, or along i where M is tall
-    const int row0 = d.tall ? j0 : i0, col0 = d.tall ? i0 : j0;
+    return scale_of(wave_sum(sum), t.eps);
+}
+
+// A square tile of M / norm, rows i and columns j of X from (i0, j0) on, as split words in LDS, row stride SIDE + 1;
+// Muon: the momentum is stored on the way.  N neighbours of a row of M at once: along j, or along i where M is tall.
+template <typename T, bool DENSE, int SIDE, int THREADS>
+__device__ __forceinline__ void first_tile(const NsTable &t, const NsItem &it, const NsDims &d, Scale scaled, int i0, int j0,
+                                           unsigned *tile)
+{
+    constexpr int N = DENSE ? 16 / sizeof(T) : 1, ACROSS = SIDE / N, DOWN = THREADS / ACROSS, WORDS = SIDE / DOWN, LD = SIDE + 1;
+    constexpr int FLY = DENSE ? WORDS : WORDS < 8 ? WORDS : 8;               // loads under way
     const int step_j = d.tall ? LD : 1, step_i = d.tall ? 1 : LD;           // of a row and a column of M in the tile
-    if (DENSE && row0 + PACK <= it.m && col0 + PACK <= it.n) {
-        constexpr int WORDS = PACK * PACK / N / 256;
-        Word<T> g[WORDS], m[WORDS];
-        const int rr = threadIdx.x / (PACK / N), cc = threadIdx.x % (PACK / N) * N;
-        const long long e = (long long)(row0 + rr) * it.n + col0 + cc, down = 256 / (PACK / N) * (long long)it.n;
+    const int rr = threadIdx.x / ACROSS, cc = threadIdx.x % ACROSS * N;
+    const int row0 = (d.tall ? j0 : i0) + rr, col = (d.tall ? i0 : j0) + cc;
+    unsigned *to = tile + rr * step_i + cc * step_j;
+#pragma unroll 1
+    for (int first = 0; first < WORDS; first += FLY) {
+        float x[FLY][16 / sizeof(T)] = {};
+        if constexpr (DENSE) {
+            const long long e = (long long)row0 * it.n + col, down = (long long)DOWN * it.n;
+            Word<T> g[FLY], m[FLY];
 #pragma unroll
-        for (int w = 0; w < WORDS; ++w)
-            load_words<T>(t, it, e + w * down, g[w], m[w]);
+            for (int w = 0; w < FLY; ++w)
+                if (row0 + w * DOWN < it.m && col + N <= it.n)
+                    load_words<T>(t, it, e + w * down, g[w], m[w]);
 #pragma unroll
-        for (int w = 0; w < WORDS; ++w) {
-            float x[N];
-            elements<T>(t, g[w], m[w], x);
-            if (t.muon)
-                *reinterpret_cast<Word<T> *>((T *)it.momentum + e + w * down) = m[w];
+            for (int w = 0; w < FLY; ++w) {
+                if (row0 + w * DOWN < it.m && col + N <= it.n) {
+                    elements<T>(t, g[w], m[w], x[w]);
+                    if (t.muon)
+                        *reinterpret_cast<Word<T> *>((T *)it.momentum + e + w * down) = m[w];
+                } else if (row0 + w * DOWN < it.m && col < it.n) {           // a row's last ones
+#pragma unroll
+                    for (int q = 0; q < N - 1; ++q)
+                        if (col + q < it.n) {
+                            float mom;
+                            x[w][q] = element<T>(t, it, row0 + w * DOWN, col + q, mom);
+                            if (t.muon)
+                                ((T *)it.momentum)[e + w * down + q] = (T)mom;
+                        }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int w = 0; w < FLY; ++w) {                                  // (strides are orthogonalize's alone)
+                float mom;
+                const int row = row0 + (first + w) * DOWN;
+                if (row < it.m && col < it.n)
+                    x[w][0] = element<T>(t, it, row, col, mom);
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < FLY; ++w)
 #pragma unroll
             for (int q = 0; q < N; ++q)
-                tile[(rr + w * (256 / (PACK / N))) * step_i + (cc + q) * step_j] = split_word(scaled(x[q]));
-        }
-    } else {
-#pragma unroll 4
-        for (int n = 0; n < PACK * PACK / 256; ++n) {
-            const int rr = threadIdx.x / PACK + n * (256 / PACK), cc = threadIdx.x % PACK, row = row0 + rr, col = col0 + cc;
-            float x = 0.0f;
-            if (row < it.m && col < it.n) {
-                float mom;
-                x = element<T>(t, it, row, col, mom);
-                if (t.muon)
-                    ((T *)it.momentum)[(long long)row * it.n + col] = (T)mom;
-            }
-            tile[rr * step_i + cc * step_j] = split_word(scaled(x));
-        }
+                to[(first + w) * DOWN * step_i + q * step_j] = split_word(scaled(x[w][q]));
     }
     __syncthreads();
+}
+
+// M / norm -> the first X, a tile of 64 x 64 a workgroup
+template <typename T, bool DENSE> __global__ __launch_bounds__(256) void k_ns_pack(const NsTable *__restrict__ tp)
+{
+    const NsTable &t = *tp;
+    __shared__ unsigned tile[PACK * (PACK + 1)];
+    int index, local;
+    const NsItem it = find_item(t, t.pack, blockIdx.x, index, local);
+    const NsDims d = ns_dims(it.m, it.n);
+    NsSpace s;
+    ns_space(it.ws, d, it.split, s);
+    const int across = d.kp / PACK, i0 = local / across * PACK, j0 = local % across * PACK;
+    first_tile<T, DENSE, PACK, 256>(t, it, d, item_scale(t, s, index), i0, j0, tile);
     const size_t plane = (size_t)d.rp * d.kp;
     put_rows<PACK, PACK, 256>(s.xk[0], plane, d.rp, i0, j0, tile);
     put_cols<PACK, PACK, 256>(s.xr[0], plane, d.kp, i0, j0, tile);
@@ -981,8 +1007,55 @@ __device__ __forceinline__ void narrow_stage(const _Float16 *p, size_t plane, in
         copy_words(src + ((size_t)(c >> 1) * rows + (c & 1) * 64) * 8, to + ((c >> 1) * PAD + (c & 1) * 64) * 16);
 }
 
-// step -1: only the first A.  The last step writes the result, and no A.
-template <typename T> __global__ __launch_bounds__(NARROW_THREADS) void k_ns_narrow(const NsTable *__restrict__ tp, int step)
+// a share of A, where k_ns_sum looks for it: quarter by quarter of the tile, 4 x 4 fragments each
+__device__ __forceinline__ void put_share(float *part, const Triangular &t, const f32x4 (&v)[5])
+{
+    f32x4 *out = reinterpret_cast<f32x4 *>(part) + (threadIdx.x & 63);
+    with_kind(t, [&](auto kind) {
+        triangular_of<decltype(kind)::value>([&](int f, int i, int j) {
+            const int fi = t.row[i], fj = t.row[j];
+            out[(((fi >> 2) * 2 + (fj >> 2)) * 16 + (fi & 3) * 4 + (fj & 3)) * 64] = v[f];
+        });
+    });
+}
+
+__device__ __forceinline__ void zero(f32x4 (&acc)[5])
+{
+#pragma unroll
+    for (int f = 0; f < 5; ++f)
+        acc[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+}
+
+// M / norm -> the first X and the shares of its A
+constexpr int FIRST_TILE = PAD * (PAD + 1) * 4, FIRST_LDS = FIRST_TILE + REGION;
+template <typename T, bool DENSE> __global__ __launch_bounds__(NARROW_THREADS) void k_ns_narrow_first(const NsTable *__restrict__ tp)
+{
+    const NsTable &t = *tp;
+    extern __shared__ __align__(16) char lds[];
+    unsigned *tile = reinterpret_cast<unsigned *>(lds);
+    char *columns = lds + FIRST_TILE;
+    int index, local;
+    const NsItem it = find_item(t, t.narrow, die_order(), index, local);
+    const NsDims d = ns_dims(it.m, it.n);
+    NsSpace s;
+    ns_space(it.ws, d, it.split, s);
+    const Scale scaled = item_scale(t, s, index);
+    const Triangular mine = triangular();
+    f32x4 next[5];
+    zero(next);
+#pragma unroll 1
+    for (int c = local; c < d.kp / PAD; c += it.split) {
+        first_tile<T, DENSE, PAD, NARROW_THREADS>(t, it, d, scaled, 0, c * PAD, tile);
+        put_rows<PAD, PAD, NARROW_THREADS>((_Float16 *)columns, REGION / 4, PAD, 0, 0, tile);
+        put_cols<PAD, PAD, NARROW_THREADS>(s.xr[0], (size_t)PAD * d.kp, d.kp, 0, c * PAD, tile);
+        __syncthreads();
+        triangular_gemm(next, mine, columns);
+    }
+    put_share(s.part + (size_t)local * PAD * PAD, mine, next);
+}
+
+// A step; the last one writes the result, and no A
+template <typename T> __global__ __launch_bounds__(NARROW_THREADS) void k_ns_narrow(const NsTable *__restrict__ tp, int last)
 {
     const NsTable &t = *tp;
     extern __shared__ __align__(16) char lds[];
@@ -993,94 +1066,71 @@ template <typename T> __global__ __launch_bounds__(NARROW_THREADS) void k_ns_nar
     NsSpace s;
     ns_space(it.ws, d, it.split, s);
     const size_t rect = (size_t)PAD * d.kp, share = PAD * PAD;
-    const int tiles = d.kp / PAD, last = step + 1 == t.steps;
+    const int tiles = d.kp / PAD;
     const Triangular mine = triangular();
-    f32x4 next[5];
-#pragma unroll
-    for (int f = 0; f < 5; ++f)
-        next[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (step < 0) {
-        for (int c = local; c < tiles; c += it.split) {
-            narrow_stage(s.xk[0] + (size_t)c * (PAD / 8) * PAD * 8, rect, PAD, columns);
-            gemm_wait();
-            triangular_gemm(next, mine, columns);
-            __syncthreads();
-        }
-    } else {
-        narrow_stage(s.a, share, PAD, square);
-        narrow_stage(s.xr[0] + (size_t)local * PAD * 8, rect, d.kp, columns);
-        gemm_wait<8>();                                       // A; the columns are on their way
-        f32x4 q[5];
-#pragma unroll
-        for (int f = 0; f < 5; ++f)
-            q[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        triangular_gemm(q, mine, square);
-        const float ca = t.c * dance::pow2f(-2 * X_EXP) * t.q_mul, ba = t.b * dance::pow2f(-X_EXP) * t.q_mul, one = t.a * t.q_mul;
-        with_kind(mine, [&](auto kind) {
-            constexpr int KIND = decltype(kind)::value;
-            const int row = 4 * ((threadIdx.x & 63) >> 4), col = threadIdx.x & 15;
-            triangular_of<KIND>([&](int f, int i, int j) {
-                const int i0 = 16 * mine.row[i], j0 = 16 * mine.row[j];
-                // A is symmetric: 4 rows of a column are 4 neighbours of that column's row
-                const _Float16 *p = (const _Float16 *)square + (((i0 + row) >> 3) * PAD + j0 + col) * 8 + (row & 7);
-                const h4 hi = *reinterpret_cast<const h4 *>(p), lo = *reinterpret_cast<const h4 *>(p + REGION / 4);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    q[f][e] = poly_of(ca, q[f][e], ba, hi[e], lo[e]);
-                    if (KIND != BLOCK && i == j)
-                        q[f][e] += row + e == col && j0 + col < d.r ? one : 0.0f;
-                }
-            });
-        });
-        f32x4 v[4][2];
-        const float mul = 1.0f / t.q_mul;
-#pragma unroll 1
-        for (int c = local; c < tiles; c += it.split) {
-            gemm_wait();                                      // A, and the columns before, have been read; the first are here
-            if (c == local || last)
-                with_kind(mine, [&](auto kind) { put_triangular<decltype(kind)::value>(square, mine, q); });
-            __syncthreads();
-            if (c != local) {
-                narrow_stage(s.xr[0] + (size_t)c * PAD * 8, rect, d.kp, columns);
-                gemm_wait();
-            }
-            zero(v);
-            narrow_gemm(v, square, columns);
-            __syncthreads();
-            if (!last) {
-                // in place, and with k along the columns for the share of A
-                _Float16 *to = s.xr[0] + (size_t)c * PAD * 8;
-                narrow_each([&](int i, int j, int row, int col) {
-                    Quad x = split4(v[i][j] * mul);
-                    put4(to + ((size_t)(row >> 3) * d.kp + col) * 8 + (row & 7), rect, x);
-                    transpose4(x);                            // 4 columns of row row + lane % 4
-                    put4((_Float16 *)columns + ((col >> 3) * PAD + row + (threadIdx.x & 3)) * 8 + (col & 4), REGION / 4, x);
-                });
-                __syncthreads();
-                triangular_gemm(next, mine, columns);
-            } else {
-                // the tile in fp32 over both regions; Q is needed again if there are more columns
-                float *tile = reinterpret_cast<float *>(lds);
-                narrow_each([&](int i, int j, int row, int col) {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        tile[(row + q) * (PAD + 1) + col] = v[i][j][q] * (mul * dance::pow2f(-X_EXP));
-                });
-                __syncthreads();
-                put_result<T, PAD, NARROW_THREADS>(t, it, d, 0, c * PAD, tile);
-            }
-        }
-    }
-    if (last)
-        return;
-    // where k_ns_sum looks for them: quarter by quarter of the tile, 4 x 4 fragments each
-    f32x4 *out = reinterpret_cast<f32x4 *>(s.part + local * share) + (threadIdx.x & 63);
+    f32x4 next[5], q[5], v[4][2];
+    zero(next);
+    zero(q);
+    narrow_stage(s.a, share, PAD, square);
+    narrow_stage(s.xr[0] + (size_t)local * PAD * 8, rect, d.kp, columns);
+    gemm_wait<8>();                                       // A; the columns are on their way
+    triangular_gemm(q, mine, square);
+    const float ca = t.c * dance::pow2f(-2 * X_EXP) * t.q_mul, ba = t.b * dance::pow2f(-X_EXP) * t.q_mul, one = t.a * t.q_mul;
     with_kind(mine, [&](auto kind) {
-        triangular_of<decltype(kind)::value>([&](int f, int i, int j) {
-            const int fi = mine.row[i], fj = mine.row[j];
-            out[(((fi >> 2) * 2 + (fj >> 2)) * 16 + (fi & 3) * 4 + (fj & 3)) * 64] = next[f];
+        constexpr int KIND = decltype(kind)::value;
+        const int row = 4 * ((threadIdx.x & 63) >> 4), col = threadIdx.x & 15;
+        triangular_of<KIND>([&](int f, int i, int j) {
+            const int i0 = 16 * mine.row[i], j0 = 16 * mine.row[j];
+            // A is symmetric: 4 rows of a column are 4 neighbours of that column's row
+            const _Float16 *p = (const _Float16 *)square + (((i0 + row) >> 3) * PAD + j0 + col) * 8 + (row & 7);
+            const h4 hi = *reinterpret_cast<const h4 *>(p), lo = *reinterpret_cast<const h4 *>(p + REGION / 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                q[f][e] = poly_of(ca, q[f][e], ba, hi[e], lo[e]);
+                if (KIND != BLOCK && i == j)
+                    q[f][e] += row + e == col && j0 + col < d.r ? one : 0.0f;
+            }
         });
     });
+    const float mul = 1.0f / t.q_mul;
+#pragma unroll 1
+    for (int c = local; c < tiles; c += it.split) {
+        gemm_wait();                                      // A, and the columns before, have been read; the first are here
+        if (c == local || last)
+            with_kind(mine, [&](auto kind) { put_triangular<decltype(kind)::value>(square, mine, q); });
+        __syncthreads();
+        if (c != local) {
+            narrow_stage(s.xr[0] + (size_t)c * PAD * 8, rect, d.kp, columns);
+            gemm_wait();
+        }
+        zero(v);
+        narrow_gemm(v, square, columns);
+        __syncthreads();
+        if (!last) {
+            // in place, and with k along the columns for the share of A
+            _Float16 *to = s.xr[0] + (size_t)c * PAD * 8;
+            narrow_each([&](int i, int j, int row, int col) {
+                Quad x = split4(v[i][j] * mul);
+                put4(to + ((size_t)(row >> 3) * d.kp + col) * 8 + (row & 7), rect, x);
+                transpose4(x);                            // 4 columns of row row + lane % 4
+                put4((_Float16 *)columns + ((col >> 3) * PAD + row + (threadIdx.x & 3)) * 8 + (col & 4), REGION / 4, x);
+            });
+            __syncthreads();
+            triangular_gemm(next, mine, columns);
+        } else {
+            // the tile in fp32 over both regions; Q is needed again if there are more columns
+            float *tile = reinterpret_cast<float *>(lds);
+            narrow_each([&](int i, int j, int row, int col) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    tile[(row + q) * (PAD + 1) + col] = v[i][j][q] * (mul * dance::pow2f(-X_EXP));
+            });
+            __syncthreads();
+            put_result<T, PAD, NARROW_THREADS>(t, it, d, 0, c * PAD, tile);
+        }
+    }
+    if (!last)
+        put_share(s.part + local * share, mine, next);
 }
 
 // ------------------------------------------------------------------------------- small matrices
@@ -1521,11 +1571,11 @@ struct Chain {
             const NsDims d = ns_dims(t.it[i].m, t.it[i].n);
             const long long want = ((long long)t.it[i].m * t.it[i].n + 8191) / 8192;
             slices += want < NS_SLICES ? want : NS_SLICES;
-            pack += (long long)(d.rp / PACK) * (d.kp / PACK);
             if (narrow(d)) {
                 narrows += t.it[i].split;
                 sum += 4;
             } else {
+                pack += (long long)(d.rp / PACK) * (d.kp / PACK);
                 gram += (long long)lower_tiles(d, t.gram_side) * t.it[i].split;
                 sum += (long long)lower_tiles(d, t.gram_side) * (t.gram_side == PAD ? 4 : 1);
                 poly += lower_tiles(d, poly_side);
@@ -1544,11 +1594,11 @@ struct Chain {
         return with_type([&](auto type, auto is_dense) {
             using T = decltype(type);
             constexpr bool D = decltype(is_dense)::value;
-            if (int e = dance::allow_lds((const void *)k_ns_narrow<T>, NARROW_LDS, fn))
-                return e;
             hipLaunchKernelGGL((k_ns_norm<T, D>), dim3((unsigned)slices), dim3(256), 0, st, t, kept);
             if (int e = launched())
                 return e;
+            if (pack == 0)
+                return 0;
             hipLaunchKernelGGL((k_ns_pack<T, D>), dim3((unsigned)pack), dim3(256), 0, st, (const NsTable *)kept);
             return launched();
         });
@@ -1576,9 +1626,18 @@ struct Chain {
         if (done)
             return 0;
         if (narrows > 0) {
-            e = with_type([&](auto type, auto) {
-                hipLaunchKernelGGL(k_ns_narrow<decltype(type)>, dim3((unsigned)narrows), dim3(NARROW_THREADS), NARROW_LDS, st,
-                                   (const NsTable *)kept, s);
+            e = with_type([&](auto type, auto is_dense) {
+                using T = decltype(type);
+                constexpr bool D = decltype(is_dense)::value;
+                const dim3 grid((unsigned)narrows), block(NARROW_THREADS);
+                const NsTable *table = kept;
+                if (int r = s < 0 ? dance::allow_lds((const void *)k_ns_narrow_first<T, D>, FIRST_LDS, fn)
+                                  : dance::allow_lds((const void *)k_ns_narrow<T>, NARROW_LDS, fn))
+                    return r;
+                if (s < 0)
+                    hipLaunchKernelGGL((k_ns_narrow_first<T, D>), grid, block, FIRST_LDS, st, table);
+                else
+                    hipLaunchKernelGGL(k_ns_narrow<T>, grid, block, NARROW_LDS, st, table, last);
                 return launched();
             });
         }
