@@ -487,20 +487,24 @@ template <typename T, bool DENSE> __global__ __launch_bounds__(256) void k_ns_pa
 // ------------------------------------------------------------------------------------------- GEMM
 // A square tile of side S = 32 F by 4 waves of F x F fragments of 16 x 16, three products each, k in steps of 32.  A
 // step's operands, S rows of each side, are copied from L2 to LDS without passing registers (global_load_lds_dwordx4),
-// DEPTH - 1 steps ahead.
-//   F = 4 (128): per step and wave 48 MFMAs (768 clocks) stand against 16 KB read from LDS (512 clocks for all four
-//     waves); two buffers, so that two workgroups share a compute unit and one multiplies while the other waits: 820
-//     clocks a step.
-//   F = 2 (64): 192 against 256 clocks, so less of the chip's rate, but four times the workgroups: for launches whose
-//     128-tiles would not give every compute unit one, where a step of those lasts 1550 clocks.  Four buffers: alone on
-//     its compute unit a workgroup has to cover the copies' latency itself.
+// into DEPTH buffers, DEPTH - 1 steps ahead.
+//   F = 4 (128): per step and wave 48 MFMAs (768 clocks) stand against 16 KB read from LDS (about 300 clocks for all four
+//     waves, at the 210 bytes a clock measured); two buffers, so that two workgroups share a compute unit and one
+//     multiplies while the other waits: 820 clocks a step.
+//   F = 2 (64): 192 against 150 clocks, but twice the copies a product and four times the workgroups: for launches whose
+//     128-tiles would not give every compute unit one, where a step of those lasts 1550 clocks.  Up to two workgroups a
+//     compute unit have four buffers and cover the copies' latency themselves, more of them two buffers, so that five
+//     share a compute unit.  us with four / two: 272 tiles of 32 steps 19.7 / 21.1, 450 of 9 8.5 / 8.8, 720 of 8 14.4 / 13.0.
 constexpr int STEP = 32;
 template <int F> struct Tile {
-    static constexpr int SIDE = 32 * F, LD = SIDE + 1, DEPTH = F == 2 ? 4 : 2;
+    static constexpr int SIDE = 32 * F, LD = SIDE + 1;
     static constexpr int SIDE_BYTES = 2 * (STEP / 8) * SIDE * 16;        // [plane][k block][row] words of 16 bytes
     static constexpr int BUFFER = 2 * SIDE_BYTES, COPIES = STEP / 8 * F / 2;      // COPIES: of a wave and step
-    static constexpr int LDS = DEPTH * BUFFER > SIDE * LD * 4 ? DEPTH * BUFFER : SIDE * LD * 4;       // then the tile in 32 bits
 };
+// the buffers, then the tile in 32 bits
+template <int F, int DEPTH>
+constexpr int TILE_LDS = DEPTH * Tile<F>::BUFFER > Tile<F>::SIDE * Tile<F>::LD * 4 ? DEPTH * Tile<F>::BUFFER
+                                                                                   : Tile<F>::SIDE * Tile<F>::LD * 4;
 constexpr int GEMM_THREADS = 256;
 
 struct Side {
@@ -555,9 +559,9 @@ __device__ __forceinline__ unsigned lds_address(const void *p)
 }
 
 // acc = U V' over `steps` steps; same: both sides are the same rows, copied once.  lds: the kernel's dynamic LDS,
-// Tile<F>::LDS bytes; free again at return.  acc[i][j]: rows 16 i + 4 (lane / 16) .., column 16 j + lane % 16 of the
+// TILE_LDS bytes; free again at return.  acc[i][j]: rows 16 i + 4 (lane / 16) .., column 16 j + lane % 16 of the
 // wave's quarter (wave / 2, wave % 2).
-template <int F>
+template <int F, int DEPTH>
 __device__ __forceinline__ void tile_gemm(f32x4 (&acc)[F][F], char *lds, const Side &u, const Side &v, bool same, int steps)
 {
     constexpr int SIDE_BYTES = Tile<F>::SIDE_BYTES, SIDE = Tile<F>::SIDE;
@@ -578,7 +582,7 @@ __device__ __forceinline__ void tile_gemm(f32x4 (&acc)[F][F], char *lds, const S
     const int word = (lane >> 4) * SIDE + (lane & 15);
     const char *us = lds + ((wave >> 1) * 16 * F + word) * 16;
     const char *vs = lds + (same ? 0 : SIDE_BYTES) + ((wave & 1) * 16 * F + word) * 16;
-    constexpr int DEPTH = Tile<F>::DEPTH, AHEAD = DEPTH - 1;
+    constexpr int AHEAD = DEPTH - 1;
 #pragma unroll
     for (int b = 0; b < AHEAD; ++b)
         if (b < steps)
@@ -646,7 +650,8 @@ __device__ __forceinline__ const W *tile_to_lds(const f32x4 (&acc)[F][F], char *
 }
 
 // A = X X', lower tiles, each over a share of k: the accumulators as they lie, 16 bytes a lane
-template <int F> __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_gram(const NsTable *__restrict__ tp, int step)
+template <int F, int DEPTH>
+__global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_gram(const NsTable *__restrict__ tp, int step)
 {
     const NsTable &t = *tp;
     constexpr int SIDE = Tile<F>::SIDE;
@@ -662,7 +667,7 @@ template <int F> __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_gram(co
     const _Float16 *x = step & 1 ? s.xk[1] : s.xk[0];
     const size_t plane = (size_t)d.rp * d.kp;
     f32x4 acc[F][F];
-    tile_gemm<F>(acc, lds, side_of(x, plane, d.rp, ti * SIDE, s0 * STEP), side_of(x, plane, d.rp, tj * SIDE, s0 * STEP),
+    tile_gemm<F, DEPTH>(acc, lds, side_of(x, plane, d.rp, ti * SIDE, s0 * STEP), side_of(x, plane, d.rp, tj * SIDE, s0 * STEP),
                  ti == tj, s1 - s0);
     f32x4 *out = reinterpret_cast<f32x4 *>(s.part + (size_t)local * SIDE * SIDE) + (threadIdx.x >> 6) * F * F * 64 + (threadIdx.x & 63);
 #pragma unroll
@@ -728,7 +733,8 @@ __global__ __launch_bounds__(SUM_THREADS) void k_ns_sum(const NsTable *__restric
 }
 
 // Q = a I + b A + c A A, lower tiles and their mirror images
-template <int F> __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_poly(const NsTable *__restrict__ tp)
+template <int F, int DEPTH>
+__global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_poly(const NsTable *__restrict__ tp)
 {
     const NsTable &t = *tp;
     constexpr int SIDE = Tile<F>::SIDE;
@@ -754,7 +760,7 @@ template <int F> __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_poly(co
             lo[i][j] = *reinterpret_cast<const h4 *>(pij + plane);
         }
     f32x4 acc[F][F];
-    tile_gemm<F>(acc, lds, side_of(s.a, plane, d.rp, i0, 0), side_of(s.a, plane, d.rp, j0, 0), ti == tj, d.rp / STEP);
+    tile_gemm<F, DEPTH>(acc, lds, side_of(s.a, plane, d.rp, i0, 0), side_of(s.a, plane, d.rp, j0, 0), ti == tj, d.rp / STEP);
     const float ca = t.c * dance::pow2f(-2 * X_EXP) * t.q_mul, ba = t.b * dance::pow2f(-X_EXP) * t.q_mul, a = t.a * t.q_mul;
     const unsigned *tile = tile_to_lds<unsigned>(acc, lds, [&](int i, int j, f32x4 v) {
 #pragma unroll
@@ -810,7 +816,8 @@ __device__ __forceinline__ void put_result(const NsTable &t, const NsItem &it, c
 }
 
 // X <- Q X; the last step writes the result
-template <int F> __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_apply(const NsTable *__restrict__ tp, int step, int last)
+template <int F, int DEPTH>
+__global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_apply(const NsTable *__restrict__ tp, int step, int last)
 {
     const NsTable &t = *tp;
     constexpr int SIDE = Tile<F>::SIDE;
@@ -823,7 +830,7 @@ template <int F> __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_apply(c
     const int down = d.rp / SIDE, i0 = local % down * SIDE, j0 = local / down * SIDE;
     const size_t square = (size_t)d.rp * d.rp, rect = (size_t)d.rp * d.kp;
     f32x4 acc[F][F];
-    tile_gemm<F>(acc, lds, side_of(s.q, square, d.rp, i0, 0), side_of(step & 1 ? s.xr[1] : s.xr[0], rect, d.kp, j0, 0), false,
+    tile_gemm<F, DEPTH>(acc, lds, side_of(s.q, square, d.rp, i0, 0), side_of(step & 1 ? s.xr[1] : s.xr[0], rect, d.kp, j0, 0), false,
               d.rp / STEP);
     const float mul = 1.0f / t.q_mul;
     if (!last) {
@@ -1604,18 +1611,20 @@ struct Chain {
         });
     }
 
-    // kernel<F> on `tiles` tiles of side `side`, F = side / 32
+    // kernel<F, DEPTH> on `tiles` tiles of side `side`, F = side / 32
     template <typename K, typename... Args> int tiled(int side, long long tiles, K &&kernel, Args... args) const
     {
-        auto go = [&](auto f) {
-            constexpr int F = decltype(f)::value;
-            auto k = kernel(f);
-            if (int r = dance::allow_lds((const void *)k, Tile<F>::LDS, fn))
+        auto go = [&](auto f, auto depth) {
+            constexpr int LDS = TILE_LDS<decltype(f)::value, decltype(depth)::value>;
+            auto k = kernel(f, depth);
+            if (int r = dance::allow_lds((const void *)k, LDS, fn))
                 return r;
-            hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(GEMM_THREADS), Tile<F>::LDS, st, (const NsTable *)kept, args...);
+            hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(GEMM_THREADS), LDS, st, (const NsTable *)kept, args...);
             return launched();
         };
-        return side == 128 ? go(std::integral_constant<int, 4>{}) : go(std::integral_constant<int, 2>{});
+        constexpr std::integral_constant<int, 2> two{};
+        constexpr std::integral_constant<int, 4> four{};
+        return side == 128 ? go(four, two) : tiles > 512 ? go(two, two) : go(two, four);
     }
 
     // step s of the X of all matrices, and the A of the next step; X itself is the -1st
@@ -1642,11 +1651,11 @@ struct Chain {
             });
         }
         if (e == 0 && rect > 0 && s >= 0)
-            e = tiled(poly_side, poly, [](auto f) { return k_ns_poly<decltype(f)::value>; });
+            e = tiled(poly_side, poly, [](auto f, auto depth) { return k_ns_poly<decltype(f)::value, decltype(depth)::value>; });
         if (e == 0 && rect > 0 && s >= 0)
-            e = tiled(rect_side, rect, [](auto f) { return k_ns_apply<decltype(f)::value>; }, s, last);
+            e = tiled(rect_side, rect, [](auto f, auto depth) { return k_ns_apply<decltype(f)::value, decltype(depth)::value>; }, s, last);
         if (e == 0 && rect > 0 && !last)
-            e = tiled(t.gram_side, gram, [](auto f) { return k_ns_gram<decltype(f)::value>; }, s + 1);
+            e = tiled(t.gram_side, gram, [](auto f, auto depth) { return k_ns_gram<decltype(f)::value, decltype(depth)::value>; }, s + 1);
         if (e == 0 && !last) {
             hipLaunchKernelGGL(k_ns_sum, dim3((unsigned)sum), dim3(SUM_THREADS), 0, st, (const NsTable *)kept);
             e = launched();

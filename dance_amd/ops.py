@@ -618,6 +618,8 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="relu"):
                            % (tuple(x.stride()),))
     if num_groups < 1 or c < 1 or c % num_groups:
         raise RuntimeError("group_norm_act: %d channels do not divide into %d groups" % (c, num_groups))
+    if x.size(0) > 65535 or c > 4096:
+        raise RuntimeError("group_norm_act: at most 65535 images and 4096 channels (2048 of fp32), got %s" % (tuple(x.shape),))
     for name, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
@@ -664,6 +666,8 @@ def orthogonalize(x, steps=5, eps=1e-7, coefficients=NS_COEFFICIENTS):
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("orthogonalize is not differentiable: call it on a detached tensor or under torch.no_grad()")
     m, n = x.shape[-2:]
+    if m * n >= 2 ** 31 or math.prod(x.shape[:-2]) >= 2 ** 31:
+        raise RuntimeError("orthogonalize: fewer than 2^31 matrices of fewer than 2^31 elements expected, got %s" % (tuple(x.shape),))
     dev = x.device
     out = torch.empty(x.shape, dtype=x.dtype, device=dev)
     x = x.reshape((-1, m, n)) if x.numel() else x.new_empty((0, m, n))

@@ -402,3 +402,11 @@ def test_maps_larger_than_the_cache(device, dtype, c, lo, hi):
     for name, got in (("y", y), ("dx", dfull.permute(0, 3, 1, 2)[:, lo:hi]), ("dweight", dw), ("dbias", db)):
         _check(got, want[name], name)
     assert not bool(dfull[..., :lo].any()) and not bool(dfull[..., hi:].any())
+
+
+def test_more_images_or_channels_than_a_call_takes(device):
+    one = torch.zeros((1, 8), device=device)
+    for big in (one.expand(65536, 8), one.expand(2 ** 32 + 1, 8), torch.zeros((1, 8192), device=device)):
+        with pytest.raises(RuntimeError, match="at most 65535 images and 4096 channels"):
+            ops.group_norm_act(big, 1)
+    assert ops.group_norm_act(one.expand(65535, 8), 1).shape == (65535, 8)

@@ -204,6 +204,17 @@ def test_refusals(device):
         assert not ops.orthogonalize(x.clone().requires_grad_(True)).requires_grad
 
 
+def test_sizes_past_the_library_s_integers(device):
+    """refused before anything is allocated or launched"""
+    one = torch.zeros((1, 1), device=device)
+    for big in (one.expand(2 ** 32, 1), one.expand(2 ** 16, 2 ** 15), one[None].expand(2 ** 31, 1, 1)):
+        with pytest.raises(RuntimeError, match="2\\^31"):
+            ops.orthogonalize(big)
+    p, m = (torch.empty((2 ** 31, 1), device=device, dtype=torch.float16) for _ in range(2))
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        optim.muon_step([p], [p], [m], lr=0.1)
+
+
 # ------------------------------------------------------------------------------------------- Muon
 def _muon_check(params, grads, buffers, before, dtype, lr, momentum, nesterov, weight_decay, what):
     """params, buffers after a step that started from `before`"""

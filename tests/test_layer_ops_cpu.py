@@ -89,7 +89,8 @@ def test_orthogonalize_empty_and_workspace():
     assert size(0, 4, 8) == 0 and size(1, 0, 8) == 0 and size(1, 1 << 16, 1 << 15) == 0
     assert size(1, 64, 200) == 0 and size(48, 32, 9) == 0   # a compute unit's LDS holds the whole chain
     need = size(3, 100, 500)
-    assert need >= 3 * 16 * 100 * 500                       # two layouts, two steps, 4 bytes each
+    assert need >= 3 * 4 * 100 * 500                        # up to 128 rows: X in place, 4 bytes each
+    assert size(3, 200, 500) >= 3 * 16 * 200 * 500          # more: two layouts, two steps
     fake = ctypes.c_void_p(64)
     good = dict(x=fake, out=fake, batch=3, m=100, n=500)
     assert _orth(ws=fake, ws_bytes=need - 1, **good) == BAD and _orth(ws=None, ws_bytes=need, **good) == BAD
