@@ -35,6 +35,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
 constexpr int PAD = 128;                            // rows and columns are padded to whole tiles of the GEMM
+constexpr long long MOST_ELEMENTS = INT_MAX - PAD;  // of a matrix: its padded sides fit an int
 constexpr int PACK = 64;                            // side of the tiles M is packed by
 constexpr int NS_ITEMS = 48;                        // 48 descriptions fit the 4 KB of kernel arguments
 constexpr int NS_SLICES = 256;                      // most workgroups that share a matrix's norm
@@ -1670,7 +1671,7 @@ bool usable(double a, double b, double c) { return isfinite(a) && isfinite(b) &&
 
 extern "C" int64_t dance_orthogonalize_workspace_bytes(int batch, int m, int n)
 {
-    if (batch <= 0 || m <= 0 || n <= 0 || (long long)m * n >= (1ll << 31))
+    if (batch <= 0 || m <= 0 || n <= 0 || (long long)m * n > MOST_ELEMENTS)
         return 0;
     NsTable t;
     t.count = batch < NS_ITEMS ? batch : NS_ITEMS;
@@ -1685,7 +1686,7 @@ extern "C" int dance_orthogonalize(const void *x, int64_t batch_stride, int64_t 
                                    int dtype, void *out, int batch, int m, int n, int steps, float a, float b, float c,
                                    float eps, void *ws, int64_t ws_bytes, void *stream)
 {
-    DANCE_REQUIRE(batch >= 0 && m >= 0 && n >= 0 && (long long)m * n < (1ll << 31));
+    DANCE_REQUIRE(batch >= 0 && m >= 0 && n >= 0 && (long long)m * n <= MOST_ELEMENTS);
     DANCE_REQUIRE(known_dtype(dtype) && steps >= 1 && steps <= 100 && usable(a, b, c) && eps > 0.0f);
     DANCE_REQUIRE(batch_stride >= 0 && row_stride >= 0 && col_stride >= 0);
     if (batch == 0 || m == 0 || n == 0)
@@ -1739,6 +1740,22 @@ int take(const dance_muon_item *items, int count, bool wide, int at, NsTable &t)
     }
     return at;
 }
+
+// The workspace of the narrow matrices' chains and of the others', the largest of either kind: the chains of a kind
+// follow each other on one stream, those of the other kind run beside them on another -> both together
+int64_t muon_space(const dance_muon_item *items, int count, int64_t (&most)[2])
+{
+    for (int wide = 0; wide < 2; ++wide) {
+        most[wide] = 0;
+        for (int at = 0; at < count;) {
+            NsTable t;
+            at = take(items, count, wide, at, t);
+            const int64_t bytes = lay_out(t, nullptr);
+            most[wide] = bytes > most[wide] ? bytes : most[wide];
+        }
+    }
+    return most[0] + most[1];
+}
 }  // namespace
 
 extern "C" int64_t dance_muon_workspace_bytes(const dance_muon_item *items_host, int count)
@@ -1746,19 +1763,10 @@ extern "C" int64_t dance_muon_workspace_bytes(const dance_muon_item *items_host,
     if (count <= 0 || !items_host)
         return 0;
     for (int i = 0; i < count; ++i)
-        if (items_host[i].rows <= 0 || items_host[i].cols <= 0 || (long long)items_host[i].rows * items_host[i].cols >= (1ll << 31))
+        if (items_host[i].rows <= 0 || items_host[i].cols <= 0 || (long long)items_host[i].rows * items_host[i].cols > MOST_ELEMENTS)
             return 0;
-    int64_t most = 0;
-    for (int at[2] = {0, 0}; at[0] < count || at[1] < count;) {
-        int64_t sum = 0;
-        for (int wide = 0; wide < 2; ++wide) {
-            NsTable t;
-            at[wide] = take(items_host, count, wide, at[wide], t);
-            sum += lay_out(t, nullptr);
-        }
-        most = sum > most ? sum : most;
-    }
-    return most;
+    int64_t most[2];
+    return muon_space(items_host, count, most);
 }
 
 extern "C" int dance_muon_step(const dance_muon_item *items_host, int count, int dtype, double lr, double momentum,
@@ -1773,14 +1781,14 @@ extern "C" int dance_muon_step(const dance_muon_item *items_host, int count, int
     for (int i = 0; i < count; ++i) {
         DANCE_REQUIRE(items_host[i].param && items_host[i].grad && items_host[i].momentum);
         DANCE_REQUIRE(items_host[i].rows >= 1 && items_host[i].cols >= 1);
-        DANCE_REQUIRE((long long)items_host[i].rows * items_host[i].cols < (1ll << 31));
+        DANCE_REQUIRE((long long)items_host[i].rows * items_host[i].cols <= MOST_ELEMENTS);
     }
-    const int64_t need = dance_muon_workspace_bytes(items_host, count);
+    int64_t most[2];
+    const int64_t need = muon_space(items_host, count, most);
     DANCE_REQUIRE(ws_bytes >= need && (ws || need == 0));
     for (int at[2] = {0, 0}; at[0] < count || at[1] < count;) {
         // the narrow matrices and the others: two chains, launched in turn so that two streams run beside each other
         Chain chains[2];
-        char *space = (char *)ws;
         for (int wide = 1; wide >= 0; --wide) {
             NsTable &t = chains[wide].t;
             memset(&t, 0, sizeof t);
@@ -1799,10 +1807,9 @@ extern "C" int dance_muon_step(const dance_muon_item *items_host, int count, int
                 const double m = t.it[i].m, n = t.it[i].n;
                 t.it[i].scale = (float)(lr * (m > n ? sqrt(m / n) : 1.0));
             }
-            const int64_t bytes = lay_out(t, space);
-            if (int rc = chains[wide].prepare(space, (hipStream_t)(wide && side_stream ? side_stream : stream), __func__))
+            if (int rc = chains[wide].prepare((char *)ws + (wide ? most[0] : 0),
+                                              (hipStream_t)(wide && side_stream ? side_stream : stream), __func__))
                 return rc;
-            space += bytes;
         }
         for (int s = -1; s < steps; ++s)
             for (int wide = 1; wide >= 0; --wide)

@@ -637,6 +637,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="relu"):
 
 
 # -------------------------------------------------------------------- orthogonalised updates
+MOST_ELEMENTS = 2 ** 31 - 129                   # of a matrix: the kernels' indexes, its sides padded, fit an int
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)     # singular values from 0.01 up end within 0.7 .. 1.2 in 5 steps
 
 
@@ -666,8 +667,9 @@ def orthogonalize(x, steps=5, eps=1e-7, coefficients=NS_COEFFICIENTS):
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("orthogonalize is not differentiable: call it on a detached tensor or under torch.no_grad()")
     m, n = x.shape[-2:]
-    if m * n >= 2 ** 31 or math.prod(x.shape[:-2]) >= 2 ** 31:
-        raise RuntimeError("orthogonalize: fewer than 2^31 matrices of fewer than 2^31 elements expected, got %s" % (tuple(x.shape),))
+    if m * n > MOST_ELEMENTS or math.prod(x.shape[:-2]) >= 2 ** 31:
+        raise RuntimeError("orthogonalize: fewer than 2^31 matrices of at most 2^31 - 129 elements expected, got %s"
+                           % (tuple(x.shape),))
     dev = x.device
     out = torch.empty(x.shape, dtype=x.dtype, device=dev)
     x = x.reshape((-1, m, n)) if x.numel() else x.new_empty((0, m, n))

@@ -13,7 +13,7 @@ import threading
 import torch
 
 from ._lib import MuonItemStruct, check, lib, on_device, ptr, stream_of
-from .ops import DTYPE_CODES, NS_COEFFICIENTS, _need_gpu, _scratch, check_newton_schulz
+from .ops import DTYPE_CODES, MOST_ELEMENTS, NS_COEFFICIENTS, _need_gpu, _scratch, check_newton_schulz
 
 
 NARROW_ROWS = 128           # up to so many rows (of the smaller side) a step of the chain is a launch of its own
@@ -93,8 +93,8 @@ def muon_step(params, grads, momentum_buffers, *, lr, momentum=0.95, nesterov=Tr
         size = shape.numel()
         if size == 0:
             continue
-        if size >= 2 ** 31:
-            raise RuntimeError("%s: a matrix of 2^31 elements or more: %s" % (what, tuple(shape)))
+        if size > MOST_ELEMENTS:
+            raise RuntimeError("%s: a matrix of more than 2^31 - 129 elements: %s" % (what, tuple(shape)))
         rows = shape[0]
         cols = size // rows
         chain = chains.get((index, dtype))

@@ -691,7 +691,7 @@ int dance_group_norm_act_backward(const void *dy, int64_t dy_image_stride, int64
  * x: element strides >= 0 of the batch, the rows and the columns.  The products are fp32-accurate (split
  * halves, three f16 MFMAs each) for every type; out is rounded once.  Coefficients have to keep the
  * singular values below 2 (the usual 3.4445, -4.7750, 2.0315 stay below 1.21), or the result is not finite.
- * A matrix with a NaN or an infinity comes out NaN, a zero matrix zero.  m n < 2^31.  ws:
+ * A matrix with a NaN or an infinity comes out NaN, a zero matrix zero.  m n <= 2^31 - 129.  ws:
  * dance_orthogonalize_workspace_bytes of 16-byte aligned scratch (0 for small matrices: NULL), nothing to clear. */
 int64_t dance_orthogonalize_workspace_bytes(int batch, int m, int n);
 int dance_orthogonalize(const void *x, int64_t batch_stride, int64_t row_stride, int64_t col_stride,

@@ -420,6 +420,22 @@ def test_narrow_and_wide_matrices_beside_each_other(device, repeat):
     _muon_check(params[:7], grads, buffers, before, torch.float32, 0.1, 0.95, True, 0.0, "both")
 
 
+@pytest.mark.parametrize("narrow,wide", [(60, 3), (3, 60), (100, 50)])
+def test_many_of_one_kind_beside_few_of_the_other(device, narrow, wide):
+    """the launches of one kind reuse their part of the workspace while the other kind's may still run"""
+    shapes = [(100, 300 + i % 3) for i in range(narrow)] + [(400, 500 + i % 2) for i in range(wide)]
+    def lists():
+        return [[_matrix(*s, 1000 * k + i).to(device) for i, s in enumerate(shapes)] for k in range(3)]
+    params, grads, buffers = lists()
+    alone = lists()
+    for _ in range(3):
+        optim.muon_step(params, grads, buffers, lr=0.1)
+    for _ in range(3):
+        optim.muon_step(*[t[:narrow] for t in alone], lr=0.1)
+        optim.muon_step(*[t[narrow:] for t in alone], lr=0.1)
+    assert all(torch.equal(a, b) for a, b in zip(params + buffers, alone[0] + alone[2]))
+
+
 def test_captured_on_two_streams(device):
     """the fork into the step's own stream and the join are part of a captured graph; two graphs and eager steps in turn,
     captured and replayed on a stream of the caller's"""

@@ -87,6 +87,7 @@ def test_orthogonalize_empty_and_workspace():
     assert _orth(batch=0) == 0 and _orth(m=0) == 0 and _orth(n=0) == 0
     size = _lib.lib().dance_orthogonalize_workspace_bytes
     assert size(0, 4, 8) == 0 and size(1, 0, 8) == 0 and size(1, 1 << 16, 1 << 15) == 0
+    assert size(1, 1, 2 ** 31 - 1) == 0 and _orth(m=1, n=2 ** 31 - 1) == BAD          # the padded side would not fit an int
     assert size(1, 64, 200) == 0 and size(48, 32, 9) == 0   # a compute unit's LDS holds the whole chain
     need = size(3, 100, 500)
     assert need >= 3 * 4 * 100 * 500                        # up to 128 rows: X in place, 4 bytes each
@@ -123,6 +124,20 @@ def test_muon_refuses():
         setattr(items[1], field, bad)
         assert _muon(items, **good) == BAD, field
         setattr(items[1], field, keep)
+
+
+def test_muon_workspace_keeps_the_kinds_apart():
+    """matrices of up to 128 rows and the others run beside each other on two streams, and more of a kind than one launch
+    takes follow each other: what one kind uses must not depend on how many launches the other one takes"""
+    def size(*shapes):
+        items = (_lib.MuonItemStruct * len(shapes))()
+        for it, s in zip(items, shapes):
+            it.param, it.grad, it.momentum, it.rows, it.cols = 64, 64, 64, s[0], s[1]
+        return _lib.lib().dance_muon_workspace_bytes(items, len(shapes))
+    narrow, wide = [(100, 900)], [(200, 300)]
+    for n, w in ((1, 1), (48, 5), (60, 5), (5, 60), (100, 100)):
+        assert size(*narrow * n, *wide * w) == size(*narrow * n) + size(*wide * w)
+        assert size(*narrow * n) == size(*narrow * min(n, 48)) and size(*wide * w) == size(*wide * min(w, 48))
 
 
 def test_muon_item_layout_matches_header():
