@@ -5,17 +5,23 @@
 //
 // Arithmetic.  The chain multiplies an error of its first step by up to a^4 = 140, so operands of 8 or 11 bits
 // are not enough.  Every matrix is carried as split halves hi + lo (p16.h, 22 bits) and every product is three
-// f16 MFMAs summed in fp32: the chain's error is then the fp32 chain's (5 steps on 128 x 1152: 1.4e-6 norm-wise
-// either way), at 16/3 of the fp32 MFMA rate.  (The same steps taken on A alone, with one product by X at the
+// f16 MFMAs summed in fp32: the chain's error is then the fp32 chain's (5 steps on 128 x 1152, norm-wise: 0.6e-6
+// against 1.3e-6), at 7.5 / 3 of the fp32 rate (f16 and fp32 products of 8192 x 8192: 1153 and 154 TFLOP/s).  (The same steps taken on A alone, with one product by X at the
 // end, would be a third of the work for wide matrices, but small singular values then come out of A, where
 // they are squared: 1e-4 .. 1e-2 off.)  Normalisation bounds every entry, so the power-of-two scales that keep
 // lo halves normal numbers are constants.
 //
 // Layout.  A GEMM here is  C[i][j] = sum_k U[i][k] V[j][k].  An operand of `rows` rows is stored
 // [plane hi / lo][k / 8][row][8]: the 8 consecutive k of one row an MFMA lane takes are one 16-byte word, the
-// 16 rows of a fragment are 256 consecutive bytes, so fragments come straight from L2, without LDS or barriers.
-// X is kept twice, with k along its columns (for X X') and along its rows (for Q X); A and Q are symmetric.
-// Rows and columns are padded with zeros to whole tiles of 64.
+// 16 rows of a fragment are 256 consecutive bytes: memory and LDS hold the same words, a copy moves them as they
+// lie and fragments are read without bank conflicts.  X is kept twice, with k along its columns (for X X') and
+// along its rows (for Q X); A and Q are symmetric, their products are taken on and below the diagonal.  Rows and
+// columns are padded with zeros to whole tiles of 128.
+//
+// Three kinds of matrices: those whose chain fits one compute unit's LDS (k_ns_small: the whole chain in one
+// workgroup, a launch for all of them), those of up to 128 rows (k_ns_narrow: a launch a step and one that adds
+// shares), and the others (k_ns_gram, k_ns_sum, k_ns_poly, k_ns_apply).  us a matrix or batch, one way / the next
+// kind's: 64 x 256 24 / 73, 21 of 128 x 1152 104 / 152.
 //
 // One launch covers matrices of any number of shapes (up to NS_ITEMS): a workgroup finds its matrix from the tile
 // counts in a table.  The first kernel gets the table as its arguments and leaves it in the workspace for the
@@ -55,8 +61,9 @@ static_assert(sizeof(NsItem) == 48, "three words of 16 bytes: find_item");
 
 struct NsTable {
     NsItem it[NS_ITEMS];
-    // workgroups up to and including item i, INT_MAX past the last: slices of the norm; pack tiles; shares of a narrow
-    // matrix; of the others the lower tiles of A, times split; units (64 x 64) of the sum; lower tiles of Q; tiles of X
+    // workgroups up to and including item i, INT_MAX past the last: slices of the norm; shares of a narrow matrix; fours of
+    // fragments of the sum; of matrices that are not narrow the pack tiles, lower tiles of A, times split, lower tiles of
+    // Q, tiles of X
     int slices[NS_ITEMS], pack[NS_ITEMS], narrow[NS_ITEMS], gram[NS_ITEMS], sum[NS_ITEMS], poly[NS_ITEMS], rect[NS_ITEMS];
     int count, dtype;
     long long row_stride, col_stride;                // of src, orthogonalize only
@@ -212,7 +219,7 @@ __device__ __forceinline__ void load_words(const NsTable &t, const NsItem &it, l
 }
 
 // sums[slice] = sum of squares of a slice of the matrix, in fp64: no square over- or underflows.  DENSE: whole
-// vectors first, the rest one by one; otherwise any strides.
+// vectors first, the rest one by one; otherwise any strides.  Bound by its start and its loads: 5.9 us for 12.4 MB.
 template <typename T, bool DENSE> __global__ __launch_bounds__(256) void k_ns_norm(NsTable t, NsTable *kept)
 {
     constexpr int N = 16 / sizeof(T);
@@ -468,7 +475,8 @@ __device__ __forceinline__ void first_tile(const NsTable &t, const NsItem &it, c
     __syncthreads();
 }
 
-// M / norm -> the first X, a tile of 64 x 64 a workgroup
+// M / norm -> the first X, a tile of 64 x 64 a workgroup.  Bound by memory: 2 x 1024 x 4096 bf16, 17 MB in and 67 MB
+// out, 16.9 us (5.0 TB/s).
 template <typename T, bool DENSE> __global__ __launch_bounds__(256) void k_ns_pack(const NsTable *__restrict__ tp)
 {
     const NsTable &t = *tp;
@@ -650,7 +658,9 @@ __device__ __forceinline__ const W *tile_to_lds(const f32x4 (&acc)[F][F], char *
     return reinterpret_cast<const W *>(lds);
 }
 
-// A = X X', lower tiles, each over a share of k: the accumulators as they lie, 16 bytes a lane
+// A = X X', lower tiles, each over a share of k: the accumulators as they lie, 16 bytes a lane.  2 x 1024 x 4096: 32 us,
+// 900 TFLOP/s of f16 products where a library product of 8192 reaches 1153; two workgroups a compute unit, the first and
+// the last steps of each are what is lost.
 template <int F, int DEPTH>
 __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_gram(const NsTable *__restrict__ tp, int step)
 {
@@ -678,62 +688,54 @@ __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_gram(const NsTable *__re
             out[(i * F + j) * 64] = acc[i][j];
 }
 
-// the shares added in order, split, mirrored: 64 x 64 of A a workgroup, a quarter of a tile of 128 or a tile of 64.
-// 16 bytes of a share a thread, eight shares at once: one or two trips to memory.
-constexpr int SUM_THREADS = 1024;
+// The shares added in order, split, mirrored: a fragment on or below the diagonal a wave, 16 bytes of a share a lane,
+// eight shares at once.  What lies above the diagonal is the mirror image of what lies below it, so A is symmetric to the
+// bit at either side of the tiles, and a matrix gets the same bits whatever the launch holds besides it.
+constexpr int SUM_THREADS = 256;
 __global__ __launch_bounds__(SUM_THREADS) void k_ns_sum(const NsTable *__restrict__ tp)
 {
     const NsTable &t = *tp;
-    constexpr int UNIT = 64, LD = UNIT + 1;
-    __shared__ unsigned tile[UNIT * LD];
-    int index, local, ti, tj;
+    int index, local, fi, fj;
     const NsItem it = find_item(t, t.sum, die_order(), index, local);
     const NsDims d = ns_dims(it.m, it.n);
     NsSpace s;
     ns_space(it.ws, d, it.split, s);
-    const int side = narrow(d) ? PAD : t.gram_side, parts = side == PAD ? 4 : 1;
-    const int part = local & (parts - 1);
-    lower_tile(local / parts, ti, tj);
-    // A unit or fragment above the diagonal is the mirror image of the one below it: A is symmetric to the bit at either
-    // side of the tiles, and a matrix gets the same bits whatever the launch holds besides it
-    const int i0 = ti * side + (part >> 1) * UNIT, j0 = tj * side + (part & 1) * UNIT;
-    if (i0 < j0)
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int fragment = local * (SUM_THREADS / 64) + wave;
+    if (fragment >= lower_tiles(d, 16))
         return;
+    lower_tile(fragment, fi, fj);
+    fi = __builtin_amdgcn_readfirstlane(fi);
+    fj = __builtin_amdgcn_readfirstlane(fj);
+    // the fragment's tile, and its place there: quarter by quarter, as the waves of k_ns_gram have them
+    const int side = narrow(d) ? PAD : t.gram_side, f = side / 32, ti = fi / (2 * f), tj = fj / (2 * f);
+    const int i = fi % (2 * f), j = fj % (2 * f), place = ((i / f) * 2 + j / f) * f * f + i % f * f + j % f;
     const size_t share = (size_t)lower_tiles(d, side) * side * side / 4;
-    const f32x4 *in = reinterpret_cast<const f32x4 *>(s.part + (size_t)(local / parts) * side * side) + part * 16 * 64 + threadIdx.x;
-    // fragment f of the unit: 4 x 4 of a wave, or 2 x 2 of each of 4 waves
-    const int f = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int i = parts == 4 ? f >> 2 : (f >> 3) * 2 + (f >> 1 & 1), j = parts == 4 ? f & 3 : (f >> 2 & 1) * 2 + (f & 1);
-    if (i0 > j0 || i >= j) {
-        f32x4 v = in[0];
-        for (int k = 1; k < it.split; k += 8) {
-            f32x4 w[8];
+    const f32x4 *in = reinterpret_cast<const f32x4 *>(s.part + (size_t)(ti * (ti + 1) / 2 + tj) * side * side) + place * 64 + lane;
+    f32x4 v = in[0];
+    for (int k = 1; k < it.split; k += 8) {
+        f32x4 w[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-                w[u] = in[min(k + u, it.split - 1) * share];
+        for (int u = 0; u < 8; ++u)
+            w[u] = in[min(k + u, it.split - 1) * share];
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (k + u < it.split)
-                    v += w[u];
-        }
-        const int row = 16 * i + 4 * (lane >> 4), col = 16 * j + (lane & 15);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const unsigned word = split_word(v[q] * dance::pow2f(-X_EXP));
-            tile[(row + q) * LD + col] = word;
-            if (i0 == j0 && i > j)
-                tile[col * LD + row + q] = word;
-        }
+        for (int u = 0; u < 8; ++u)
+            if (k + u < it.split)
+                v += w[u];
     }
-    __syncthreads();
+    Quad x = split4(v * dance::pow2f(-X_EXP));
     const size_t plane = (size_t)d.rp * d.rp;
-    if (threadIdx.x < SUM_THREADS / 2)
-        put_rows<UNIT, UNIT, SUM_THREADS / 2>(s.a, plane, d.rp, i0, j0, tile);
-    else if (i0 != j0)
-        put_cols<UNIT, UNIT, SUM_THREADS / 2>(s.a, plane, d.rp, i0, j0, tile, threadIdx.x - SUM_THREADS / 2);
+    const int row = 16 * fi + 4 * (lane >> 4), col = 16 * fj + (lane & 15);
+    put4(s.a + ((size_t)(row >> 3) * d.rp + col) * 8 + (row & 7), plane, x);
+    if (fi != fj) {
+        transpose4(x);                                            // 4 columns of row row + lane % 4
+        put4(s.a + ((size_t)(col >> 3) * d.rp + row + (lane & 3)) * 8 + (col & 4), plane, x);
+    }
 }
 
-// Q = a I + b A + c A A, lower tiles and their mirror images
+// Q = a I + b A + c A A, lower tiles and their mirror images.  2 x 1024 x 1024, 272 tiles of 64: 19 us, 0.45 us a step of
+// 32 k; more buffers, fragments read a step ahead or products in another order did not change that, and 128-tiles would
+// be 72 workgroups for 256 compute units.
 template <int F, int DEPTH>
 __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_poly(const NsTable *__restrict__ tp)
 {
@@ -816,7 +818,8 @@ __device__ __forceinline__ void put_result(const NsTable &t, const NsItem &it, c
     }
 }
 
-// X <- Q X; the last step writes the result
+// X <- Q X; the last step writes the result.  2 x 1024 x 4096: 52 us, 983 TFLOP/s of f16 products: bound by the matrix
+// cores.
 template <int F, int DEPTH>
 __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_apply(const NsTable *__restrict__ tp, int step, int last)
 {
@@ -852,10 +855,11 @@ __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_apply(const NsTable *__r
 }
 
 // ------------------------------------------------------------------------------ narrow matrices
-// Up to 128 rows: a whole step in a launch of its own and one that adds the shares of A (k_ns_sum).  A workgroup owns
-// columns of X, a tile of 128 at a time.  It takes A, computes Q (128^3, in every workgroup: cheaper than a launch),
-// replaces its columns by Q X and sums their own share of the next A.  A, then Q, and the columns lie in LDS, 64 KB
-// each; 8 waves of 64 x 32.
+// Up to 128 rows: a step is a launch of its own and one that adds the shares of A (k_ns_sum).  A workgroup owns columns of
+// X, a tile of 128 at a time.  It takes A, computes Q (in every workgroup: cheaper than a launch), replaces its columns
+// by Q X and sums their own share of the next A.  A, then Q, and the columns lie in LDS, 64 KB each; 8 waves, of 64 x 32
+// in Q X.  21 x 128 x 1152, 189 workgroups: 14.2 us a step.  Of a workgroup's 22 thousand clocks 7 are the matrix
+// instructions' own; copies in, three epilogues and the way out wait for each other, a second workgroup has no room.
 constexpr int NARROW_THREADS = 512;
 constexpr int REGION = 2 * (PAD / 8) * PAD * 16;             // [plane][k block][row] words of 16 bytes
 constexpr int NARROW_LDS = 2 * REGION;
@@ -1034,7 +1038,8 @@ __device__ __forceinline__ void zero(f32x4 (&acc)[5])
         acc[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 }
 
-// M / norm -> the first X and the shares of its A
+// M / norm -> the first X and the shares of its A: 12.7 us for 21 x 128 x 1152, where a launch that lays X out both ways
+// and one that takes A were 10.5 + 7.4
 constexpr int FIRST_TILE = PAD * (PAD + 1) * 4, FIRST_LDS = FIRST_TILE + REGION;
 template <typename T, bool DENSE> __global__ __launch_bounds__(NARROW_THREADS) void k_ns_narrow_first(const NsTable *__restrict__ tp)
 {
@@ -1143,7 +1148,9 @@ template <typename T> __global__ __launch_bounds__(NARROW_THREADS) void k_ns_nar
 
 // ------------------------------------------------------------------------------- small matrices
 // The whole chain of a matrix in one workgroup, X, A and Q in LDS: [plane][k / 8][row][8] as above, padded to 32.
-// 16 waves; a fragment of 16 x 16 of a product is one wave's.
+// 16 waves; a fragment of 16 x 16 of a product is one wave's.  64 x 256, 5 steps: 24 us, 11 thousand clocks until the
+// first X stands and 8.5 a step: X X' 2.4, Q 1.6 and Q X 4.5, whose epilogue (split, transposed, written both ways) is
+// bound by vector instructions.
 constexpr int SMALL_THREADS = 1024, SMALL_WAVES = SMALL_THREADS / 64, SMALL_PAD = 32;
 constexpr size_t SMALL_LDS = 160 * 1024;
 constexpr size_t SMALL_MOST = SMALL_LDS - 1024;
@@ -1471,8 +1478,9 @@ bool is_small(int m, int n) { return small_dims(m, n).bytes <= SMALL_MOST; }
 int split_of(const NsDims &d)
 {
     if (narrow(d)) {
-        // of the column tiles, T: a share is about 1000 clocks to add, a tile 16 times that
-        const int tiles = d.kp / PAD, each = (int)sqrt(tiles / 16.0);
+        // of the T column tiles: a share is about 350 clocks to add, a tile 32 times that.  128 x 65536 with two tiles a
+        // workgroup 284 us, with four 268; 8 x 128 x 16384 with two 311, with one 376
+        const int tiles = d.kp / PAD, each = (int)sqrt(tiles / 32.0);
         return each <= 1 ? tiles : (tiles + each - 1) / each;
     }
     const int want = 256 / lower_tiles(d, PAD), most = d.kp / STEP / 8, split = want < most ? want : most;
@@ -1579,13 +1587,12 @@ struct Chain {
             const NsDims d = ns_dims(t.it[i].m, t.it[i].n);
             const long long want = ((long long)t.it[i].m * t.it[i].n + 8191) / 8192;
             slices += want < NS_SLICES ? want : NS_SLICES;
+            sum += (lower_tiles(d, 16) + SUM_THREADS / 64 - 1) / (SUM_THREADS / 64);
             if (narrow(d)) {
                 narrows += t.it[i].split;
-                sum += 4;
             } else {
                 pack += (long long)(d.rp / PACK) * (d.kp / PACK);
                 gram += (long long)lower_tiles(d, t.gram_side) * t.it[i].split;
-                sum += (long long)lower_tiles(d, t.gram_side) * (t.gram_side == PAD ? 4 : 1);
                 poly += lower_tiles(d, poly_side);
                 rect += (long long)(d.rp / rect_side) * (d.kp / rect_side);
             }
