@@ -564,6 +564,29 @@ def _group_norm_forward(x, groups, weight, bias, eps, act):
     return y, x, saved, (strides, image, pixel, dt, at, act, groups, b, c, hw)
 
 
+def _group_norm_backward(ctx, dy):
+    x, weight, bias, saved = ctx.saved_tensors
+    want_x, want_w, want_b = ctx.needs_input_grad[:3]
+    strides, image, pixel, dt, at, act, groups, b, c, hw = ctx.sizes
+    dev = x.device
+    dx = torch.empty_strided(x.shape, strides, dtype=x.dtype, device=dev) if want_x else None
+    dw = torch.empty_like(weight) if want_w else None
+    db = torch.empty_like(bias) if want_b else None
+    if b == 0 or hw == 0:                            # empty sums
+        return dx, dw if dw is None else dw.zero_(), db if db is None else db.zero_(), None, None, None
+    dy_image, dy_pixel = c * hw, c
+    if dy.stride() != strides:
+        dy, dy_image, dy_pixel = _nhwc_view(dy)
+    h = lib()
+    nbytes = h.dance_group_norm_workspace_bytes(b, c, hw, groups, dt, 1)
+    ws = _scratch(nbytes, dev)
+    with on_device(dev):
+        check(h.dance_group_norm_act_backward(dy.data_ptr(), dy_image, dy_pixel, x.data_ptr(), image, pixel, dt, at, act, groups,
+                                              saved.data_ptr(), ptr(dx), ptr(dw), ptr(db), ptr(ws), nbytes, b, c, hw,
+                                              stream_of(dev)), "group_norm_act backward")
+    return dx, dw, db, None, None, None
+
+
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
@@ -571,30 +594,12 @@ class _GroupNormAct(torch.autograd.Function):
         ctx.save_for_backward(x, weight, bias, saved)
         return y
 
+    # (the wrapper that refuses a second derivative only where one could be asked for)
+    _once = staticmethod(torch.autograd.function.once_differentiable(_group_norm_backward))
+
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, saved = ctx.saved_tensors
-        want_x, want_w, want_b = ctx.needs_input_grad[:3]
-        strides, image, pixel, dt, at, act, groups, b, c, hw = ctx.sizes
-        dev = x.device
-        dx = torch.empty_strided(x.shape, strides, dtype=x.dtype, device=dev) if want_x else None
-        dw = torch.empty_like(weight) if want_w else None
-        db = torch.empty_like(bias) if want_b else None
-        if b == 0 or hw == 0:                        # empty sums
-            return dx, dw if dw is None else dw.zero_(), db if db is None else db.zero_(), None, None, None
-        dy_image, dy_pixel = c * hw, c
-        if dy.stride() != strides:
-            dy, dy_image, dy_pixel = _nhwc_view(dy)
-        h = lib()
-        nbytes = h.dance_group_norm_workspace_bytes(b, c, hw, groups, dt, 1)
-        ws = _scratch(nbytes, dev)
-        with on_device(dev):
-            check(h.dance_group_norm_act_backward(dy.data_ptr(), dy_image, dy_pixel, x.data_ptr(), image, pixel, dt,
-                                                  at, act, groups, saved.data_ptr(), ptr(dx), ptr(dw), ptr(db),
-                                                  ptr(ws), nbytes, b, c, hw, stream_of(dev)),
-                  "group_norm_act backward")
-        return dx, dw, db, None, None, None
+        return _GroupNormAct._once(ctx, dy) if torch.is_grad_enabled() else _group_norm_backward(ctx, dy)
 
 
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="relu"):
