@@ -252,7 +252,8 @@ template <int FL, typename F> __device__ __forceinline__ void for_batch(long lon
     }
 }
 
-// partial (b, nch, groups, 2): sums of a chunk of pixels.  grid: b * nch workgroups, slab = the whole map.
+// partial (b, nch, groups, 2): sums of a chunk of pixels.  grid: b * nch workgroups, slab = the whole map.  Bound by
+// memory: (8, 256, 200, 304) fp32 86 us (5.8 TB/s), (1, 256, 200, 304) bf16 10 us (3.1 TB/s, start and reduction show).
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(MAX_THREADS) void k_gn_stats(const T *__restrict__ x, long long image_stride,
                                                    long long pixel_stride, double *__restrict__ partial, GnDims d)
@@ -291,7 +292,7 @@ __global__ __launch_bounds__(MAX_THREADS) void k_gn_stats(const T *__restrict__ 
 // The mean as a sum of two floats: x - mu keeps its low bits when the mean is large against the spread.  With
 // e = x - mu:  z = e (rstd w) + beta.  Written once an image and channel (by k_gn_finish or k_gn_one), read
 // as one 16-byte word: gathering mean, rstd, weight and bias of each of its channels cost a thread of the
-// apply pass two dozen dependent loads, 8 us of its 17 on a (1, 256, 200, 304) bf16 map.
+// apply pass two dozen dependent loads (17.5 against 15.0 us on a (1, 256, 200, 304) bf16 map).
 struct alignas(16) Channel {
     float mhi, mlo, rw, beta;
 };
@@ -325,7 +326,8 @@ __device__ __forceinline__ Channel channel_constants(double mean, double rstd, f
 
 __device__ __forceinline__ float centred(float x, const Channel &k) { return (x - k.mhi) - k.mlo; }
 
-// partial (b, nch, groups, 2) -> the saved words of a group and its channels.  grid: (groups, b).
+// partial (b, nch, groups, 2) -> the saved words of a group and its channels.  grid: (groups, b).  3 - 5 us: a launch,
+// the reads of a group's partial sums, the affine parameters beside them.
 __global__ __launch_bounds__(256) void k_gn_finish(const double *__restrict__ partial, Saved out, const void *weight,
                                                    const void *bias, int affine_dtype, double count, double eps, GnDims d)
 {
@@ -397,7 +399,8 @@ template <typename T> __device__ __forceinline__ Word<T> apply_word(const Word<T
     return r;
 }
 
-// grid: b * nch workgroups, slab = the whole map
+// grid: b * nch workgroups, slab = the whole map.  Bound by memory: (8, 256, 200, 304) fp32 158 us (6.3 TB/s),
+// (1, 256, 200, 304) bf16 12.5 us (5.0 TB/s).
 template <typename T, bool WHOLE, int ACT, bool STREAM>
 __global__ __launch_bounds__(MAX_THREADS) void k_gn_apply(const T *__restrict__ x, long long image_stride,
                                                           long long pixel_stride, const Channel *__restrict__ channels,
@@ -431,7 +434,8 @@ __global__ __launch_bounds__(MAX_THREADS) void k_gn_apply(const T *__restrict__ 
 }
 
 // Small maps: a workgroup owns a slab of whole groups of an image over all its pixels, at most U vectors a
-// thread, and keeps them in registers: one read, one launch.  grid: b * slabs.
+// thread, and keeps them in registers: one read, one launch.  grid: b * slabs.  (1, 256, 25, 38) fp32: 6.6 us, the trips
+// to memory and the two reductions one after the other.
 template <typename T, bool WHOLE, int U>
 __global__ __launch_bounds__(MAX_THREADS) void k_gn_one(const T *__restrict__ x, long long image_stride, long long pixel_stride,
                                                  const void *weight, const void *bias, int affine_dtype, double eps,
@@ -522,7 +526,8 @@ __device__ __forceinline__ float grad_x(float dz, float e, const Channel &k, flo
 template <bool WHOLE> constexpr int GRAD_IN_FLIGHT = WHOLE ? 4 : 1;       // of each of the two maps
 
 // Per-channel sums of dz and dz xh over a chunk of pixels: partial (b, nch, c, 2) fp32, a thread's own sums
-// of at most chunk / rows terms.  grid: b * nch, slab = the whole map.
+// of at most chunk / rows terms.  grid: b * nch, slab = the whole map.  Bound by memory: (2, 256, 200, 304) fp32 45 us
+// (5.5 TB/s).
 template <typename T, bool WHOLE, int ACT>
 __global__ __launch_bounds__(MAX_THREADS) void k_gn_grad_sums(const T *__restrict__ dy, long long dy_image,
                                                               long long dy_pixel, const T *__restrict__ x,
@@ -581,7 +586,7 @@ __global__ __launch_bounds__(MAX_THREADS) void k_gn_grad_sums(const T *__restric
 }
 
 // partial (b, nch, c, 2) -> sums (b, c, 2) in fp64 and a group's a1, a2 of grad_x.  grid: (groups, b).  Neighbouring
-// threads read neighbouring channels of a chunk, the chunks are dealt to rows of threads.
+// threads read neighbouring channels of a chunk, the chunks are dealt to rows of threads.  (2, 256, 200, 304): 7.3 us.
 __global__ __launch_bounds__(MAX_THREADS) void k_gn_grad_finish(const float *__restrict__ partial, Saved saved,
                                                                 double *__restrict__ sums, float2 *__restrict__ means,
                                                                 GnDims d)
@@ -649,7 +654,8 @@ __global__ __launch_bounds__(64) void k_gn_grad_affine(const double *__restrict_
 }
 
 // grid: b * nch workgroups, slab = the whole map; dx may be NULL (only dw, dbeta wanted: one workgroup then).
-// The last workgroups write dw and dbeta, too: no launch of their own.
+// The last workgroups write dw and dbeta, too: no launch of their own.  Bound by memory: (2, 256, 200, 304) fp32 54 us
+// (6.9 TB/s).
 template <typename T, bool WHOLE, int ACT, bool STREAM>
 __global__ __launch_bounds__(MAX_THREADS) void k_gn_grad_apply(const T *__restrict__ dy, long long dy_image,
                                                                long long dy_pixel, const T *__restrict__ x,
@@ -706,7 +712,8 @@ __global__ __launch_bounds__(MAX_THREADS) void k_gn_grad_apply(const T *__restri
 }
 
 // The backward pass of small maps as k_gn_one is the forward's: x and dy of a slab in registers.  sums
-// (b, c, 2) for k_gn_grad_affine, or, of a single image, dw and dbeta themselves.  grid: b * slabs.
+// (b, c, 2) for k_gn_grad_affine, or, of a single image, dw and dbeta themselves.  grid: b * slabs.  (2, 256, 25, 38)
+// bf16: 12 us.
 template <typename T, bool WHOLE, int U>
 __global__ __launch_bounds__(MAX_THREADS) void k_gn_grad_one(const T *__restrict__ dy, long long dy_image,
                                                              long long dy_pixel, const T *__restrict__ x,

@@ -20,8 +20,8 @@
 //
 // Three kinds of matrices: those whose chain fits one compute unit's LDS (k_ns_small: the whole chain in one
 // workgroup, a launch for all of them), those of up to 128 rows (k_ns_narrow: a launch a step and one that adds
-// shares), and the others (k_ns_gram, k_ns_sum, k_ns_poly, k_ns_apply).  us a matrix or batch, one way / the next
-// kind's: 64 x 256 24 / 73, 21 of 128 x 1152 104 / 152.
+// shares), and the others (k_ns_gram, k_ns_sum, k_ns_poly, k_ns_apply).  us, its kind / the next one: 64 x 256 25 / 85,
+// 64 of 32 x 288 34 / 184; 128 x 256 87 / 94, 21 of 128 x 1152 105 / 144.
 //
 // One launch covers matrices of any number of shapes (up to NS_ITEMS): a workgroup finds its matrix from the tile
 // counts in a table.  The first kernel gets the table as its arguments and leaves it in the workspace for the
@@ -690,7 +690,9 @@ __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_gram(const NsTable *__re
 
 // The shares added in order, split, mirrored: a fragment on or below the diagonal a wave, 16 bytes of a share a lane,
 // eight shares at once.  What lies above the diagonal is the mirror image of what lies below it, so A is symmetric to the
-// bit at either side of the tiles, and a matrix gets the same bits whatever the launch holds besides it.
+// bit at either side of the tiles, and a matrix gets the same bits whatever the launch holds besides it.  7 shares of
+// 2 x 1024 x 1024 (31 MB in, 17 MB out) 8.2 us, 9 shares of 21 x 128 x 128 4.2 us; through LDS, 64 x 64 a workgroup, 9.9
+// and 4.7, and far more for long matrices (128 x 16384 in all 178 -> 150 us).
 constexpr int SUM_THREADS = 256;
 __global__ __launch_bounds__(SUM_THREADS) void k_ns_sum(const NsTable *__restrict__ tp)
 {
@@ -858,7 +860,7 @@ __global__ __launch_bounds__(GEMM_THREADS, 2) void k_ns_apply(const NsTable *__r
 // Up to 128 rows: a step is a launch of its own and one that adds the shares of A (k_ns_sum).  A workgroup owns columns of
 // X, a tile of 128 at a time.  It takes A, computes Q (in every workgroup: cheaper than a launch), replaces its columns
 // by Q X and sums their own share of the next A.  A, then Q, and the columns lie in LDS, 64 KB each; 8 waves, of 64 x 32
-// in Q X.  21 x 128 x 1152, 189 workgroups: 14.2 us a step.  Of a workgroup's 22 thousand clocks 7 are the matrix
+// in Q X.  21 x 128 x 1152, 189 workgroups: 14.2 us a step.  Of a workgroup's 20 thousand clocks 6.5 are the matrix
 // instructions' own; copies in, three epilogues and the way out wait for each other, a second workgroup has no room.
 constexpr int NARROW_THREADS = 512;
 constexpr int REGION = 2 * (PAD / 8) * PAD * 16;             // [plane][k block][row] words of 16 bytes

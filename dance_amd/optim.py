@@ -113,7 +113,8 @@ def muon_step(params, grads, momentum_buffers, *, lr, momentum=0.95, nesterov=Tr
         nbytes = h.dance_muon_workspace_bytes(items, count)
         with on_device(dev):
             ws, cur, side = _scratch(nbytes, dev), None, None
-            if narrow and wide:                  # they leave each other room on the chip: beside each other on two streams
+            if narrow and wide:                  # beside each other on two streams (the refinement net's weights: 276 against
+                                                 # 322 us), since each leaves compute units idle between its launches
                 cur, (side, fork, join) = torch.cuda.current_stream(dev), _side_stream(dev)
                 fork.record(cur)
                 side.wait_event(fork)
