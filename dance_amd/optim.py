@@ -125,13 +125,17 @@ def muon_step(params, grads, momentum_buffers, *, lr, momentum=0.95, nesterov=Tr
                 cur.wait_event(join)
             check(code, what)
     # written behind autograd's back: what caches by version (saved tensors, the modules' packed weights) must see it
+    # (inference tensors have no version)
+    if any(map(torch.is_inference, written)):
+        written = [t for t in written if not t.is_inference()]
     if written:
         torch.autograd.graph.increment_version(written)
 
 
 class Muon(torch.optim.Optimizer):
     """torch.optim optimizer over muon_step.  Every parameter a matrix (two dimensions or more, the first one the
-    rows); parameters without a gradient are left as they are."""
+    rows); parameters without a gradient are left as they are.  A step can be captured into a graph once every
+    momentum buffer exists; its replays keep the settings, lr among them, that it was captured with."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, eps=1e-7,
                  coefficients=NS_COEFFICIENTS):
@@ -160,6 +164,9 @@ class Muon(torch.optim.Optimizer):
             params = [p for p in group["params"] if p.grad is not None]
             for p in params:
                 if "momentum_buffer" not in self.state[p]:
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                        # (a replay would clear the buffer again)
+                        raise RuntimeError("Muon: take a step before the one that is captured into a graph")
                     self.state[p]["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.preserve_format)
             muon_step(params, [p.grad for p in params], [self.state[p]["momentum_buffer"] for p in params],
                       **{k: v for k, v in group.items() if k in ("lr", "momentum", "nesterov", "weight_decay", "steps", "eps",

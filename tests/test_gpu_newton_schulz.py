@@ -351,6 +351,45 @@ def test_muon_optimizer(device):
         y.backward()
 
 
+def test_optimizer_step_captured(device):
+    """refused before the momentum buffers exist (a replay would clear them); afterwards replays are eager steps"""
+    weights = [[torch.nn.Parameter(_matrix(*s, i).to(device)) for i, s in enumerate(((40, 70), (150, 160)))] for _ in range(2)]
+    opts = [optim.Muon(w, lr=0.1, weight_decay=0.1) for w in weights]
+    for w in weights:
+        for i, p in enumerate(w):
+            p.grad = _matrix(*p.shape, 10 + i).to(device)
+    fresh = optim.Muon([torch.nn.Parameter(weights[0][0].detach().clone())])
+    fresh.param_groups[0]["params"][0].grad = weights[0][0].grad.clone()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="before the one that is captured"):
+        with torch.cuda.graph(graph):
+            fresh.step()
+    for opt in opts:
+        opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opts[0].step()
+    for turn in range(4):
+        for w in weights:
+            for i, p in enumerate(w):
+                p.grad.copy_(_matrix(*p.shape, 20 + 2 * turn + i).to(device))
+        graph.replay()
+        opts[1].step()
+        torch.cuda.synchronize()
+        for a, b in zip(*weights):
+            assert torch.equal(a, b) and torch.equal(opts[0].state[a]["momentum_buffer"], opts[1].state[b]["momentum_buffer"]), turn
+
+
+def test_inference_tensors(device):
+    """made under inference_mode, they carry no version"""
+    with torch.inference_mode():
+        p, g, m = (_matrix(30, 50, i).to(device) for i in range(3))
+        before = [(p.clone(), m.clone())]
+        optim.muon_step([p], [g], [m], lr=0.1)
+        _muon_check([p], [g], [m], before, torch.float32, 0.1, 0.95, True, 0.0, "inference")
+        assert ops.orthogonalize(g).is_inference() and ops.group_norm_act(g, 5).is_inference()
+
+
 def test_modules_repack_after_a_step(device):
     """the heads cache weights packed for their kernels; a step on them must be seen"""
     cfg = config.dance_r50(num_sampling=128, num_convs=2)
