@@ -863,11 +863,15 @@ GnDims dims_of(int b, int c, long long hw, int groups, int dtype)
     return d;
 }
 
-// The one-launch form: MAX_THREADS a workgroup, at most `most` vectors a thread.  A slab is the fewest whole
-// groups that make whole vectors and a wanted width.  Wide slabs share fewer cache lines with other
-// workgroups, narrow ones are more workgroups with fewer vectors a thread: 64 bytes a pixel where that still
-// gives the chip a workgroup per unit, else 32, else 16.  false: the map is too large for any.
+// The one-launch form: MAX_THREADS a workgroup, at most `most` vectors a thread.  A slab is the fewest whole groups that
+// make whole vectors and a wanted width: the widest of 1 KB ... 64 bytes a pixel that gives every compute unit a
+// workgroup, else 64 bytes.  Narrower ones, 32 and 16 bytes, read parts of cache lines and are for maps that are in the
+// caches anyway; larger maps that fit no other slab take the two-pass form.  us forward and backward, this rule / at most
+// 64 bytes always: 2048 of (256, 3, 3) 47 / 299, 64 of (256, 25, 38) 118 / 124; this rule / narrow slabs for any size:
+// 64 of (256, 50, 50) fp32 232 / 333, bf16 172 / 373, (256, 50, 50) 24.0 / 27.3; narrow slabs / this rule without them:
+// (256, 25, 38) fp32 16.2 / 20.3, bf16 16.2 / 30.1.  false: the map is too large for any.
 constexpr int ONE_MOST = 16, GRAD_ONE_MOST = 8;
+constexpr double NARROW_MOST = 1.5e6;                     // bytes
 
 bool one_launch(GnDims &d, int b, int dtype, int most)
 {
@@ -875,13 +879,15 @@ bool one_launch(GnDims &d, int b, int dtype, int most)
     const bool whole = d.c % n == 0;
     if (!whole)
         most = 4;                                         // a vector of scalar loads is n registers
+    const bool narrow = (double)b * d.c * d.hw * (16 / n) <= NARROW_MOST;
     bool fits = false;
-    for (int least = 4 * n; least >= n; least /= 2) {
+    for (int least = 64 * n; least >= (narrow ? n : 4 * n); least /= 2) {
         int k = 1;                                        // groups of a slab
         while (k < d.groups && (d.groups % k != 0 || k * d.gc < least || (whole && k * d.gc % n != 0)))
             ++k;
         const int cs = k * d.gc, cv = ceil_div(cs, n);
-        if (cv > MAX_THREADS)
+        const bool enough = (long long)b * (d.c / cs) >= 256;
+        if (cv > MAX_THREADS || (least > 4 * n && !enough))
             continue;
         const int rows = MAX_THREADS / cv;
         if (d.hw > (long long)rows * most)
@@ -890,7 +896,7 @@ bool one_launch(GnDims &d, int b, int dtype, int most)
         d.cs = cs;
         d.cv = cv;
         d.rows = rows < d.hw ? rows : (int)d.hw;
-        if ((long long)b * (d.c / cs) >= 256)
+        if (enough)
             break;
     }
     return fits;

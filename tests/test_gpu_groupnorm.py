@@ -410,3 +410,20 @@ def test_more_images_or_channels_than_a_call_takes(device):
         with pytest.raises(RuntimeError, match="at most 65535 images and 4096 channels"):
             ops.group_norm_act(big, 1)
     assert ops.group_norm_act(one.expand(65535, 8), 1).shape == (65535, 8)
+
+
+@pytest.mark.parametrize("shape,groups", [((65535, 4), 2), ((300, 40, 9, 9), 8), ((600, 256, 3, 3), 32), ((40, 64, 70, 71), 8),
+                                          ((17, 96, 50, 50), 4), ((129, 75, 2, 3), 5)])
+def test_many_images(device, shape, groups):
+    """whole maps a workgroup, and the parameters' gradients over many images"""
+    for dtype in (torch.float32, torch.bfloat16):
+        x = _map(shape, dtype, device, 3).requires_grad_(True)
+        w, be = (t.requires_grad_(True) for t in _affine(shape[1], torch.float32, device, 3))
+        dy = _map(shape, dtype, device, 4)
+        y = ops.group_norm_act(x, groups, w, be, act="silu")
+        got = torch.autograd.grad(y, (x, w, be), dy)
+        want = _oracle(x, groups, w, be, "silu", dy)
+        for name, t in zip(("y", "dx", "dweight", "dbias"), (y,) + got):
+            _check(t, want[name], "%s %s %s" % (shape, dtype, name))
+        only, = torch.autograd.grad(ops.group_norm_act(x.detach(), groups, w, be, act="silu"), (w,), dy)
+        assert torch.equal(only, got[1])
