@@ -77,7 +77,7 @@ class _ConvNormAct(nn.Conv2d):
     """conv3x3 (+ GroupNorm) + ReLU with detectron2.layers.Conv2d's state-dict keys
     (`weight`, `norm.weight`, `norm.bias`).  In eval mode on the GPU the shipped shape
     (C -> C, C % 128 == 0, GroupNorm(32), no bias, dilation 1) runs on the feature-prep kernels
-    (conv3x3 as split-half f16 MFMA implicit GEMM + GroupNorm + ReLU, DESIGN.md 5b; output in
+    (conv3x3 as split-half f16 MFMA implicit GEMM + GroupNorm + ReLU; output in
     channels_last memory); anything else, `DANCE_FEATPREP=torch`, or `use_hip = False` runs
     the stock torch.nn ops.  With `DANCE_GROUPNORM=hip` the norm and the activation of that path run on
     ops.group_norm_act, in training mode and under autograd too, where the convolution's output is
