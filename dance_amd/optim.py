@@ -3,7 +3,8 @@
 A parameter of more than two dimensions is its (first dimension, the rest) matrix: a convolution's weight is
 (out channels, in channels * taps).  Vectors (biases, norm weights) are not Muon's: give them to another
 optimizer.  The whole step -- momentum, Nesterov's look-ahead, the chain of products, the parameter update --
-is one chain of launches for all matrices of one type and device, whatever their shapes.
+shares its launches among all matrices of one type and device, whatever their shapes: one launch where each fits a
+compute unit, else one chain of them for up to 128 rows and one for the others.
 
 The reference trains with Detectron2's SGD (train_net.py:22-70) and has no counterpart.
 """
