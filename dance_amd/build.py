@@ -109,11 +109,8 @@ def device_code_objects(so_path, out_dir):
     return objs
 
 
-def device_isa_counts(so_path=OUT, patterns=PACKED_FP32 + ("v_mfma_f32", "scratch_")):
-    """Disassemble every gfx950 code object bundled in `so_path` and count the instructions whose
-    mnemonic starts with one of `patterns`.  The guard behind NOPK: the flag is a compiler
-    feature switch that a later toolchain may stop honouring (its host-pass warning is filtered
-    out in _compile), so the ISA itself is what build() and tests/test_abi.py look at."""
+def device_isa(so_path=OUT):
+    """The disassembly of every gfx950 code object bundled in `so_path`, a list of lines each."""
     import shutil
     import tempfile
     tmp = tempfile.mkdtemp(prefix="dance_isa_")
@@ -121,20 +118,46 @@ def device_isa_counts(so_path=OUT, patterns=PACKED_FP32 + ("v_mfma_f32", "scratc
         objs = device_code_objects(so_path, tmp)
         if not objs:
             raise RuntimeError("no gfx950 code object found in %s" % so_path)
-        counts = {p: 0 for p in patterns}
-        for f in objs:
-            text = subprocess.run([OBJDUMP, "-d", "--mcpu=" + ARCH, f], check=True,
-                                  stdout=subprocess.PIPE, text=True).stdout
-            for line in text.splitlines():
-                parts = line.split()
-                if parts:
-                    for p in patterns:
-                        if parts[0].startswith(p):
-                            counts[p] += 1
-        counts["code_objects"] = len(objs)
-        return counts
+        return [subprocess.run([OBJDUMP, "-d", "--mcpu=" + ARCH, f], check=True, stdout=subprocess.PIPE,
+                               text=True).stdout.splitlines() for f in objs]
     finally:
         shutil.rmtree(tmp, ignore_errors=True)
+
+
+def device_isa_counts(so_path=OUT, patterns=PACKED_FP32 + ("v_mfma_f32", "scratch_")):
+    """Disassemble every gfx950 code object bundled in `so_path` and count the instructions whose
+    mnemonic starts with one of `patterns`.  The guard behind NOPK: the flag is a compiler
+    feature switch that a later toolchain may stop honouring (its host-pass warning is filtered
+    out in _compile), so the ISA itself is what build() and tests/test_abi.py look at."""
+    texts = device_isa(so_path)
+    counts = {p: 0 for p in patterns}
+    for text in texts:
+        for line in text:
+            parts = line.split()
+            if parts:
+                for p in patterns:
+                    if parts[0].startswith(p):
+                        counts[p] += 1
+    counts["code_objects"] = len(texts)
+    return counts
+
+
+def lds_copies(so_path=OUT):
+    """(copies from memory to LDS, those of them that directly follow a scalar write of M0).  Such a copy takes its
+    LDS address from M0 and needs one wait state after the write; the compiler sees to it for its own instructions,
+    not inside inline assembly."""
+    copies = unwaited = 0
+    for text in device_isa(so_path):
+        before = []
+        for line in text:
+            parts = line.split()
+            if not parts:
+                continue
+            if "_load_lds_" in parts[0] or (parts[0].startswith("buffer_load_") and "lds" in parts):
+                copies += 1
+                unwaited += len(before) > 1 and before[0].startswith("s_") and before[1] == "m0,"
+            before = parts
+    return copies, unwaited
 
 
 def check_no_packed_fp32(so_path=OUT):

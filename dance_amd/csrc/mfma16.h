@@ -269,7 +269,8 @@ __device__ __forceinline__ void stage_commit(const u32x4 (&reg)[(StageGeo<RT, CB
 // s_waitcnt vmcnt(0) before the barrier that publishes the image (stage_dma_wait).
 //   lds_dst: byte offset of the image inside the workgroup's LDS (wave-uniform)
 // (M0 is on the asm's clobber list so that the compiler never carries a value of its own in it across
-// the statement; clang notes that M0 is a reserved register it will not save -- which is what is wanted)
+// the statement; clang notes that M0 is a reserved register it will not save -- which is what is wanted.
+// s_nop: the copy needs one wait state after the write of M0, and the compiler adds none inside the asm)
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 template <int RT, int CBC, int NW>
@@ -292,7 +293,7 @@ __device__ __forceinline__ void stage_dma(int jlo, int jhi, const char *src, uns
                 // nt: the staged activations are read once; without the hint they displace the
                 // weights every workgroup re-reads from L2 (fusion 0.464 -> 0.452 ms at 1536 contours)
                 // (m0 is clobbered: the compiler must not keep a value of its own in it across the asm)
-                asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off nt" : : "v"(g), "s"(l) : "memory", "m0");
+                asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" : : "v"(g), "s"(l) : "memory", "m0");
         }
 }
 

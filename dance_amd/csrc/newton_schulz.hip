@@ -530,11 +530,12 @@ __device__ __forceinline__ Side side_of(const _Float16 *op, size_t plane, int ro
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 // 64 words of 16 bytes, a lane each, from memory to LDS at byte `lds` on.  Inline assembly so that the compiler does
-// not wait for the copy at every LDS read; gemm_wait does before the barrier.
+// not wait for the copy at every LDS read; gemm_wait does before the barrier.  The copy reads M0 one wait state after
+// it was written at the earliest, which nothing but the s_nop sees to inside the assembly.
 __device__ __forceinline__ void copy_words(const _Float16 *from, unsigned lds)
 {
     const unsigned l = __builtin_amdgcn_readfirstlane(lds);
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(l) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(l) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 
