@@ -545,7 +545,7 @@ def _scratch(nbytes, device):
 
 
 def _group_norm_forward(x, groups, weight, bias, eps, act):
-    """-> (y, the map as it was read, what the backward call takes: a tensor, and sizes and strides)"""
+    """-> (y, the map as it was read, what the backward call takes: a tensor, and sizes, types and strides)"""
     shape, dev, dtype = x.shape, x.device, x.dtype
     b, c, hw = shape[0], shape[1], math.prod(shape[2:])
     x, image, pixel = _nhwc_view(x)
@@ -561,17 +561,24 @@ def _group_norm_forward(x, groups, weight, bias, eps, act):
         check(h.dance_group_norm_act(x.data_ptr(), image, pixel, dt, ptr(weight), ptr(bias), at, eps, act, groups,
                                      y.data_ptr(), saved.data_ptr(), ptr(ws), nbytes, b, c, hw, stream_of(dev)),
               "group_norm_act")
-    return y, x, saved, (strides, image, pixel, dt, at, act, groups, b, c, hw)
+    types = [None if t is None else t.dtype for t in (weight, bias)]
+    return y, x, saved, (x.stride(), image, pixel, saved.shape, shape, strides, dtype, dev, types, dt, at, act, groups, b, c, hw)
 
 
 def _group_norm_backward(ctx, dy):
-    x, weight, bias, saved = ctx.saved_tensors
+    x, saved = ctx.saved_tensors
     want_x, want_w, want_b = ctx.needs_input_grad[:3]
-    strides, image, pixel, dt, at, act, groups, b, c, hw = ctx.sizes
-    dev = x.device
-    dx = torch.empty_strided(x.shape, strides, dtype=x.dtype, device=dev) if want_x else None
-    dw = torch.empty_like(weight) if want_w else None
-    db = torch.empty_like(bias) if want_b else None
+    x_strides, image, pixel, saved_shape, shape, strides, dtype, dev, types, dt, at, act, groups, b, c, hw = ctx.sizes
+    # saved-tensor hooks give back what they like: the values in another layout is what those of torch do
+    if x.shape != shape or x.dtype != dtype or x.device != dev or saved.shape != saved_shape or saved.dtype != torch.uint8 \
+            or saved.device != dev:
+        raise RuntimeError("group_norm_act backward: a saved-tensor hook gave back tensors of another shape, type or device")
+    if x.stride() != x_strides:
+        x, image, pixel = _nhwc_view(x)
+    saved = saved.contiguous()
+    dx = torch.empty_strided(shape, strides, dtype=dtype, device=dev) if want_x else None
+    dw = torch.empty((c,), dtype=types[0], device=dev) if want_w else None
+    db = torch.empty((c,), dtype=types[1], device=dev) if want_b else None
     if b == 0 or hw == 0:                            # empty sums
         return dx, dw if dw is None else dw.zero_(), db if db is None else db.zero_(), None, None, None
     dy_image, dy_pixel = c * hw, c
@@ -591,7 +598,7 @@ class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
         y, x, saved, ctx.sizes = _group_norm_forward(x, groups, weight, bias, eps, act)
-        ctx.save_for_backward(x, weight, bias, saved)
+        ctx.save_for_backward(x, saved)              # (the weight as the kernels want it is in `saved`)
         return y
 
     # (the wrapper that refuses a second derivative only where one could be asked for)

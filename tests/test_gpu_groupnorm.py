@@ -427,3 +427,21 @@ def test_many_images(device, shape, groups):
             _check(t, want[name], "%s %s %s" % (shape, dtype, name))
         only, = torch.autograd.grad(ops.group_norm_act(x.detach(), groups, w, be, act="silu"), (w,), dy)
         assert torch.equal(only, got[1])
+
+
+@pytest.mark.parametrize("pin", [False, True])
+@pytest.mark.parametrize("dtype,lo", [(torch.float32, 0), (torch.float32, 1), (torch.bfloat16, 0), (torch.float16, 3)])
+@pytest.mark.parametrize("hw", [(9, 11), (70, 71)])
+def test_saved_tensors_in_host_memory(device, hw, dtype, lo, pin):
+    """save_on_cpu gives the map back in other strides, pinned also channels first: the same bits as without it"""
+    x = _map((2, 40 + lo, *hw), dtype, device, 30)[:, lo:].requires_grad_(True)
+    w, be = _affine(40, dtype, device, 30)
+    w.requires_grad_(True)
+    be.requires_grad_(True)
+    dy = _map((2, 40, *hw), dtype, device, 31)
+    y = ops.group_norm_act(x, 8, w, be, act="silu")
+    want = (y.detach(),) + torch.autograd.grad(y, (x, w, be), dy)
+    with torch.autograd.graph.save_on_cpu(pin_memory=pin):
+        y = ops.group_norm_act(x, 8, w, be, act="silu")
+    got = (y.detach(),) + torch.autograd.grad(y, (x, w, be), dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

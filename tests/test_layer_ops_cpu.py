@@ -1,4 +1,5 @@
 """CPU: the group-norm entry points report bad arguments before anything is enqueued."""
+import contextlib
 import ctypes
 
 import pytest
@@ -164,3 +165,80 @@ def test_rows_outermost():
     assert f(t) and f(t.to(memory_format=torch.channels_last)) and f(t[2:4]) and f(t[:1, 1:2])
     assert not f(t.transpose(0, 1)) and not f(t[:, ::2]) and not f(t[::2]) and not f(t[:, :, :2])
     assert f(torch.zeros((1, 9)).t()) and not f(torch.zeros((3, 9)).t())
+
+
+class _Kernels:
+    """In the library's place: the backward call reads x where and as it is told to (and nowhere outside the tensors of
+    `held`), so that a CPU tensor can stand for the GPU's."""
+
+    def __init__(self, held):
+        self.held, self.called, self.read = held, False, None
+
+    def dance_group_norm_saved_bytes(self, b, c, groups):
+        return 64
+
+    def dance_group_norm_workspace_bytes(self, *sizes):
+        return 0
+
+    def dance_group_norm_act(self, *args):
+        return 0
+
+    def dance_group_norm_act_backward(self, dy, dy_image, dy_pixel, x, image, pixel, *rest):
+        self.called = True
+        if not self.held:
+            return 0
+        b, c, hw = rest[-4:-1]
+        if x in self.held:
+            t = self.held[x]
+            left = t.untyped_storage().nbytes() // 4 - t.storage_offset()
+            assert (b - 1) * image + (hw - 1) * pixel + c <= left, "reads past the end of x"
+        values = (ctypes.c_float * ((b - 1) * image + (hw - 1) * pixel + c)).from_address(x)
+        self.read = [[[values[i * image + p * pixel + ch] for p in range(hw)] for ch in range(c)] for i in range(b)]
+        return 0
+
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """ops' group norm on CPU tensors, up to the library's calls"""
+    kernels = _Kernels({})
+    monkeypatch.setattr(ops, "_need_gpu", lambda *tensors: None)
+    monkeypatch.setattr(ops, "lib", lambda: kernels)
+    monkeypatch.setattr(ops, "on_device", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(ops, "stream_of", lambda device: 0)
+    return kernels
+
+
+def _slice(shape, channels):
+    """a channels-last map, the first channel of a wider one left out"""
+    b, c, h, w = shape
+    wide = torch.arange(b * h * w * (c + channels), dtype=torch.float32).reshape(b, h, w, c + channels)
+    return wide.permute(0, 3, 1, 2)[:, channels:]
+
+
+@pytest.mark.parametrize("channels", [0, 1])
+@pytest.mark.parametrize("unpack", [lambda t: t, torch.clone, lambda t: torch.empty(t.shape, dtype=t.dtype).copy_(t),
+                                    lambda t: t[..., None].expand(*t.shape, 2).contiguous()[..., 0]],
+                         ids=["same", "dense", "channels_first", "spread"])
+def test_group_norm_backward_reads_what_a_hook_gives_back(on_cpu, unpack, channels):
+    """saved-tensor hooks (torch's save_on_cpu among them) give x back in other strides"""
+    x = _slice((2, 8, 4, 5), channels).requires_grad_(True)
+
+    def back(t):
+        t = unpack(t)
+        on_cpu.held[t.data_ptr()] = t
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), back):
+        y = ops.group_norm_act(x, 4)
+        y.backward(torch.ones_like(y))
+    assert on_cpu.read == x.detach().flatten(2).tolist()
+
+
+@pytest.mark.parametrize("unpack", [lambda t: t.double(), lambda t: t[:1], lambda t: t.half(), lambda t: t.to("meta")])
+def test_group_norm_backward_refuses_other_saved_tensors(on_cpu, unpack):
+    x = _slice((2, 8, 4, 5), 0).requires_grad_(True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), unpack):
+        y = ops.group_norm_act(x, 4, torch.ones(8, requires_grad=True))
+        with pytest.raises(RuntimeError, match="saved-tensor hook"):
+            y.backward(torch.ones_like(y))
+    assert not on_cpu.called
