@@ -32,13 +32,16 @@ template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Word { 
 // and output fit: there the next layer finds its input in the cache.
 typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
-__device__ __forceinline__ float load_affine(const void *p, int dtype, int i, float otherwise)
+__device__ __forceinline__ float load_any(const void *p, int dtype, long long i)
 {
-    if (p == nullptr)
-        return otherwise;
     if (dtype == DANCE_F32)
         return ((const float *)p)[i];
     return dtype == DANCE_F16 ? (float)((const _Float16 *)p)[i] : (float)((const __bf16 *)p)[i];
+}
+
+__device__ __forceinline__ float load_affine(const void *p, int dtype, int i, float otherwise)
+{
+    return p == nullptr ? otherwise : load_any(p, dtype, i);
 }
 
 __device__ __forceinline__ void store_affine(void *p, int dtype, int i, double v)
@@ -163,26 +166,41 @@ __device__ __forceinline__ void for_group_sums(const A (*red)[2], int groups, in
 }
 
 // ------------------------------------------------------------------------------------- statistics
-// Sum and sum of squares in fp64: the difference that makes the variance then loses nothing at any mean /
-// spread ratio fp32 inputs can hold.  An fp64 fma is as fast as an fp32 one here; the pass stays bound by
-// its loads.
-template <typename T> __device__ __forceinline__ void add_word(double (&s)[Vec<T>::N], double (&q)[Vec<T>::N], const Word<T> &w)
-{
-#pragma unroll
-    for (int j = 0; j < Vec<T>::N; ++j) {
-        const double x = (double)(float)w.v[j];
-        s[j] += x;
-        q[j] = fma(x, x, q[j]);
-    }
-}
-
-// A thread's sums into red [rows][units].  A unit is a channel, or a whole vector where no vector holds two
-// groups (gc a multiple of it): an eighth or a quarter of the LDS and of the folding.
+// A unit of a workgroup's sums is a channel, or a whole vector where no vector holds two groups (gc a multiple of it): an
+// eighth or a quarter of the LDS and of the folding.
 template <typename T, bool WHOLE> __device__ __forceinline__ bool vector_units(const GnDims &d)
 {
     return WHOLE && d.gc % Vec<T>::N == 0;
 }
 
+// Sums in fp64 of d = x - pivot and d d, the pivot of a group being its first value (channel g gc of pixel 0) in every
+// workgroup.  The variance is the difference of mean d d and (mean d)^2; the pivot is one of the n values, so
+// (mean d)^2 <= n var, and the roundings cost the variance a few n 2^-53 of itself at most, whatever the mean.  (Sums of
+// x and x x: mean 1e6 and spread 0.1 left rstd 1e-3 off.)  An fp64 subtraction or fma is as fast as an fp32 one here;
+// the pass stays bound by its loads.
+template <typename T>
+__device__ __forceinline__ void add_word(double (&s)[Vec<T>::N], double (&q)[Vec<T>::N], const Word<T> &w,
+                                         const double (&pivot)[Vec<T>::N])
+{
+#pragma unroll
+    for (int j = 0; j < Vec<T>::N; ++j) {
+        const double x = (double)(float)w.v[j] - pivot[j];
+        s[j] += x;
+        q[j] = fma(x, x, q[j]);
+    }
+}
+
+// pixel0: the slab's first channel of pixel 0
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void load_pivots(double (&pivot)[Vec<T>::N], const T *pixel0, const GnDims &d, int v)
+{
+    const bool vu = vector_units<T, WHOLE>(d);
+#pragma unroll
+    for (int j = 0; j < Vec<T>::N; ++j)
+        pivot[j] = vu && j > 0 ? pivot[0] : (double)(float)pixel0[min(channel_of<T, WHOLE>(d, v, j), d.cs - 1) / d.gc * d.gc];
+}
+
+// A thread's sums into red [rows][units].
 template <typename T, bool WHOLE>
 __device__ __forceinline__ void put_units(double (*red)[2], const double (&s)[Vec<T>::N], const double (&q)[Vec<T>::N],
                                           const GnDims &d, int row, int v)
@@ -207,10 +225,11 @@ __device__ __forceinline__ void put_units(double (*red)[2], const double (&s)[Ve
     }
 }
 
-__device__ __forceinline__ void finish_group(double s, double q, double count, double eps, double &mean, double &rstd)
+__device__ __forceinline__ void finish_group(double pivot, double s, double q, double count, double eps, double &mean, double &rstd)
 {
-    mean = s / count;
-    double var = q / count - mean * mean;
+    s /= count;
+    mean = pivot + s;
+    double var = q / count - s * s;
     var = var < 0.0 ? 0.0 : var;                          // (a NaN stays one: infinities in the map give NaN, as in torch)
     rstd = 1.0 / sqrt(var + eps);
 }
@@ -269,10 +288,12 @@ __global__ __launch_bounds__(MAX_THREADS) void k_gn_stats(const T *__restrict__ 
         Word<T> w[FL], next[FL];
         long long p = p0 + row;
         load_batch<T, WHOLE, false>(w, xp, pixel_stride, p, p1, d, v);
+        double pivot[N];
+        load_pivots<T, WHOLE>(pivot, xp, d, v);
         for (; p < p1; p += FL * d.rows) {
             if (p + FL * d.rows < p1)
                 load_batch<T, WHOLE, false>(next, xp, pixel_stride, p + FL * d.rows, p1, d, v);
-            for_batch<FL>(p, p1, d.rows, [&](int u) { add_word<T>(s, q, w[u]); });
+            for_batch<FL>(p, p1, d.rows, [&](int u) { add_word<T>(s, q, w[u], pivot); });
 #pragma unroll
             for (int u = 0; u < FL; ++u)
                 w[u] = next[u];
@@ -327,9 +348,10 @@ __device__ __forceinline__ Channel channel_constants(double mean, double rstd, f
 __device__ __forceinline__ float centred(float x, const Channel &k) { return (x - k.mhi) - k.mlo; }
 
 // partial (b, nch, groups, 2) -> the saved words of a group and its channels.  grid: (groups, b).  3 - 5 us: a launch,
-// the reads of a group's partial sums, the affine parameters beside them.
-__global__ __launch_bounds__(256) void k_gn_finish(const double *__restrict__ partial, Saved out, const void *weight,
-                                                   const void *bias, int affine_dtype, double count, double eps, GnDims d)
+// the reads of a group's partial sums, the affine parameters and the pivot beside them.
+__global__ __launch_bounds__(256) void k_gn_finish(const double *__restrict__ partial, const void *__restrict__ x, int dtype,
+                                                   long long image_stride, Saved out, const void *weight, const void *bias,
+                                                   int affine_dtype, double count, double eps, GnDims d)
 {
     __shared__ double red[4][2];
     const int g = blockIdx.x, b = blockIdx.y;
@@ -340,7 +362,8 @@ __global__ __launch_bounds__(256) void k_gn_finish(const double *__restrict__ pa
         s += p.x;
         q += p.y;
     }
-    // (the affine parameters arrive meanwhile)
+    // (the pivot and the affine parameters arrive meanwhile)
+    const double pivot = (double)load_any(x, dtype, b * image_stride + g * d.gc);
     int cl = threadIdx.x;
     float w = 1.0f, beta = 0.0f;
     if (cl < d.gc) {
@@ -358,8 +381,8 @@ __global__ __launch_bounds__(256) void k_gn_finish(const double *__restrict__ pa
     }
     __syncthreads();
     double mean, rstd;
-    finish_group(red[0][0] + red[1][0] + red[2][0] + red[3][0], red[0][1] + red[1][1] + red[2][1] + red[3][1], count, eps,
-                 mean, rstd);
+    finish_group(pivot, red[0][0] + red[1][0] + red[2][0] + red[3][0], red[0][1] + red[1][1] + red[2][1] + red[3][1], count,
+                 eps, mean, rstd);
     if (threadIdx.x == 0) {
         double *o = out.stats + ((long long)b * d.groups + g) * 2;
         o[0] = mean;
@@ -442,10 +465,13 @@ __global__ __launch_bounds__(MAX_THREADS) void k_gn_one(const T *__restrict__ x,
                                                  int act, T *__restrict__ y, Saved out, GnDims d)
 {
     constexpr int N = Vec<T>::N;
-    extern __shared__ __align__(16) double red[][2];
+    extern __shared__ __align__(16) double lds[][2];
     const int slabs = d.c / d.cs, b = blockIdx.x / slabs, c0 = (blockIdx.x - b * slabs) * d.cs;
     const int row = threadIdx.x / d.cv, v = threadIdx.x - row * d.cv;
     const bool live = row < d.rows;
+    const int sg = d.cs / d.gc;
+    float *pivots = reinterpret_cast<float *>(lds);               // of the slab's groups
+    double (*red)[2] = lds + (sg + 3) / 4;
     const T *xp = x + b * image_stride + c0;
     Word<T> w[U];
     double s[N] = {}, q[N] = {};
@@ -453,21 +479,25 @@ __global__ __launch_bounds__(MAX_THREADS) void k_gn_one(const T *__restrict__ x,
 #pragma unroll
         for (int u = 0; u < U; ++u)
             w[u] = load_word<T, WHOLE>(xp + min((long long)(row + u * d.rows), d.hw - 1) * pixel_stride, d, v);
+        double pivot[N];
+        load_pivots<T, WHOLE>(pivot, xp, d, v);
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (row + u * d.rows < d.hw)
-                add_word<T>(s, q, w[u]);
+                add_word<T>(s, q, w[u], pivot);
         put_units<T, WHOLE>(red, s, q, d, row, v);
     }
+    for (int g = threadIdx.x; g < sg; g += blockDim.x)
+        pivots[g] = (float)xp[g * d.gc];
     const bool vu = vector_units<T, WHOLE>(d);
-    const int units = vu ? d.cv : d.cv * N, sg = d.cs / d.gc;
+    const int units = vu ? d.cv : d.cv * N;
     fold_rows(red, d.rows, units);
     const double (*sums)[2] = red;
     double (*done)[2] = red + units;                      // behind row 0, whose sums are still read
     Channel *constants = reinterpret_cast<Channel *>(done + sg);
     double *st = out.stats + ((long long)b * d.groups + c0 / d.gc) * 2;
     for_group_sums(sums, sg, vu ? d.gc / N : d.gc, [&](int g, double gs, double gq) {
-        finish_group(gs, gq, (double)d.gc * (double)d.hw, eps, done[g][0], done[g][1]);
+        finish_group((double)pivots[g], gs, gq, (double)d.gc * (double)d.hw, eps, done[g][0], done[g][1]);
         st[g * 2] = done[g][0];
         st[g * 2 + 1] = done[g][1];
     });
@@ -987,10 +1017,12 @@ extern "C" int dance_group_norm_act(const void *x, int64_t image_stride, int64_t
             auto one = [&](auto u) {
                 constexpr int U = decltype(u)::value;
                 const int units = vu ? d.cv : d.cv * Vec<T>::N;
-                // the sums of the rows; or row 0 and, behind it, the groups' statistics and the channels' constants
+                // the groups' pivots; the sums of the rows, or row 0 and, behind it, the groups' statistics and the channels'
+                // constants
                 const size_t sums = (size_t)d.rows * units * 2 * sizeof(double);
                 const size_t after = ((size_t)units + d.cs / d.gc) * 2 * sizeof(double) + d.cs * sizeof(Channel);
-                const size_t lds = sums > after ? sums : after;
+                const size_t pivots = (size_t)(d.cs / d.gc + 3) / 4 * 16;
+                const size_t lds = pivots + (sums > after ? sums : after);
                 if (int rc = dance::allow_lds((const void *)k_gn_one<T, W, U>, lds, fn))
                     return rc;
                 hipLaunchKernelGGL((k_gn_one<T, W, U>), dim3((unsigned)(b * (c / d.cs))), dim3(MAX_THREADS), lds, st,
@@ -1011,8 +1043,8 @@ extern "C" int dance_group_norm_act(const void *x, int64_t image_stride, int64_t
                            (long long)pixel_stride, partial, d);
         if (int rc = launch_check(fn))
             return rc;
-        hipLaunchKernelGGL(k_gn_finish, dim3(groups, b), dim3(256), 0, st, (const double *)partial, out, weight, bias,
-                           affine_dtype, (double)d.gc * (double)d.hw, (double)eps, d);
+        hipLaunchKernelGGL(k_gn_finish, dim3(groups, b), dim3(256), 0, st, (const double *)partial, x, dtype,
+                           (long long)image_stride, out, weight, bias, affine_dtype, (double)d.gc * (double)d.hw, (double)eps, d);
         if (int rc = launch_check(fn))
             return rc;
         return with_act(act, [&](auto a) {

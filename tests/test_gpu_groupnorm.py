@@ -445,3 +445,37 @@ def test_saved_tensors_in_host_memory(device, hw, dtype, lo, pin):
         y = ops.group_norm_act(x, 8, w, be, act="silu")
     got = (y.detach(),) + torch.autograd.grad(y, (x, w, be), dy)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("mean,spread,first", [(1e6, 0.1, 0.0), (1e5, 1e-2, 0.0), (1e4, 1e-3, 0.0), (-1e4, 1e-2, 0.0),
+                                               (1e4, 1e-2, -1e6), (3.0, 1.0, 1e5)])
+@pytest.mark.parametrize("shape,groups", [((1, 32, 200, 304), 4), ((2, 30, 150, 130), 5), ((2, 16, 16, 32), 4), ((3, 10, 5, 7), 2)])
+def test_any_mean_and_any_first_value(device, shape, groups, mean, spread, first):
+    """the statistics keep their bits at any ratio of mean and spread that fp32 values can have, also where a group's
+    first value (`first` away from the others) is not like them.  To the tolerances above comes what a mean far from the
+    values' spread adds: its low float is rounded, U |mlo| <= U^2 |mean|, and the oracle's own mean; 2 U^2 |mean| of x
+    are e = 2 U^2 |mean| rstd of xh, in every place that xh has."""
+    g = torch.Generator().manual_seed(11)
+    b, c = shape[:2]
+    x = mean + spread * torch.randn((b, *shape[2:], c), generator=g)
+    x[:, 0, 0, ::c // groups] += first
+    x = x.to(device).permute(0, 3, 1, 2).requires_grad_(True)
+    w, be = _affine(c, torch.float32, device, 11)
+    w.requires_grad_(True)
+    be.requires_grad_(True)
+    dy = torch.randn((b, *shape[2:], c), generator=g).to(device).permute(0, 3, 1, 2)
+    y = ops.group_norm_act(x, groups, w, be, act=None)
+    dx, dw, db = torch.autograd.grad(y, (x, w, be), dy)
+    want = _oracle(x, groups, w, be, None, dy)
+    gx = x.detach().double().reshape(b, groups, -1)
+    far = gx.mean(2, keepdim=True)
+    rstd = 1 / torch.sqrt(((gx - far) ** 2).mean(2, keepdim=True) + 1e-5)
+    e = 2 * U * U * far.abs() * rstd
+    wdz = (dy.double() * w.detach().double()[None, :, None, None]).reshape(gx.shape)
+    xh = (gx - far) * rstd
+    of_dx = rstd * e * ((wdz * xh).mean(2, keepdim=True).abs() + xh.abs() * wdz.abs().mean(2, keepdim=True))
+    each = e.expand(gx.shape).reshape(shape)
+    more = {"y": each * w.detach().double().abs()[None, :, None, None], "dx": of_dx.reshape(shape),
+            "dweight": (dy.double().abs() * each).sum((0, 2, 3)), "dbias": 0.0}
+    for name, got in (("y", y), ("dx", dx), ("dweight", dw), ("dbias", db)):
+        _check(got, (want[name][0], want[name][1] + more[name]), name)
