@@ -893,20 +893,40 @@ GnDims dims_of(int b, int c, long long hw, int groups, int dtype)
     return d;
 }
 
+// LDS of the one-launch form.  Forward: the groups' pivots; the sums of the rows, or row 0 and, behind it, the groups'
+// statistics and the channels' constants.  Backward: the sums of the rows; or row 0, the weighted sums and the groups' means.
+constexpr size_t LDS_MOST = 160 * 1024;
+
+size_t one_lds(const GnDims &d, int dtype, bool backward)
+{
+    const int n = vector_of(dtype);
+    const size_t groups = d.cs / d.gc, channels = (size_t)d.cv * n;
+    if (backward) {
+        const size_t sums = d.rows * channels, after = 2 * channels + groups;
+        return (sums > after ? sums : after) * 2 * sizeof(float);
+    }
+    const size_t units = d.c % n == 0 && d.gc % n == 0 ? d.cv : channels;         // vector_units
+    const size_t sums = d.rows * units * 2 * sizeof(double);
+    const size_t after = (units + groups) * 2 * sizeof(double) + d.cs * sizeof(Channel);
+    return (groups + 3) / 4 * 16 + (sums > after ? sums : after);
+}
+
 // The one-launch form: MAX_THREADS a workgroup, at most `most` vectors a thread.  A slab is the fewest whole groups that
 // make whole vectors and a wanted width: the widest of 1 KB ... 64 bytes a pixel that gives every compute unit a
 // workgroup, else 64 bytes.  Narrower ones, 32 and 16 bytes, read parts of cache lines and are for maps that are in the
 // caches anyway; larger maps that fit no other slab take the two-pass form.  us forward and backward, this rule / at most
 // 64 bytes always: 2048 of (256, 3, 3) 47 / 299, 64 of (256, 25, 38) 118 / 124; this rule / narrow slabs for any size:
 // 64 of (256, 50, 50) fp32 232 / 333, bf16 172 / 373, (256, 50, 50) 24.0 / 27.3; narrow slabs / this rule without them:
-// (256, 25, 38) fp32 16.2 / 20.3, bf16 16.2 / 30.1.  false: the map is too large for any.
+// (256, 25, 38) fp32 16.2 / 20.3, bf16 16.2 / 30.1.  false: the map is too large for any, or only a slab of thousands of
+// groups has whole vectors (a group a channel, a prime number of them) and their constants do not fit LDS.
 constexpr int ONE_MOST = 16, GRAD_ONE_MOST = 8;
 constexpr double NARROW_MOST = 1.5e6;                     // bytes
 
-bool one_launch(GnDims &d, int b, int dtype, int most)
+bool one_launch(GnDims &d, int b, int dtype, bool backward)
 {
     const int n = vector_of(dtype);
     const bool whole = d.c % n == 0;
+    int most = backward ? GRAD_ONE_MOST : ONE_MOST;
     if (!whole)
         most = 4;                                         // a vector of scalar loads is n registers
     const bool narrow = (double)b * d.c * d.hw * (16 / n) <= NARROW_MOST;
@@ -922,10 +942,14 @@ bool one_launch(GnDims &d, int b, int dtype, int most)
         const int rows = MAX_THREADS / cv;
         if (d.hw > (long long)rows * most)
             continue;
+        GnDims slab = d;
+        slab.cs = cs;
+        slab.cv = cv;
+        slab.rows = rows < d.hw ? rows : (int)d.hw;
+        if (one_lds(slab, dtype, backward) > LDS_MOST)
+            continue;
         fits = true;
-        d.cs = cs;
-        d.cv = cv;
-        d.rows = rows < d.hw ? rows : (int)d.hw;
+        d = slab;
         if (enough)
             break;
     }
@@ -973,8 +997,8 @@ extern "C" int64_t dance_group_norm_workspace_bytes(int b, int c, int64_t hw, in
         return 0;
     GnDims d = dims_of(b, c, hw, groups, dtype), one = d;
     if (!backward)
-        return one_launch(one, b, dtype, ONE_MOST) ? 0 : (int64_t)b * d.nch * groups * 2 * sizeof(double);
-    if (one_launch(one, b, dtype, GRAD_ONE_MOST))
+        return one_launch(one, b, dtype, false) ? 0 : (int64_t)b * d.nch * groups * 2 * sizeof(double);
+    if (one_launch(one, b, dtype, true))
         return b == 1 ? 0 : (int64_t)b * c * 2 * sizeof(double);
     return (int64_t)(whole_16((size_t)b * d.nch * c * 2 * sizeof(float)) + (size_t)b * c * 2 * sizeof(double) +
                      (size_t)b * groups * sizeof(float2));
@@ -1012,17 +1036,10 @@ extern "C" int dance_group_norm_act(const void *x, int64_t image_stride, int64_t
     return with_type(dtype, c % vector_of(dtype) == 0, [&](auto t, auto whole) {
         using T = decltype(t);
         constexpr bool W = decltype(whole)::value;
-        const bool vu = W && d.gc % Vec<T>::N == 0;
-        if (one_launch(d, b, dtype, ONE_MOST)) {
+        if (one_launch(d, b, dtype, false)) {
             auto one = [&](auto u) {
                 constexpr int U = decltype(u)::value;
-                const int units = vu ? d.cv : d.cv * Vec<T>::N;
-                // the groups' pivots; the sums of the rows, or row 0 and, behind it, the groups' statistics and the channels'
-                // constants
-                const size_t sums = (size_t)d.rows * units * 2 * sizeof(double);
-                const size_t after = ((size_t)units + d.cs / d.gc) * 2 * sizeof(double) + d.cs * sizeof(Channel);
-                const size_t pivots = (size_t)(d.cs / d.gc + 3) / 4 * 16;
-                const size_t lds = pivots + (sums > after ? sums : after);
+                const size_t lds = one_lds(d, dtype, false);
                 if (int rc = dance::allow_lds((const void *)k_gn_one<T, W, U>, lds, fn))
                     return rc;
                 hipLaunchKernelGGL((k_gn_one<T, W, U>), dim3((unsigned)(b * (c / d.cs))), dim3(MAX_THREADS), lds, st,
@@ -1036,6 +1053,7 @@ extern "C" int dance_group_norm_act(const void *x, int64_t image_stride, int64_t
             return one(std::integral_constant<int, 4>{});
         }
         double *partial = (double *)ws;
+        const bool vu = W && d.gc % Vec<T>::N == 0;
         const size_t lds = (size_t)d.rows * d.cv * (vu ? 1 : Vec<T>::N) * 2 * sizeof(double);
         if (int rc = dance::allow_lds((const void *)k_gn_stats<T, W>, lds, fn))
             return rc;
@@ -1089,13 +1107,10 @@ extern "C" int dance_group_norm_act_backward(const void *dy, int64_t dy_image_st
     return with_type(dtype, c % vector_of(dtype) == 0, [&](auto t, auto whole) {
         using T = decltype(t);
         constexpr bool W = decltype(whole)::value;
-        if (one_launch(d, b, dtype, GRAD_ONE_MOST)) {
+        if (one_launch(d, b, dtype, true)) {
             auto one = [&](auto u) {
                 constexpr int U = decltype(u)::value;
-                const int units = d.cv * Vec<T>::N;
-                // the sums of the rows; or row 0, the weighted sums and the groups' means
-                const size_t sums = (size_t)d.rows * units, after = 2 * (size_t)units + d.cs / d.gc;
-                const size_t lds = (sums > after ? sums : after) * 2 * sizeof(float);
+                const size_t lds = one_lds(d, dtype, true);
                 if (int rc = dance::allow_lds((const void *)k_gn_grad_one<T, W, U>, lds, fn))
                     return rc;
                 hipLaunchKernelGGL((k_gn_grad_one<T, W, U>), dim3((unsigned)(b * (c / d.cs))), dim3(MAX_THREADS), lds, st,

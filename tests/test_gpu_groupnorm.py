@@ -479,3 +479,19 @@ def test_any_mean_and_any_first_value(device, shape, groups, mean, spread, first
             "dweight": (dy.double().abs() * each).sum((0, 2, 3)), "dbias": 0.0}
     for name, got in (("y", y), ("dx", dx), ("dweight", dw), ("dbias", db)):
         _check(got, (want[name][0], want[name][1] + more[name]), name)
+
+
+@pytest.mark.parametrize("shape,groups", [((1, 4093, 2, 2), 4093), ((300, 4072, 1), 4072), ((1, 4078, 2, 2), 2039),
+                                          ((2, 4096, 3, 1), 4096), ((2, 4095, 2), 9)])
+def test_thousands_of_groups(device, shape, groups):
+    """groups of a channel or two, as many as there can be"""
+    x = _map(shape, torch.bfloat16, device, 40).requires_grad_(True)
+    w, be = _affine(shape[1], torch.float32, device, 40)
+    w.requires_grad_(True)
+    be.requires_grad_(True)
+    dy = _map(shape, torch.bfloat16, device, 41)
+    y = ops.group_norm_act(x, groups, w, be, act="silu")
+    got = (y,) + torch.autograd.grad(y, (x, w, be), dy)
+    want = _oracle(x, groups, w, be, "silu", dy)
+    for name, value in zip(("y", "dx", "dweight", "dbias"), got):
+        _check(value, want[name], name)

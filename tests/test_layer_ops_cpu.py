@@ -51,6 +51,13 @@ def test_group_norm_workspace():
         assert _norm(ws=fake, ws_bytes=need - 1, **big) == BAD and _norm(ws=None, ws_bytes=need, **big) == BAD
 
 
+@pytest.mark.parametrize("b,c,hw,groups", [(1, 4093, 4, 4093), (300, 4072, 1, 4072), (1, 4078, 4, 2039)])
+def test_group_norm_of_thousands_of_groups(b, c, hw, groups):
+    """no slab of them fits a compute unit's LDS with its groups' statistics and channels' constants: the form of three
+    launches, which has a workspace"""
+    assert _lib.lib().dance_group_norm_workspace_bytes(b, c, hw, groups, 2, 0) >= b * groups * 16
+
+
 def test_group_norm_needs_a_gpu_tensor():
     with pytest.raises(RuntimeError, match="GPU tensors"):
         ops.group_norm_act(torch.zeros((1, 8, 2, 2)), 2)
