@@ -8,6 +8,7 @@ import math
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import (ACT_NONE, ACT_RELU, ACT_SILU, ABSMAX_OF_FEATURES, ABSMAX_OF_GN_RELU, ABSMAX_OF_LAYOUT, ABSMAX_WORDS, DTYPE_BF16,
                    DTYPE_F16, DTYPE_F32, check, current_stream, lib, on_device, ptr, stream_of)
@@ -22,6 +23,13 @@ def _need_gpu(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise RuntimeError("dance_amd ops need GPU tensors (got a %s tensor)" % t.device)
+
+
+def _no_tangents(what, *tensors):
+    """The operators with gradients of their own have no forward-mode ones: a dual tensor is refused, its tangent would
+    be dropped without a word."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("%s has no forward-mode derivative: call it on tensors without tangents" % what)
 
 
 def _f32c(t):
@@ -615,9 +623,10 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="relu"):
 
     x (B, C, *spatial) fp32 / fp16 / bf16 with adjacent channels (torch.channels_last memory, a channel slice
     of it, or a (B, C) matrix); a map whose pixels are not evenly spaced (a crop) is copied first, a
-    channels-first map is refused.  weight, bias (C) of one type, or None; act None, "relu" or "silu".  The
+    channels-first map is refused, so is one with a tangent (forward mode).  weight, bias (C) of one type, or None; act None, "relu" or "silu".  The
     statistics cover the whole map as F.group_norm's do, in fp64.  Returns y of x's type, channels last."""
     _need_gpu(x, weight, bias)
+    _no_tangents("group_norm_act", x, weight, bias)
     if x.dim() < 2:
         raise RuntimeError("group_norm_act: (B, C, *spatial) expected, got %d dimension(s)" % x.dim())
     if x.dtype not in DTYPE_CODES:
@@ -673,6 +682,7 @@ def orthogonalize(x, steps=5, eps=1e-7, coefficients=NS_COEFFICIENTS):
     coefficients have to keep singular values below 2.  Returns a dense tensor of x's shape and type; not
     differentiable (call it on a detached tensor or under no_grad)."""
     _need_gpu(x)
+    _no_tangents("orthogonalize", x)
     steps, eps, (a, b, c) = check_newton_schulz("orthogonalize", steps, eps, coefficients)
     if x.dim() < 2 or x.dtype not in DTYPE_CODES:
         raise RuntimeError("orthogonalize: (..., m, n) fp32, fp16 or bf16 expected, got %s %s" % (tuple(x.shape), x.dtype))

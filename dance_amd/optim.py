@@ -14,7 +14,7 @@ import threading
 import torch
 
 from ._lib import MuonItemStruct, check, lib, on_device, ptr, stream_of
-from .ops import DTYPE_CODES, MOST_ELEMENTS, NS_COEFFICIENTS, _need_gpu, _scratch, check_newton_schulz
+from .ops import DTYPE_CODES, MOST_ELEMENTS, NS_COEFFICIENTS, _need_gpu, _no_tangents, _scratch, check_newton_schulz
 
 
 NARROW_ROWS = 128           # up to so many rows (of the smaller side) a step of the chain is a launch of its own
@@ -70,6 +70,7 @@ def muon_step(params, grads, momentum_buffers, *, lr, momentum=0.95, nesterov=Tr
     if not len(params) == len(grads) == len(momentum_buffers):
         raise RuntimeError("%s: %d params, %d grads, %d momentum buffers"
                            % (what, len(params), len(grads), len(momentum_buffers)))
+    _no_tangents(what, *params, *grads, *momentum_buffers)
     # checked a property at a time over the lists, which takes Python a third of the time of a matrix at a time
     shapes, dtypes, places = ([t.shape for t in params], [t.dtype for t in params], [t.get_device() for t in params])
     for other in (grads, momentum_buffers):

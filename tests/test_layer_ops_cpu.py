@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from dance_amd import _lib, ops
+from dance_amd import _lib, ops, optim
 
 BAD = 1                                                    # hipErrorInvalidValue
 
@@ -248,4 +248,29 @@ def test_group_norm_backward_refuses_other_saved_tensors(on_cpu, unpack):
         y = ops.group_norm_act(x, 4, torch.ones(8, requires_grad=True))
         with pytest.raises(RuntimeError, match="saved-tensor hook"):
             y.backward(torch.ones_like(y))
+    assert not on_cpu.called
+
+
+def test_tangents_are_refused(on_cpu, monkeypatch):
+    """forward-mode derivatives: dual tensors, and those that torch.func.jvp makes"""
+    x, t = _slice((2, 8, 4, 5), 0), torch.ones((2, 8, 4, 5))
+    w, tw = torch.ones(8), torch.ones(8)
+    monkeypatch.setattr(optim, "_need_gpu", lambda *tensors: None)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual
+        with torch.no_grad():
+            for args in ((dual(x, t), 4), (x, 4, dual(w, tw)), (x, 4, w, dual(w, tw))):
+                with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    ops.group_norm_act(*args)
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            ops.orthogonalize(dual(x, t))
+        for k in range(3):
+            lists = [[torch.ones((4, 6))] for _ in range(3)]
+            lists[k] = [dual(torch.ones((4, 6)), torch.ones((4, 6)))]
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                optim.muon_step(*lists, lr=0.1)
+        assert ops.group_norm_act(x, 4, w).shape == x.shape         # a level alone is no reason
+    for f in (lambda v: ops.group_norm_act(v, 4), ops.orthogonalize):
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            torch.func.jvp(f, (x,), (t,))
     assert not on_cpu.called
