@@ -136,7 +136,8 @@ def muon_step(params, grads, momentum_buffers, *, lr, momentum=0.95, nesterov=Tr
 
 class Muon(torch.optim.Optimizer):
     """torch.optim optimizer over muon_step.  Every parameter a matrix (two dimensions or more, the first one the
-    rows); parameters without a gradient are left as they are.  A step can be captured into a graph once every
+    rows); parameters without a gradient are left as they are.  A momentum buffer in another memory format than its
+    parameter's (a loaded state, a module converted after its first step) is laid out again.  A step can be captured into a graph once every
     momentum buffer exists; its replays keep the settings, lr among them, that it was captured with."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, eps=1e-7,
@@ -165,11 +166,17 @@ class Muon(torch.optim.Optimizer):
         for group in self.param_groups:
             params = [p for p in group["params"] if p.grad is not None]
             for p in params:
-                if "momentum_buffer" not in self.state[p]:
-                    if p.is_cuda and torch.cuda.is_current_stream_capturing():
-                        # (a replay would clear the buffer again)
-                        raise RuntimeError("Muon: take a step before the one that is captured into a graph")
+                held = self.state[p].get("momentum_buffer")
+                if held is not None and (held.stride() == p.stride() or held.shape != p.shape):
+                    continue
+                if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                    # (a replay would make the buffer again)
+                    raise RuntimeError("Muon: take a step before the one that is captured into a graph")
+                if held is None:
                     self.state[p]["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                else:                            # of a loaded state, or from before the module took another memory format
+                    self.state[p]["momentum_buffer"] = torch.empty_like(p, dtype=held.dtype, device=held.device,
+                                                                        memory_format=torch.preserve_format).copy_(held)
             muon_step(params, [p.grad for p in params], [self.state[p]["momentum_buffer"] for p in params],
                       **{k: v for k, v in group.items() if k in ("lr", "momentum", "nesterov", "weight_decay", "steps", "eps",
                                                                  "coefficients")})

@@ -548,3 +548,25 @@ def test_training_a_norm_layer_stack(device):
     _muon_check([c.weight.contiguous() for c in convs], [c.weight.grad.contiguous() for c in convs],
                 [opt.state[c.weight]["momentum_buffer"].contiguous() for c in convs],
                 [(p.contiguous(), m.contiguous()) for p, m in before], torch.float32, 0.05, 0.95, True, 0.0, "stack")
+
+
+def test_optimizer_state_of_another_memory_format(device):
+    """a state saved from contiguous weights carries on with channels_last ones"""
+    g = torch.Generator().manual_seed(77)
+    shape = (48, 20, 3, 3)
+    start, grads = torch.randn(shape, generator=g), [torch.randn(shape, generator=g).to(device) for _ in range(3)]
+    p = torch.nn.Parameter(start.to(device))
+    opt = optim.Muon([p], lr=0.05)
+    p.grad = grads[0]
+    opt.step()
+    q = torch.nn.Parameter(p.detach().to(memory_format=torch.channels_last))
+    other = optim.Muon([q], lr=0.05)
+    other.load_state_dict(copy.deepcopy(opt.state_dict()))
+    for grad in grads[1:]:
+        before = [(q.detach().clone(), other.state[q]["momentum_buffer"].clone())]
+        p.grad = q.grad = grad
+        opt.step()
+        other.step()
+        _muon_check([q], [grad], [other.state[q]["momentum_buffer"]], before, torch.float32, 0.05, 0.95, True, 0.0, "loaded")
+    m, n = opt.state[p]["momentum_buffer"], other.state[q]["momentum_buffer"]
+    assert n.stride() == q.stride() != p.stride() and torch.equal(m, n)

@@ -274,3 +274,38 @@ def test_tangents_are_refused(on_cpu, monkeypatch):
         with pytest.raises(RuntimeError, match="no forward-mode derivative"):
             torch.func.jvp(f, (x,), (t,))
     assert not on_cpu.called
+
+
+def test_muon_lays_out_buffers_of_another_memory_format(monkeypatch):
+    """a state loaded from contiguous weights into channels_last ones, a module converted after its first step"""
+    taken = []
+    monkeypatch.setattr(optim, "muon_step", lambda params, grads, buffers, **settings: taken.extend(buffers))
+    shapes = [(8, 4, 3, 3), (8, 4, 1, 1), (6, 5)]
+
+    def optimizer(memory_format):
+        params = [torch.nn.Parameter(torch.zeros(s)) for s in shapes]
+        for p in params:
+            p.data = p.data.to(memory_format=memory_format) if p.dim() == 4 else p.data
+            p.grad = torch.zeros_like(p)
+        return optim.Muon(params), params
+
+    opt, params = optimizer(torch.contiguous_format)
+    opt.step()
+    with torch.no_grad():
+        for m in taken:
+            m.copy_(torch.arange(m.numel()).reshape(m.shape))
+    want = [m.clone() for m in taken]
+    other, others = optimizer(torch.channels_last)
+    other.load_state_dict(opt.state_dict())
+    for p in params[:2]:
+        p.data = p.data.to(memory_format=torch.channels_last)
+        p.grad = torch.zeros_like(p)
+    for o, ps in ((other, others), (opt, params)):
+        taken.clear()
+        o.step()
+        assert [m.stride() for m in taken] == [p.stride() for p in ps]
+        assert all(torch.equal(m, v) for m, v in zip(taken, want))
+        held = list(taken)
+        taken.clear()
+        o.step()
+        assert all(m is h for m, h in zip(taken, held))
