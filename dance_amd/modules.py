@@ -81,7 +81,7 @@ class _ConvNormAct(nn.Conv2d):
     channels_last memory); anything else, `DANCE_FEATPREP=torch`, or `use_hip = False` runs
     the stock torch.nn ops.  With `DANCE_GROUPNORM=hip` the norm and the activation of that path run on
     ops.group_norm_act, in training mode and under autograd too, where the convolution's output is
-    channels_last."""
+    channels_last and no larger than that call takes; results are of the stock path's type, under autocast too."""
 
     use_hip = True
 
@@ -113,9 +113,11 @@ class _ConvNormAct(nn.Conv2d):
             if layer is not None:
                 return ops.bottom_out16(x, 0, [layer], groups=32, eps=self.norm.eps, measure=False).permute(0, 3, 1, 2)
         x = super().forward(x)
-        if (self.norm is not None and x.is_cuda and os.environ.get("DANCE_GROUPNORM", "torch") == "hip"
-                and ops.is_channels_last(x)):
-            return ops.group_norm_act(x, self.norm.num_groups, self.norm.weight, self.norm.bias, eps=self.norm.eps)
+        if self.norm is not None and x.is_cuda and os.environ.get("DANCE_GROUPNORM", "torch") == "hip":
+            # (the stock norm takes 16-bit maps in fp32 under autocast, and returns that)
+            wide = x.float() if x.dtype in (torch.float16, torch.bfloat16) and torch.is_autocast_enabled("cuda") else x
+            if ops.is_channels_last(wide):
+                return ops.group_norm_act(wide, self.norm.num_groups, self.norm.weight, self.norm.bias, eps=self.norm.eps)
         if self.norm is not None:
             x = self.norm(x)
         return F.relu(x)

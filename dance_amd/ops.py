@@ -525,8 +525,9 @@ def _channels_last_strides(t):
 
 
 def is_channels_last(t):
-    """Does group_norm_act read this GPU tensor in place?"""
-    return t.is_cuda and t.dim() >= 2 and t.dtype in DTYPE_CODES and _channels_last_strides(t) is not None
+    """Does group_norm_act take this GPU tensor, and read it in place?"""
+    return (t.is_cuda and t.dim() >= 2 and t.dtype in DTYPE_CODES and _channels_last_strides(t) is not None
+            and t.size(0) <= 65535 and t.size(1) * t.element_size() <= 8192)
 
 
 def _nhwc_view(t):

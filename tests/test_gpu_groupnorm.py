@@ -495,3 +495,35 @@ def test_thousands_of_groups(device, shape, groups):
     want = _oracle(x, groups, w, be, "silu", dy)
     for name, value in zip(("y", "dx", "dweight", "dbias"), got):
         _check(value, want[name], name)
+
+
+def test_conv_layers_under_autocast(device, monkeypatch):
+    """DANCE_GROUPNORM=hip returns the stock path's type: fp32, from the 16-bit output of the convolution"""
+    layer = modules._ConvNormAct(32, 64, 1, "GN").to(device).to(memory_format=torch.channels_last)
+    layer.use_hip = False
+    x = _map((2, 32, 9, 10), torch.float32, device, 50)
+    results = {}
+    for knob in ("torch", "hip"):
+        monkeypatch.setenv("DANCE_GROUPNORM", knob)
+        for dtype in (torch.float16, torch.bfloat16):
+            with torch.autocast("cuda", dtype=dtype):
+                results[knob, dtype] = layer(x)
+    with torch.no_grad():
+        for dtype in (torch.float16, torch.bfloat16):
+            want, got = results["torch", dtype], results["hip", dtype]
+            assert got.dtype == want.dtype == torch.float32
+            conv = torch.nn.functional.conv2d(x.to(dtype), layer.weight.to(dtype), padding=1)
+            _check(got, _oracle(conv, 32, layer.norm.weight, layer.norm.bias, "relu")["y"], str(dtype))
+
+
+def test_conv_layers_of_more_channels_than_a_call_takes(device, monkeypatch):
+    """stay on the stock path"""
+    monkeypatch.setenv("DANCE_GROUPNORM", "hip")
+    layer = modules._ConvNormAct(4, 2080, 1, "GN").to(device).to(memory_format=torch.channels_last)
+    layer.use_hip = False
+    x = _map((1, 4, 5, 6), torch.float32, device, 51)
+    assert ops.is_channels_last(_map((1, 2048, 2, 2), torch.float32, device, 52))
+    assert ops.is_channels_last(_map((1, 4096, 2, 2), torch.bfloat16, device, 52))
+    assert not ops.is_channels_last(_map((1, 2052, 2, 2), torch.float32, device, 52))
+    assert not ops.is_channels_last(_map((70000, 4), torch.float32, device, 52))
+    assert layer(x).shape == (1, 2080, 5, 6)
