@@ -190,14 +190,20 @@ __device__ __forceinline__ void add_word(double (&s)[Vec<T>::N], double (&q)[Vec
     }
 }
 
-// pixel0: the slab's first channel of pixel 0
+// pixel0: the slab's first channel of pixel 0.  A load a channel, behind the batch of vectors that the sums start with;
+// sharing the groups' pivots through LDS instead was no faster (statistics of (3, 96, 67, 101) fp16, groups of 3, 7.4
+// against 8.0 us, of (1, 256, 200, 304) bf16 10.5 against 10.1; k_gn_one 7.0 against 6.8).
 template <typename T, bool WHOLE>
 __device__ __forceinline__ void load_pivots(double (&pivot)[Vec<T>::N], const T *pixel0, const GnDims &d, int v)
 {
     const bool vu = vector_units<T, WHOLE>(d);
+    int first = channel_of<T, WHOLE>(d, v, 0) / d.gc * d.gc;                   // of the group
 #pragma unroll
-    for (int j = 0; j < Vec<T>::N; ++j)
-        pivot[j] = vu && j > 0 ? pivot[0] : (double)(float)pixel0[min(channel_of<T, WHOLE>(d, v, j), d.cs - 1) / d.gc * d.gc];
+    for (int j = 0; j < Vec<T>::N; ++j) {
+        const int c = min(channel_of<T, WHOLE>(d, v, j), d.cs - 1);
+        first = !WHOLE ? c / d.gc * d.gc : c == first + d.gc ? c : first;
+        pivot[j] = vu && j > 0 ? pivot[0] : (double)(float)pixel0[first];
+    }
 }
 
 // A thread's sums into red [rows][units].

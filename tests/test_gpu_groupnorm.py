@@ -10,6 +10,7 @@ thread at these sizes) and a tree above them, so a sum is off by at most (N_T + 
 magnitudes.  On top comes half a step of the output's type."""
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from dance_amd import modules, ops
 
@@ -527,3 +528,21 @@ def test_conv_layers_of_more_channels_than_a_call_takes(device, monkeypatch):
     assert not ops.is_channels_last(_map((1, 2052, 2, 2), torch.float32, device, 52))
     assert not ops.is_channels_last(_map((70000, 4), torch.float32, device, 52))
     assert layer(x).shape == (1, 2080, 5, 6)
+
+
+def test_checkpointed(device):
+    """torch.utils.checkpoint gives back tensors of a second forward call: the same bits as without it"""
+    x = _map((2, 40, 21, 23), torch.float32, device, 60)[:, 4:36].requires_grad_(True)
+    w, be = _affine(32, torch.float32, device, 60)
+    w.requires_grad_(True)
+    be.requires_grad_(True)
+    dy = _map((2, 32, 21, 23), torch.float32, device, 61)
+
+    def layer(t):
+        return ops.group_norm_act(ops.group_norm_act(t, 8, w, be), 4, w, be, act="silu")
+
+    y = layer(x)
+    want = (y.detach(),) + torch.autograd.grad(y, (x, w, be), dy)
+    y = torch.utils.checkpoint.checkpoint(layer, x, use_reentrant=False)
+    got = (y.detach(),) + torch.autograd.grad(y, (x, w, be), dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
