@@ -278,7 +278,7 @@ template <int FL, typename F> __device__ __forceinline__ void for_batch(long lon
 }
 
 // partial (b, nch, groups, 2): sums of a chunk of pixels.  grid: b * nch workgroups, slab = the whole map.  Bound by
-// memory: (8, 256, 200, 304) fp32 86 us (5.8 TB/s), (1, 256, 200, 304) bf16 10 us (3.1 TB/s, start and reduction show).
+// memory: (8, 256, 200, 304) fp32 86 us (5.8 TB/s), (1, 256, 200, 304) bf16 10.5 us (3.0 TB/s, start and reduction show).
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(MAX_THREADS) void k_gn_stats(const T *__restrict__ x, long long image_stride,
                                                    long long pixel_stride, double *__restrict__ partial, GnDims d)
@@ -463,7 +463,7 @@ __global__ __launch_bounds__(MAX_THREADS) void k_gn_apply(const T *__restrict__ 
 }
 
 // Small maps: a workgroup owns a slab of whole groups of an image over all its pixels, at most U vectors a
-// thread, and keeps them in registers: one read, one launch.  grid: b * slabs.  (1, 256, 25, 38) fp32: 6.6 us, the trips
+// thread, and keeps them in registers: one read, one launch.  grid: b * slabs.  (1, 256, 25, 38) fp32: 6.8 us, the trips
 // to memory and the two reductions one after the other.
 template <typename T, bool WHOLE, int U>
 __global__ __launch_bounds__(MAX_THREADS) void k_gn_one(const T *__restrict__ x, long long image_stride, long long pixel_stride,
@@ -876,8 +876,8 @@ int threads_of(int cv) { return cv <= 256 ? 256 : MAX_THREADS; }
 
 // The two-pass form.  A workgroup takes 16 pixels a thread, so that its reduction is paid by enough reading, where that
 // still gives every compute unit a workgroup, else 8 or 4; no more than 2048 workgroups (eight a compute unit).  us of
-// statistics and apply pass with 16 / 8 pixels: (1, 256, 200, 304) bf16 10.0 + 12.9 / 10.9 + 15.4; with 8 / 4:
-// (3, 96, 67, 101) fp16 6.6 + 6.9 / 5.7 + 5.0.
+// statistics and apply pass with 16 / 8 pixels: (1, 256, 200, 304) bf16 10.5 + 12.5 / 12.2 + 14.9; with 8 / 4:
+// (3, 96, 67, 101) fp16 7.6 + 6.9 / 7.5 + 5.5.
 GnDims dims_of(int b, int c, long long hw, int groups, int dtype)
 {
     GnDims d;

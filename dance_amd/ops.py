@@ -679,9 +679,11 @@ def orthogonalize(x, steps=5, eps=1e-7, coefficients=NS_COEFFICIENTS):
     Muon optimizer does to an update): X = x / max(|x|_F, eps), then `steps` times A = X X',
     X <- a X + (b A + c A A) X, on the smaller side.
 
-    x (..., m, n) fp32 / fp16 / bf16, any strides; the products are fp32-accurate for every type.  The
-    coefficients have to keep singular values below 2.  Returns a dense tensor of x's shape and type; not
-    differentiable (call it on a detached tensor or under no_grad)."""
+    x (..., m, n) fp32 / fp16 / bf16, any strides; the products are fp32-accurate for every type, relative to the
+    matrix's norm: entries of X below 2^-39 are taken as zero (five steps never show it, twenty or more would raise
+    them).  The coefficients have to keep singular values below 2.  Where the chain does not fit a compute unit's LDS the
+    workspace is 512 to 1024 bytes a column for up to 128 rows, else 16 bytes an element, sides as multiples of 128.
+    Returns a dense tensor of x's shape and type; not differentiable (call it on a detached tensor or under no_grad)."""
     _need_gpu(x)
     _no_tangents("orthogonalize", x)
     steps, eps, (a, b, c) = check_newton_schulz("orthogonalize", steps, eps, coefficients)

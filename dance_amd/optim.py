@@ -1,4 +1,5 @@
-"""Muon: momentum SGD whose update is orthogonalised (ops.orthogonalize), for the weight matrices of the heads.
+"""Muon: momentum SGD whose update is orthogonalised (ops.orthogonalize), for the weight matrices of heads that are trained
+as torch modules (this package's own only infer).
 
 A parameter of more than two dimensions is its (first dimension, the rest) matrix: a convolution's weight is
 (out channels, in channels * taps).  Vectors (biases, norm weights) are not Muon's: give them to another

@@ -689,10 +689,13 @@ int dance_group_norm_act_backward(const void *dy, int64_t dy_image_stride, int64
  * dance_orthogonalize: of every matrix M (m, n) of a batch, out (batch, m, n) dense of x's type:
  *   X = M / max(|M|_F, eps), then `steps` times  A = X X',  X <- a X + (b A + c A A) X.
  * x: element strides >= 0 of the batch, the rows and the columns.  The products are fp32-accurate (split
- * halves, three f16 MFMAs each) for every type; out is rounded once.  Coefficients have to keep the
+ * halves, three f16 MFMAs each) for every type, entries of X below 2^-39 taken as zero (which shows after 20
+ * steps or more); out is rounded once.  Coefficients have to keep the
  * singular values below 2 (the usual 3.4445, -4.7750, 2.0315 stay below 1.21), or the result is not finite.
  * A matrix with a NaN or an infinity comes out NaN, a zero matrix zero.  m n <= 2^31 - 129.  ws:
- * dance_orthogonalize_workspace_bytes of 16-byte aligned scratch (0 for small matrices: NULL), nothing to clear. */
+ * dance_orthogonalize_workspace_bytes of 16-byte aligned scratch (0 for small matrices: NULL), nothing to clear: with
+ * both sides rounded up to multiples of 128 to r <= k, a matrix (of up to 48 at a time) takes at most 1024 k + 2^17
+ * bytes where r is 128, else 16 r k + 10 r r + 2^24 + 2^17. */
 int64_t dance_orthogonalize_workspace_bytes(int batch, int m, int n);
 int dance_orthogonalize(const void *x, int64_t batch_stride, int64_t row_stride, int64_t col_stride,
                         int dtype, void *out, int batch, int m, int n, int steps, float a, float b,

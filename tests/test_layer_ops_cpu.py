@@ -309,3 +309,14 @@ def test_muon_lays_out_buffers_of_another_memory_format(monkeypatch):
         taken.clear()
         o.step()
         assert all(m is h for m, h in zip(taken, held))
+
+
+@pytest.mark.parametrize("m,n", [(1, 10 ** 7), (8, 10 ** 6), (128, 1152), (100, 500), (65, 40000), (128, 128), (129, 129), (144, 1296),
+                                 (1024, 4096), (200, 500), (46000, 46000), (130, 16 * 10 ** 6), (4000, 300), (300, 10 ** 5)])
+def test_orthogonalize_workspace_as_documented(m, n):
+    size = _lib.lib().dance_orthogonalize_workspace_bytes
+    r, k = sorted((s + 127) // 128 * 128 for s in (m, n))
+    each = 1024 * k + 2 ** 17 if r == 128 else 16 * r * k + 10 * r * r + 2 ** 24 + 2 ** 17
+    for batch in (1, 3, 48, 1000):
+        assert size(batch, m, n) <= min(batch, 48) * each
+    assert size(1, m, n) >= (512 if r == 128 else 16 * r) * k
